@@ -7,7 +7,7 @@ keeps one path:
     attn_qk_append    q/gate split, head norms, rotation at the node's depth, K and V into the pages
     attn_tree         attention of every node over the cache and its own ancestors, gated
     gdn_tree          conv + delta rule of every node along its own path; the state is only read
-    gdn_tree_commit   state and conv window advanced along the path to the chosen leaf
+    gdn_tree_commit   state and conv window advanced along the path to the chosen leaf (the ring's phase stays)
     kv_tree_commit    the K and V rows of that path moved to consecutive positions
 
 `run` computes them in plain torch, or, with `own` set, through rapidllm_b200.ops.  Sizes are those
@@ -363,16 +363,19 @@ def _gdn_commit(s):
     weight = torch.where(on > 0, torch.exp(end - total), 0.0).float()
     new = torch.exp(end).float() * S + (k * weight).transpose(2, 3) @ u
     s["S"][slots] = torch.where((leaf >= 0).view(B, 1, 1, 1), new, S)
-    # the ring: position (phase + depth) mod 4 holds the newest input with that residue
+    # the window: the last four inputs up to the leaf, kept as a ring that starts at the slot's phase
     depth = torch.where(leaf >= 0, torch.gather(reach.sum(2), 1, leaf.clamp(min=0).unsqueeze(1)).squeeze(1).long(), 0)
-    at = (s["phase"][slots].long().unsqueeze(1) + reach.sum(2).long() - 1) % TAPS
-    keep = (on.view(B, n) > 0) & (leaf >= 0).unsqueeze(1) & (reach.sum(2).long() > depth.unsqueeze(1) - TAPS)
-    ring = s["ring"][slots]
-    hit = (at.unsqueeze(2) == torch.arange(TAPS, device="cuda")) & keep.unsqueeze(2)
-    newest = torch.gather(s["qkv"], 1, hit.long().argmax(1).unsqueeze(2).expand(-1, -1, ring.shape[1])).transpose(1, 2)
-    s["ring"][slots] = torch.where(hit.any(1).unsqueeze(1), newest, ring)
-    s["phase"][slots] = ((s["phase"][slots].long() + depth) % TAPS).to(torch.int32)
-    return [s["S"], s["ring"], s["phase"]]
+    step = torch.where(on.view(B, n) > 0, reach.sum(2).long(), -1)
+    age = depth.unsqueeze(1) + torch.arange(1 - TAPS, 1, device="cuda")                  # oldest first; <= 0: the old window's
+    hit = (step.unsqueeze(1) == age.unsqueeze(2)) & (age.unsqueeze(2) > 0)
+    fresh = torch.gather(s["qkv"], 1, hit.long().argmax(2).unsqueeze(2).expand(-1, -1, s["ring"].shape[1])).transpose(1, 2)
+    order = (s["phase"][slots].long().unsqueeze(1) + torch.arange(TAPS, device="cuda")) % TAPS
+    dim = s["ring"].shape[1]
+    past = torch.gather(s["ring"][slots], 2, order.unsqueeze(1).expand(-1, dim, -1))
+    kept = torch.gather(past, 2, (age + TAPS - 1).clamp(0, TAPS - 1).unsqueeze(1).expand(-1, dim, -1))
+    s["ring"][slots] = torch.zeros_like(past).scatter(2, order.unsqueeze(1).expand(-1, dim, -1),
+                                                      torch.where((age > 0).unsqueeze(1), fresh, kept))
+    return [s["S"], s["ring"]]
 
 
 def _kv_commit(s):
@@ -408,7 +411,7 @@ def run(state):
         if c["op"] == "gdn":
             return [ops.gdn_tree(*args, n_qk=c["n_qk"], n_nodes=s["n_nodes"], slot_ids=s["slots"], head_map=head_map, eps_l2=EPS, out=s["o"])]
         ops.gdn_tree_commit(*args, s["leaf"], n_qk=c["n_qk"], slot_ids=s["slots"], head_map=head_map, eps_l2=EPS)
-        return [s["S"], s["ring"], s["phase"]]
+        return [s["S"], s["ring"]]
     return {"append": _append, "attn": _attn, "gdn": _gdn, "gdn_commit": _gdn_commit, "kv_commit": _kv_commit}[s["case"]["op"]](s)
 
 
@@ -500,7 +503,7 @@ def _exact_gdn(s, parents, counts):
     c, dim = s["case"], s["qkv"].shape[2]
     qd, w = c["n_qk"] * DK, s["conv_w"].double()
     hs = torch.tensor([h % c["n_qk"] if c["tiled"] else h // (c["n_v"] // c["n_qk"]) for h in range(c["n_v"])], device="cuda")
-    S_all, ring_all, phase_all = s["S"].double() if c["op"] == "gdn_commit" else None, s["ring"].double(), s["phase"].clone()
+    S_all, ring_all = s["S"].double() if c["op"] == "gdn_commit" else None, s["ring"].double()
     o = torch.zeros(c["batch"], c["nodes"], c["n_v"], DK, dtype=torch.float64, device="cuda")
     for b in range(c["batch"]):
         slot = int(s["slots"][b])
@@ -532,7 +535,6 @@ def _exact_gdn(s, parents, counts):
         if c["op"] == "gdn_commit" and len(nodes):
             S, win = states[nodes[-1]]
             S_all[slot] = S
-            phase_all[slot] = (phase + len(nodes)) % TAPS
             for j in range(TAPS):
-                ring_all[slot][:, (int(phase_all[slot]) + j) % TAPS] = win[j]
-    return [o] if c["op"] == "gdn" else [S_all, ring_all, phase_all]
+                ring_all[slot][:, (phase + j) % TAPS] = win[j]
+    return [o] if c["op"] == "gdn" else [S_all, ring_all]
