@@ -408,6 +408,118 @@ int rl_delta_gates(const float* a, const float* b, const float* A_log, const flo
 
 
 /* ------------------------------------------------------------------------- */
+/* Trees of drafted tokens: append, verify, commit                            */
+/* ------------------------------------------------------------------------- */
+
+/* A draft proposes up to 64 tokens per sequence as a tree (several continuations of one token are
+ * siblings); one pass runs all of them through the mixers, then one path is kept.  The reference
+ * verifies chains only (Engine::spec_verify, include/rapidllm/runtime/cuda_engine.h:69-77;
+ * gdn_decode_tn_k, src/kernels/cuda/cuda_engine.cu:5289-5536); these calls generalise that.
+ *   parents   int32 [batch][max_nodes]: parents[i] is the node that node i continues, in [-1, i);
+ *             -1 = it continues the committed history.  NULL = a chain (parents[i] = i - 1)
+ *   n_nodes   int32 [batch], nodes of each sequence in [0, max_nodes]; NULL = max_nodes.  Rows behind
+ *             a sequence's last node are neither read nor written
+ *   leaf      int32 [batch], the last node of the path to keep, or -1 to keep none
+ * all on the device.  A parent, count or leaf out of its range is recorded like bad pages and slots
+ * (rl_device_error): the parent counts as -1, the count as 0, the leaf as -1.  The K and V rows of node i
+ * lie at cache position base_len + i until the commit; its rotary position is base_len + its depth.
+ * One verify round of a layer:
+ *   rl_attn_qk_append -> rl_attn_tree -> (choose the leaf) -> rl_kv_tree_commit,   or
+ *   rl_gdn_tree -> (choose the leaf) -> rl_gdn_tree_commit with the same inputs. */
+#define RL_TREE_MAX_NODES 64
+/* element types of q and o */
+enum { RL_TYPE_F32 = 0, RL_TYPE_F16 = 1, RL_TYPE_BF16 = 2 };
+
+typedef struct rl_attn_qk_append_params {
+    int n_q, n_kv, head_dim;     /* 24, 4, 256 */
+    int rotary_dim;              /* 64: a multiple of 16, <= head_dim */
+    int batch, n_tok;            /* sequences, rows per sequence */
+    int page_tokens, n_pages, max_pages_per_seq;
+    int q_type;                  /* RL_TYPE_* of q_out */
+    float theta, eps;            /* 1e7, 1e-6 */
+    long long qg_stride, k_stride, v_stride;   /* floats between rows (0 = dense), multiples of 4: q | gate, k
+                                                * and v may be column ranges of one projection */
+} rl_attn_qk_append_params;
+
+/* rl_attn_qk_prepare and rl_kv_append in one pass over the projections: q/gate split, head RMSNorm
+ * (1 + gamma) of q and k, rotation of the first rotary_dim dims, K and V rows (fp16, round to nearest
+ * even) into the paged F16 cache at positions pos[b] + t.  Row t of sequence b is rotated by pos[b] + t,
+ * or, with parents (n_tok <= 64), by pos[b] + depth of node t.  The rotation's angle is formed in 64 bits
+ * (rl_attn_qk_prepare follows the reference's fp32 angle, which is 4e-3 rad off at position 100 000).
+ *   qg fp32 [batch * n_tok] rows of [n_q][2 * 256] ([q | gate] per head); k, v fp32 rows of [n_kv][256]
+ *   q_norm, k_norm fp32 [256] or NULL;  q_out [batch * n_tok][n_q][256] of q_type
+ *   gate_out fp32 [batch * n_tok][n_q][256], or NULL: not copied (rl_attn_tree reads it in place)
+ * k is only read.  A row whose page is bad keeps its q_out; its K and V are left out. */
+int rl_attn_qk_append(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* pos,
+                      const int32_t* parents, const int32_t* n_nodes, const float* qg, const float* k,
+                      const float* v, const float* q_norm, const float* k_norm, void* q_out, float* gate_out,
+                      const rl_attn_qk_append_params* p, void* stream);
+
+typedef struct rl_attn_tree_params {
+    int n_q, n_kv, head_dim;     /* 24, 4, 256; n_q / n_kv <= 8 */
+    int batch, max_nodes;        /* sequences, rows per sequence in q and o (<= 64) */
+    int page_tokens, n_pages, max_pages_per_seq;
+    int max_seq_len;             /* host-side upper bound of every base_len[b] + n_nodes[b] (sizing only) */
+    int q_type;                  /* RL_TYPE_* of q */
+    int o_type;                  /* RL_TYPE_F16 or RL_TYPE_BF16 */
+    long long gate_row, gate_head;   /* floats between the gate's rows and heads (0 = dense), multiples of 4 */
+} rl_attn_tree_params;
+
+/* Scratch for these parameters on the current device; 0 with a message when they are refused. */
+size_t rl_attn_tree_workspace_bytes(const rl_attn_tree_params* p);
+
+/* rl_attn_decode for every node of a tree: node i of sequence b attends to the cache rows [0, base_len[b])
+ * and to the rows base_len[b] + j of its ancestors j and itself (already appended), softmax scale 1/16,
+ * o *= sigmoid(gate) when gate != NULL.  With parents == NULL this is the causal verify of a ragged batch.
+ *   q [batch][max_nodes][n_q][256];  gate fp32, element (row, head, d) at row * gate_row + head * gate_head + d
+ *   o [batch][max_nodes][n_q][256] in 16 bits: a mean of fp16 values times a gate in (0, 1), it fits fp16,
+ *     and the probabilities meet V as fp16, so 32 bits would carry no more
+ * The V rows of all nodes of a sequence must be finite (one that is not reaches its siblings too); K rows
+ * may hold anything where they are not visible.  Reads only the F16 cache (RL_KV_F16). */
+int rl_attn_tree(const void* k_pool, const void* v_pool, const int32_t* page_table, const int32_t* base_len,
+                 const int32_t* parents, const int32_t* n_nodes, const void* q, const float* gate, void* o,
+                 void* workspace, size_t workspace_bytes, const rl_attn_tree_params* p, void* stream);
+
+typedef struct rl_kv_tree_commit_params {
+    int n_kv, head_dim;          /* 4, 256 */
+    int batch, max_nodes;
+    int page_tokens, n_pages, max_pages_per_seq;
+} rl_kv_tree_commit_params;
+
+/* Keep one path of each sequence: the K and V rows of its nodes move to positions base_len[b],
+ * base_len[b] + 1, ...  n_accept int32 [batch] or NULL receives the length of each path (0 for leaf -1);
+ * the sequence then has base_len[b] + n_accept[b] tokens. */
+int rl_kv_tree_commit(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* base_len,
+                      const int32_t* parents, const int32_t* leaf, int32_t* n_accept,
+                      const rl_kv_tree_commit_params* p, void* stream);
+
+typedef struct rl_gdn_tree_params {
+    int n_v, n_qk, dk, dv;       /* 48, 16, 128, 128 */
+    int conv_k;                  /* 4 */
+    int batch, max_nodes, n_slots;
+    int head_map;                /* RL_HEADS_* */
+    float eps_l2;                /* 1e-6 */
+    long long qkv_stride;        /* floats between rows of qkv (0 = dense), a multiple of 4 */
+} rl_gdn_tree_params;
+
+/* rl_gdn_decode for every node of a tree, each along its own path: conv over the node, its ancestors and
+ * the slot's window, SiLU, l2 norms, delta rule; S and the windows are only read.
+ *   conv_window fp32 [n_slots][conv_dim][4] and conv_phase as in rl_gdn_decode, or conv_phase == NULL:
+ *               shifted windows, oldest tap first (rl_conv1d_update's state)
+ *   qkv fp32 [batch][max_nodes] rows of conv_dim channels;  beta, g_log fp32 [batch][max_nodes][n_v]
+ *   o   fp32 [batch][max_nodes][n_v][128] */
+int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
+                const int32_t* parents, const int32_t* n_nodes, const float* qkv, const float* conv_w,
+                const float* beta, const float* g_log, float* o, const rl_gdn_tree_params* p, void* stream);
+
+/* Keep one path: S and the conv window of each sequence's slot advance by the path's tokens, as that many
+ * decode steps would (the sums are in another order).  The window's entries move and conv_phase stays, so no
+ * rl_gdn_phase_advance follows.  The slots of a call must be distinct.  Takes rl_gdn_tree's inputs. */
+int rl_gdn_tree_commit(float* S, float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
+                       const int32_t* parents, const int32_t* leaf, const float* qkv, const float* conv_w,
+                       const float* beta, const float* g_log, const rl_gdn_tree_params* p, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Caches and the layer_types[] dispatch                                      */
 /* ------------------------------------------------------------------------- */
 

@@ -16,6 +16,8 @@ RL_KV_F16, RL_KV_Q8K_TQ3V = 0, 1
 RL_KV_POLICY_AUTO, RL_KV_POLICY_F16, RL_KV_POLICY_COMPACT = 0, 1, 2
 RL_LAYER_LINEAR_ATTENTION, RL_LAYER_FULL_ATTENTION = 0, 1
 RL_HEADS_PER_VALUE, RL_HEADS_GROUPED, RL_HEADS_TILED = 0, 1, 2
+RL_TYPE_F32, RL_TYPE_F16, RL_TYPE_BF16 = 0, 1, 2
+TREE_MAX_NODES = 64
 STATUS_NAMES = ["RL_OK", "RL_ERR_IO", "RL_ERR_FORMAT", "RL_ERR_NOMEM", "RL_ERR_UNSUPPORTED",
                 "RL_ERR_DEVICE", "RL_ERR_RANGE", "RL_ERR_INTERNAL"]
 
@@ -69,6 +71,28 @@ class Conv1dParams(C.Structure):
 class AttnQkPrepareParams(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_q", "n_kv", "head_dim", "rotary_dim", "rows", "pos0")] + [
         ("theta", C.c_float), ("eps", C.c_float)]
+
+
+class AttnQkAppendParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_q", "n_kv", "head_dim", "rotary_dim", "batch", "n_tok", "page_tokens", "n_pages",
+                                       "max_pages_per_seq", "q_type")] + [
+        ("theta", C.c_float), ("eps", C.c_float)] + [(n, C.c_longlong) for n in ("qg_stride", "k_stride", "v_stride")]
+
+
+class AttnTreeParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_q", "n_kv", "head_dim", "batch", "max_nodes", "page_tokens", "n_pages",
+                                       "max_pages_per_seq", "max_seq_len", "q_type", "o_type")] + [
+        ("gate_row", C.c_longlong), ("gate_head", C.c_longlong)]
+
+
+class KvTreeCommitParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_kv", "head_dim", "batch", "max_nodes", "page_tokens", "n_pages",
+                                       "max_pages_per_seq")]
+
+
+class GdnTreeParams(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_v", "n_qk", "dk", "dv", "conv_k", "batch", "max_nodes", "n_slots",
+                                       "head_map")] + [("eps_l2", C.c_float), ("qkv_stride", C.c_longlong)]
 
 
 class PlanInput(C.Structure):
@@ -172,6 +196,12 @@ SYMBOLS = {
     "rl_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, C.c_float, _vp]),
     "rl_cast_f32_to_bf16": (_i, [_vp, _vp, _sz, _vp]),
     "rl_delta_gates": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "rl_attn_qk_append": (_i, [_vp] * 13 + [C.POINTER(AttnQkAppendParams), _vp]),
+    "rl_attn_tree_workspace_bytes": (_sz, [C.POINTER(AttnTreeParams)]),
+    "rl_attn_tree": (_i, [_vp] * 10 + [_sz, C.POINTER(AttnTreeParams), _vp]),
+    "rl_kv_tree_commit": (_i, [_vp] * 7 + [C.POINTER(KvTreeCommitParams), _vp]),
+    "rl_gdn_tree": (_i, [_vp] * 11 + [C.POINTER(GdnTreeParams), _vp]),
+    "rl_gdn_tree_commit": (_i, [_vp] * 10 + [C.POINTER(GdnTreeParams), _vp]),
     "rl_cache_create": (_i, [C.POINTER(CacheConfig), C.POINTER(_vp)]),
     "rl_cache_destroy": (None, [_vp]),
     "rl_cache_bytes": (_sz, [_vp]),

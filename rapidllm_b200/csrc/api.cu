@@ -4,6 +4,7 @@
 #include "../../include/rl_b200.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -116,6 +117,10 @@ int dev_info(DevInfo** out) {
                                      int(rl::attn_prefill_smem_bytes())));
         RL_CUDA(cudaFuncSetAttribute(rl::attn_decode_tq_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      int(rl::attn_decode_tq_smem_bytes())));
+        RL_CUDA(cudaFuncSetAttribute(rl::attn_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     int(rl::attn_tree_smem_bytes())));
+        RL_CUDA(cudaFuncSetAttribute(rl::gdn_tree_kernel_ptr(), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     int(rl::gdn_tree_smem_bytes())));
         d.ready = true;
     }
     *out = &d;
@@ -633,6 +638,7 @@ const char* rl_device_error_string(int code) {
         case rl::DEV_ERR_WORKSPACE: return "more split-KV chunks than the workspace holds";
         case rl::DEV_ERR_BAD_SLOT: return "state slot outside the cache";
         case rl::DEV_ERR_BAD_LEN: return "sequence length or position outside the page table";
+        case rl::DEV_ERR_BAD_TREE: return "draft tree: parent, node count or leaf out of range";
         default: return "unknown device error";
     }
 }
@@ -1419,6 +1425,275 @@ int rl_conv1d_causal(const float* x, const float* w, float* y, float* state_io, 
 }
 
 // ------------------------------------------------------------------------------------
+// ---- trees of drafted tokens ----------------------------------------------------------------------
+
+static int tree_shape_check(int n_kv, int head_dim, int batch, int max_nodes, int page_tokens, int n_pages,
+                            int max_pages_per_seq) {
+    if (head_dim != rl::kHeadDim || page_tokens != rl::kPageTokens)
+        return fail(RL_ERR_UNSUPPORTED, "head_dim %d / page_tokens %d: only 256 / 64", head_dim, page_tokens);
+    if (n_kv <= 0 || n_kv > 65535 || batch < 0 || batch > 65535) return fail(RL_ERR_RANGE, "n_kv %d batch %d", n_kv, batch);
+    if (max_nodes < 0 || max_nodes > RL_TREE_MAX_NODES)
+        return fail(RL_ERR_RANGE, "%d nodes per sequence: at most %d", max_nodes, RL_TREE_MAX_NODES);
+    if (n_pages <= 0 || max_pages_per_seq <= 0 || max_pages_per_seq > 0x7fffffff / rl::kPageTokens)
+        return fail(RL_ERR_RANGE, "n_pages %d max_pages_per_seq %d", n_pages, max_pages_per_seq);
+    return RL_OK;
+}
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// the distance of a caller's rows: 0 = dense; else at least a row, in units that keep 16-byte loads aligned
+static bool row_stride(long long given, long long dense, size_t* out) {
+    *out = size_t(given ? given : dense);
+    return given == 0 || (given >= dense && given % 4 == 0);
+}
+
+int rl_attn_qk_append(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* pos, const int32_t* parents,
+                      const int32_t* n_nodes, const float* qg, const float* k, const float* v, const float* q_norm,
+                      const float* k_norm, void* q_out, float* gate_out, const rl_attn_qk_append_params* p, void* stream) {
+    if (!p) return fail(RL_ERR_RANGE, "params is NULL");
+    if (int st = tree_shape_check(p->n_kv, p->head_dim, p->batch, 0, p->page_tokens, p->n_pages, p->max_pages_per_seq)) return st;
+    if (p->n_q <= 0 || p->n_q > 65535 || p->n_tok < 0 || 1LL * p->batch * p->n_tok > 0x7fffffff)
+        return fail(RL_ERR_RANGE, "n_q %d batch %d n_tok %d", p->n_q, p->batch, p->n_tok);
+    if (parents && p->n_tok > RL_TREE_MAX_NODES)
+        return fail(RL_ERR_RANGE, "%d nodes per sequence: at most %d", p->n_tok, RL_TREE_MAX_NODES);
+    if (p->rotary_dim < 0 || p->rotary_dim > p->head_dim || p->rotary_dim % 16)
+        return fail(RL_ERR_RANGE, "rotary_dim %d must be a multiple of 16 and at most head_dim", p->rotary_dim);
+    if (p->rotary_dim > 0 && !(p->theta > 0.f)) return fail(RL_ERR_RANGE, "theta must be positive");
+    if (p->q_type != RL_TYPE_F32 && p->q_type != RL_TYPE_F16 && p->q_type != RL_TYPE_BF16)
+        return fail(RL_ERR_UNSUPPORTED, "q_type %d unknown", p->q_type);
+    rl::AttnQkAppendArgs a;
+    if (!row_stride(p->qg_stride, 2LL * p->n_q * rl::kHeadDim, &a.qg_stride) ||
+        !row_stride(p->k_stride, 1LL * p->n_kv * rl::kHeadDim, &a.k_stride) ||
+        !row_stride(p->v_stride, 1LL * p->n_kv * rl::kHeadDim, &a.v_stride))
+        return fail(RL_ERR_RANGE, "row strides %lld %lld %lld: at least a row, multiples of 4", p->qg_stride, p->k_stride, p->v_stride);
+    if (p->batch == 0 || p->n_tok == 0) return RL_OK;
+    if (!k_pool || !v_pool || !page_table || !pos || !qg || !k || !v || !q_out) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(qg) || !aligned16(k) || !aligned16(v) || !aligned16(q_norm) ||
+        !aligned16(k_norm) || !aligned16(q_out) || !aligned16(gate_out))
+        return fail(RL_ERR_RANGE, "pools, rows and norms must be 16-byte aligned");
+    DevInfo* d;
+    if (int st = dev_info(&d)) return st;
+    a.k_pool = static_cast<__half*>(k_pool);
+    a.v_pool = static_cast<__half*>(v_pool);
+    a.page_table = page_table;
+    a.pos = pos;
+    a.parents = parents;
+    a.n_nodes = n_nodes;
+    a.qg = qg;
+    a.k = k;
+    a.v = v;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.q_out = q_out;
+    a.gate_out = gate_out;
+    a.err = d->err_ptr;
+    a.n_q = p->n_q;
+    a.n_kv = p->n_kv;
+    a.n_tok = p->n_tok;
+    a.n_pages = p->n_pages;
+    a.max_pages_per_seq = p->max_pages_per_seq;
+    a.rotary_dim = p->rotary_dim;
+    a.q_type = p->q_type;
+    a.eps = p->eps;
+    const int pairs = p->rotary_dim / 2;
+    for (int i = 0; i < pairs; ++i) a.inv_turn[i] = pow(double(p->theta), -double(i) / pairs) / 6.283185307179586476925;
+    rl::launch_attn_qk_append(a, p->batch, as_stream(stream));
+    RL_CUDA(cudaGetLastError());
+    return RL_OK;
+}
+
+static int attn_tree_check(const rl_attn_tree_params* p) {
+    if (!p) return fail(RL_ERR_RANGE, "params is NULL");
+    if (int st = tree_shape_check(p->n_kv, p->head_dim, p->batch, p->max_nodes, p->page_tokens, p->n_pages, p->max_pages_per_seq))
+        return st;
+    if (p->n_q <= 0 || p->n_q % p->n_kv != 0 || p->n_q / p->n_kv > 8)
+        return fail(RL_ERR_UNSUPPORTED, "n_q %d / n_kv %d: group must divide and be <= 8", p->n_q, p->n_kv);
+    if (p->batch > rl::attn_tree_max_batch()) return fail(RL_ERR_RANGE, "batch %d above %d", p->batch, rl::attn_tree_max_batch());
+    if (p->max_seq_len <= 0 || p->max_seq_len > p->max_pages_per_seq * p->page_tokens)
+        return fail(RL_ERR_RANGE, "max_seq_len %d outside (0, max_pages_per_seq*page_tokens]", p->max_seq_len);
+    if (p->q_type != RL_TYPE_F32 && p->q_type != RL_TYPE_F16 && p->q_type != RL_TYPE_BF16)
+        return fail(RL_ERR_UNSUPPORTED, "q_type %d unknown", p->q_type);
+    if (p->o_type != RL_TYPE_F16 && p->o_type != RL_TYPE_BF16)
+        return fail(RL_ERR_UNSUPPORTED, "o_type %d: only RL_TYPE_F16 and RL_TYPE_BF16", p->o_type);
+    const long long row_tiles = (1LL * p->max_nodes * (p->n_q / p->n_kv) + rl::attn_tree_rows() - 1) / rl::attn_tree_rows();
+    if (1LL * p->batch * p->n_kv * row_tiles * p->max_pages_per_seq > 0x3fffffff)
+        return fail(RL_ERR_RANGE, "batch %d, n_kv %d, max_pages_per_seq %d: too many pages in one call", p->batch, p->n_kv, p->max_pages_per_seq);
+    return RL_OK;
+}
+
+// One persistent CTA per SM, fewer when the batch has less than kTreeMinShare pages for each.  Two pages are
+// the least that lets both softmax groups work.
+static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 2);
+struct AttnTreePlan {
+    int grid;
+    size_t o_bytes, total_bytes;
+};
+static AttnTreePlan attn_tree_plan(const rl_attn_tree_params* p, int sms) {
+    AttnTreePlan pl;
+    const int rows = rl::attn_tree_rows();
+    const long long segs = 1LL * p->batch * p->n_kv * ((p->max_nodes * (p->n_q / p->n_kv) + rows - 1) / rows);
+    const long long units = segs * ceil_div(p->max_seq_len, p->page_tokens);
+    pl.grid = int(std::max(1LL, std::min(1LL * sms, (units + kTreeMinShare - 1) / kTreeMinShare)));
+    const size_t slots = size_t(pl.grid) + size_t(segs);
+    pl.o_bytes = align_up(slots * rows * rl::kHeadDim * sizeof(float), 256);
+    pl.total_bytes = pl.o_bytes + align_up(slots * rows * 2 * sizeof(float), 256);
+    return pl;
+}
+
+size_t rl_attn_tree_workspace_bytes(const rl_attn_tree_params* p) {
+    if (attn_tree_check(p)) return 0;
+    DevInfo* d;
+    if (dev_info(&d)) return 0;
+    return attn_tree_plan(p, step_sms(d->sms)).total_bytes;
+}
+
+int rl_attn_tree(const void* k_pool, const void* v_pool, const int32_t* page_table, const int32_t* base_len,
+                 const int32_t* parents, const int32_t* n_nodes, const void* q, const float* gate, void* o, void* workspace,
+                 size_t workspace_bytes, const rl_attn_tree_params* p, void* stream) {
+    if (int st = attn_tree_check(p)) return st;
+    rl::AttnTreeArgs a;
+    const long long head = p->gate_head ? p->gate_head : rl::kHeadDim;
+    if (head < rl::kHeadDim || head % 4 || !row_stride(p->gate_row, head * p->n_q, &a.gate_row))
+        return fail(RL_ERR_RANGE, "gate strides %lld %lld: at least a row and a head, multiples of 4", p->gate_row, p->gate_head);
+    if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
+    if (!k_pool || !v_pool || !page_table || !base_len || !q || !o || !workspace) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (reinterpret_cast<uintptr_t>(k_pool) % 128 || reinterpret_cast<uintptr_t>(v_pool) % 128 || !aligned16(q) ||
+        !aligned16(gate) || !aligned16(o) || !aligned16(workspace))
+        return fail(RL_ERR_RANGE, "pools must be 128-byte aligned, q, gate, o and workspace 16-byte aligned");
+    DevInfo* d;
+    if (int st = dev_info(&d)) return st;
+    const AttnTreePlan pl = attn_tree_plan(p, step_sms(d->sms));
+    if (workspace_bytes < pl.total_bytes)
+        return fail(RL_ERR_RANGE, "workspace %zu bytes < %zu required", workspace_bytes, pl.total_bytes);
+    a.k_pool = static_cast<const __half*>(k_pool);
+    a.v_pool = static_cast<const __half*>(v_pool);
+    a.page_table = page_table;
+    a.base_len = base_len;
+    a.parents = parents;
+    a.n_nodes = n_nodes;
+    a.q = q;
+    a.gate = gate;
+    a.o = o;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.o_bytes);
+    a.err = d->err_ptr;
+    a.gate_head = size_t(head);
+    a.batch = p->batch;
+    a.max_nodes = p->max_nodes;
+    a.n_q = p->n_q;
+    a.n_kv = p->n_kv;
+    a.n_pages = p->n_pages;
+    a.max_pages_per_seq = p->max_pages_per_seq;
+    a.max_len = p->max_seq_len;
+    a.q_type = p->q_type;
+    a.o_type = p->o_type;
+    a.grid = pl.grid;
+    a.min_share = kTreeMinShare;
+    a.scale = 1.f / sqrtf(float(p->head_dim));
+    RL_CUDA(rl::launch_attn_tree(a, as_stream(stream)));
+    RL_CUDA(cudaGetLastError());
+    return RL_OK;
+}
+
+int rl_kv_tree_commit(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* base_len, const int32_t* parents,
+                      const int32_t* leaf, int32_t* n_accept, const rl_kv_tree_commit_params* p, void* stream) {
+    if (!p) return fail(RL_ERR_RANGE, "params is NULL");
+    if (int st = tree_shape_check(p->n_kv, p->head_dim, p->batch, p->max_nodes, p->page_tokens, p->n_pages, p->max_pages_per_seq))
+        return st;
+    if (p->batch == 0) return RL_OK;
+    if (!k_pool || !v_pool || !page_table || !base_len || !leaf) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(k_pool) || !aligned16(v_pool)) return fail(RL_ERR_RANGE, "pools must be 16-byte aligned");
+    DevInfo* d;
+    if (int st = dev_info(&d)) return st;
+    rl::KvTreeCommitArgs a;
+    a.k_pool = static_cast<__half*>(k_pool);
+    a.v_pool = static_cast<__half*>(v_pool);
+    a.page_table = page_table;
+    a.base_len = base_len;
+    a.parents = parents;
+    a.leaf = leaf;
+    a.n_accept = n_accept;
+    a.err = d->err_ptr;
+    a.n_kv = p->n_kv;
+    a.max_nodes = p->max_nodes;
+    a.n_pages = p->n_pages;
+    a.max_pages_per_seq = p->max_pages_per_seq;
+    rl::launch_kv_tree_commit(a, p->batch, as_stream(stream));
+    RL_CUDA(cudaGetLastError());
+    return RL_OK;
+}
+
+static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_window, const int32_t* conv_phase,
+                         const int32_t* slot_ids, const int32_t* parents, const float* qkv, const float* conv_w,
+                         const float* beta, const float* g_log, const rl_gdn_tree_params* p) {
+    if (!p) return fail(RL_ERR_RANGE, "params is NULL");
+    if (p->dk != 128 || p->dv != 128 || p->conv_k != 4)
+        return fail(RL_ERR_UNSUPPORTED, "dk %d dv %d conv_k %d: only 128 x 128, 4 taps", p->dk, p->dv, p->conv_k);
+    if (p->n_v <= 0 || p->n_v > 65535 || p->batch < 0 || p->batch > 65535 || p->n_slots <= 0)
+        return fail(RL_ERR_RANGE, "n_v %d batch %d n_slots %d", p->n_v, p->batch, p->n_slots);
+    if (p->head_map == RL_HEADS_PER_VALUE
+            ? p->n_qk != p->n_v
+            : (p->n_qk <= 0 || p->n_v % p->n_qk != 0 || p->head_map < 0 || p->head_map > RL_HEADS_TILED))
+        return fail(RL_ERR_RANGE, "n_qk %d does not fit n_v %d with head_map %d", p->n_qk, p->n_v, p->head_map);
+    if (p->max_nodes < 0 || p->max_nodes > RL_TREE_MAX_NODES)
+        return fail(RL_ERR_RANGE, "%d nodes per sequence: at most %d", p->max_nodes, RL_TREE_MAX_NODES);
+    a->conv_dim = 2 * p->n_qk * p->dk + p->n_v * p->dv;
+    if (!row_stride(p->qkv_stride, a->conv_dim, &a->x_stride))
+        return fail(RL_ERR_RANGE, "qkv_stride %lld: at least a row, a multiple of 4", p->qkv_stride);
+    if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
+    if (!S || !conv_window || !qkv || !conv_w || !beta || !g_log) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(S) || !aligned16(conv_window) || !aligned16(qkv) || !aligned16(conv_w))
+        return fail(RL_ERR_RANGE, "S, conv_window, qkv and conv_w must be 16-byte aligned");
+    DevInfo* d;
+    if (int st = dev_info(&d)) return st;
+    a->S = S;
+    a->conv = conv_window;
+    a->conv_phase = conv_phase;
+    a->slot_ids = slot_ids;
+    a->parents = parents;
+    a->x = qkv;
+    a->w = conv_w;
+    a->beta = beta;
+    a->g_log = g_log;
+    a->err = d->err_ptr;
+    a->batch = p->batch;
+    a->max_nodes = p->max_nodes;
+    a->n_v = p->n_v;
+    a->n_qk = p->n_qk;
+    a->n_slots = p->n_slots;
+    a->head_map = p->head_map;
+    a->eps_l2 = p->eps_l2;
+    return RL_OK;
+}
+
+int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
+                const int32_t* parents, const int32_t* n_nodes, const float* qkv, const float* conv_w, const float* beta,
+                const float* g_log, float* o, const rl_gdn_tree_params* p, void* stream) {
+    rl::GdnTreeArgs a = {};
+    if (int st = gdn_tree_args(&a, S, conv_window, conv_phase, slot_ids, parents, qkv, conv_w, beta, g_log, p)) return st;
+    if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
+    if (!o) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(o)) return fail(RL_ERR_RANGE, "o must be 16-byte aligned");
+    a.n_nodes = n_nodes;
+    a.o = o;
+    rl::launch_gdn_tree(a, as_stream(stream));
+    RL_CUDA(cudaGetLastError());
+    return RL_OK;
+}
+
+int rl_gdn_tree_commit(float* S, float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
+                       const int32_t* parents, const int32_t* leaf, const float* qkv, const float* conv_w, const float* beta,
+                       const float* g_log, const rl_gdn_tree_params* p, void* stream) {
+    rl::GdnTreeArgs a = {};
+    if (int st = gdn_tree_args(&a, S, conv_window, conv_phase, slot_ids, parents, qkv, conv_w, beta, g_log, p)) return st;
+    if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
+    if (!leaf) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    a.leaf = leaf;
+    a.S_out = S;
+    a.conv_out = conv_window;
+    RL_CUDA(rl::launch_gdn_tree_commit(a, as_stream(stream)));
+    RL_CUDA(cudaGetLastError());
+    return RL_OK;
+}
+
 int rl_plan_cache(const rl_plan_input* in, rl_plan_result* out) {
     if (!in || !out) return fail(RL_ERR_RANGE, "NULL argument");
     if (in->ctx <= 0 || in->max_batch <= 0 || in->page_tokens <= 0 || in->n_attn_layers < 0 || in->n_delta_layers < 0 ||

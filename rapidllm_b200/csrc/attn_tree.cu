@@ -1,0 +1,596 @@
+// Attention of a tree of drafted tokens over the paged F16 cache, for a ragged batch, on tcgen05 / TMEM.
+//
+//   o_i = sigmoid(gate_i) sum_t softmax_t(q_i . k_t / 16) v_t   over the rows t < base_len[b] of the cache
+//         and the rows base_len[b] + j of node i's ancestors j and its own
+//
+// All query rows of a KV head -- (node, query head of the group) pairs, up to 64 x 8 -- share its K and V,
+// so the 128 rows of an MMA tile are such pairs and a sequence's pages are read once per 128 rows (at 24 / 4
+// heads: once for up to 21 nodes).  Up to there the cache's bandwidth is the bound, beyond it the tensor
+// cores are.
+//
+// Work division: the (sequence, KV head, row tile, page) units of the whole batch form one list, computed on
+// the device from base_len and n_nodes (a captured step may advance them), and every CTA of a persistent
+// grid takes an equal contiguous share, cut into segments at (sequence, head, row tile) boundaries.  The
+// page ring runs on across segments.  A segment that holds all pages of its rows writes the output, the
+// others write (unnormalised o, max, sum) to slot `CTA + segment index`, distinct because a CTA's last
+// segment is the next one's first at most; attn_tree_merge_kernel joins them.
+//
+// Inside a segment: S = Q K^T (M 128, N 64) and O += P V (M 128, N 256) with Q, P, S and O in tensor memory
+// and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
+// 16 softmax warps in two groups take alternate pages, so that one page's exponentials run under the
+// other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
+// to fp16, as the cache's V is; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
+// its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.
+// Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
+// not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
+// rows past the last node are cleared for the same reason.
+#include "common.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+#include "tree.cuh"
+
+namespace rl {
+
+namespace {
+
+constexpr int kRows = 128;                        // MMA rows: (node, query head of the group)
+constexpr int kTile = kPageTokens;
+constexpr int kKStages = 3, kVStages = 3;
+constexpr int kSliceBytes = kPageTokens * kHeadDim * 2;
+constexpr int kGroupThreads = 256, kSoftmaxThreads = 512, kThreads = 608;
+constexpr int kWarpLoader = 16, kWarpQK = 17, kWarpPV = 18;
+constexpr uint32_t kTmemCols = 512;
+// tensor memory columns: S [0,64), two P buffers [64,128), O [128,384), Q (fp16 pairs) [384,512)
+constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kColQ = 384;
+constexpr float kRescaleThreshold = 8.f;          // log2 units
+constexpr float kNoMax = -1e30f;                   // of a row that has seen nothing; scores are below 2^8 * 65504 * 256
+constexpr int kMaxBatch = 512;
+
+struct Segment {
+    int b, h, rt, index;                          // index: running number of (b, h, rt)
+    int j0, n_tiles, n_all;                       // pages [j0, j0 + n_tiles) of n_all
+    int base, nodes;
+};
+
+// units and segments of the sequences before b; entry `batch` holds the totals
+struct Prefix {
+    int unit[kMaxBatch + 1], seg[kMaxBatch + 1];
+};
+
+struct Seq {
+    int base, nodes, tiles, row_tiles;
+};
+__device__ __forceinline__ Seq sequence(const AttnTreeArgs& a, int b, int* err) {
+    Seq q;
+    q.nodes = tree::node_count(a.n_nodes, b, a.max_nodes, err);
+    q.base = a.base_len[b];
+    if (q.base < 0 || (long long)q.base + q.nodes > a.max_len) {
+        set_err(err, DEV_ERR_BAD_LEN);
+        q.nodes = 0;
+    }
+    q.tiles = q.nodes ? (q.base + q.nodes + kTile - 1) / kTile : 0;
+    q.row_tiles = (q.nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
+    return q;
+}
+// one warp; every CTA computes the same table
+__device__ __forceinline__ void build_prefix(Prefix& p, const AttnTreeArgs& a, int lane, int* err) {
+    int units = 0, segs = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        int u = 0, g = 0;
+        if (b < a.batch) {
+            const Seq q = sequence(a, b, err);
+            g = a.n_kv * q.row_tiles;
+            u = g * q.tiles;
+        }
+        int su = u, sg = g;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, su, off), y = __shfl_up_sync(0xffffffffu, sg, off);
+            if (lane >= off) {
+                su += x;
+                sg += y;
+            }
+        }
+        if (b < a.batch) {
+            p.unit[b] = units + su - u;
+            p.seg[b] = segs + sg - g;
+        }
+        units += __shfl_sync(0xffffffffu, su, 31);
+        segs += __shfl_sync(0xffffffffu, sg, 31);
+    }
+    if (lane == 0) {
+        p.unit[a.batch] = units;
+        p.seg[a.batch] = segs;
+    }
+}
+// pages per CTA
+__device__ __forceinline__ int share_of(int units, const AttnTreeArgs& a) {
+    return max((units + a.grid - 1) / a.grid, a.min_share);
+}
+// the segment that starts at unit `pos` of a share that ends at `end`; b: a sequence at or before it
+__device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArgs& a, int pos, int end, int& b) {
+    while (p.unit[b + 1] <= pos) ++b;
+    Segment s;
+    const Seq q = sequence(a, b, nullptr);
+    const int in = pos - p.unit[b], hr = in / q.tiles;
+    s.b = b;
+    s.h = hr / q.row_tiles;
+    s.rt = hr - s.h * q.row_tiles;
+    s.index = p.seg[b] + hr;
+    s.j0 = in - hr * q.tiles;
+    s.n_all = q.tiles;
+    s.n_tiles = min(q.tiles - s.j0, end - pos);
+    s.base = q.base;
+    s.nodes = q.nodes;
+    return s;
+}
+
+struct Smem {
+    alignas(1024) unsigned char k[kKStages][kSliceBytes];
+    alignas(1024) unsigned char v[kVStages][kSliceBytes];
+    Prefix prefix;
+    uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+    uint64_t bar_s[2], bar_sfree[2], bar_p[2], bar_pv[2], bar_m[2], bar_q;
+    float xch[2][2][kRows][2];                    // [group][use parity] row maxima of the two column halves
+    float mrow[2][kRows];                         // [page parity] running row maximum, in units of S
+    alignas(16) float part[kRows][4];             // per row: the four threads' query maxima, later their sums
+    uint32_t tmem_base;
+    int failed;
+};
+
+__device__ __forceinline__ float sigmoid(float g) { return __frcp_rn(1.f + fast_exp2(g * -1.4426950408889634f)); }
+__device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
+    __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&b);
+}
+// 64 query values of type q_type from src, as floats
+__device__ __forceinline__ void load_q(float (&x)[64], const void* q, int q_type, size_t at) {
+    if (q_type == 0) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 f = __ldg(p + i);
+            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+        }
+    } else {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint4 w = __ldg(p + i);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = q_type == 1 ? __half22float2(*reinterpret_cast<const __half2*>(&u[e]))
+                                             : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]));
+                x[8 * i + 2 * e] = f.x;
+                x[8 * i + 2 * e + 1] = f.y;
+            }
+        }
+    }
+}
+// 32 outputs, gated, rounded to o_type
+__device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const float* gate, float (&o)[32]) {
+    if (gate) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 g = __ldcs(reinterpret_cast<const float4*>(gate + i));
+            o[i] *= sigmoid(g.x); o[i + 1] *= sigmoid(g.y); o[i + 2] *= sigmoid(g.z); o[i + 3] *= sigmoid(g.w);
+        }
+    }
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float* x = o + 8 * i;
+        dst[i] = a.o_type == 1 ? make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]))
+                               : make_uint4(pack_b2(x[0], x[1]), pack_b2(x[2], x[3]), pack_b2(x[4], x[5]), pack_b2(x[6], x[7]));
+    }
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) {
+    extern __shared__ unsigned char smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = a.n_q / a.n_kv;
+    griddep_launch();
+    if (warp == 0) build_prefix(s.prefix, a, lane, a.err);
+    if (tid == 32) {
+        for (int i = 0; i < kKStages; ++i) {
+            mbar_init(&s.k_full[i], 1);
+            mbar_init(&s.k_empty[i], 1);
+        }
+        for (int i = 0; i < kVStages; ++i) {
+            mbar_init(&s.v_full[i], 1);
+            mbar_init(&s.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.bar_s[i], 1);
+            mbar_init(&s.bar_sfree[i], kGroupThreads);
+            mbar_init(&s.bar_p[i], kGroupThreads);
+            mbar_init(&s.bar_pv[i], 1);
+            mbar_init(&s.bar_m[i], kGroupThreads);
+        }
+        mbar_init(&s.bar_q, kSoftmaxThreads);
+        s.failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == kWarpQK) tc::tmem_alloc(&s.tmem_base, kTmemCols);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = s.tmem_base;
+    const int units = s.prefix.unit[a.batch], share = share_of(units, a);
+    const int u_begin = int(min((long long)units, (long long)share * blockIdx.x)), u_end = min(units, u_begin + share);
+
+    if (warp == kWarpLoader) {
+        // ------------------------------ page loader ------------------------------
+        if (lane == 0) {
+            int b = 0, it = 0;
+            bool ok = true;
+            for (int pos = u_begin; pos < u_end && ok;) {
+                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+                pos += g.n_tiles;
+                const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq + g.j0;
+                for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
+                    const int ks = it % kKStages, vs = it % kVStages;
+                    int page = table[j];
+                    if (page < 0 || page >= a.n_pages) {
+                        set_err(a.err, DEV_ERR_BAD_PAGE);
+                        page = 0;
+                    }
+                    const size_t slice = (size_t(page) * a.n_kv + g.h) * kv_slice_elems();
+                    if (!mbar_wait(&s.k_empty[ks], ((it / kKStages) & 1) ^ 1)) { ok = false; break; }
+                    mbar_arrive_expect_tx(&s.k_full[ks], kSliceBytes);
+                    bulk_g2s(s.k[ks], a.k_pool + slice, kSliceBytes, &s.k_full[ks]);
+                    if (!mbar_wait(&s.v_empty[vs], ((it / kVStages) & 1) ^ 1)) { ok = false; break; }
+                    mbar_arrive_expect_tx(&s.v_full[vs], kSliceBytes);
+                    bulk_g2s(s.v[vs], a.v_pool + slice, kSliceBytes, &s.v_full[vs]);
+                }
+            }
+            if (!ok) {
+                set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+                s.failed = 1;
+            }
+        }
+    } else if (warp == kWarpQK) {
+        // ------------------------------ S = Q K^T issuer ------------------------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_qk = tc::idesc_f16(kRows, kTile, false, false);
+            uint64_t k_desc[kKStages];
+#pragma unroll
+            for (int i = 0; i < kKStages; ++i) k_desc[i] = tc::smem_desc(smem_u32(s.k[i]), 16, 1024);
+            const uint32_t q_tmem = tmem + kColQ, s_tmem = tmem + kColS;
+            int b = 0, it = 0, sg = 0;
+            bool ok = true;
+            for (int pos = u_begin; pos < u_end && ok; ++sg) {
+                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+                pos += g.n_tiles;
+                ok = mbar_wait(&s.bar_q, sg & 1);
+                for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
+                    const int st = it % kKStages;
+                    if (!mbar_wait(&s.k_full[st], (it / kKStages) & 1)) { ok = false; break; }
+                    // S is free once every thread of the group of the page before has read it out
+                    if (it >= 1 && !mbar_wait(&s.bar_sfree[(it - 1) & 1], ((it - 1) >> 1) & 1)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[2]);
+#pragma unroll
+                    for (int kk = 0; kk < 16; ++kk)
+                        tc::mma_ts(s_tmem, q_tmem + kk * 8, kd + uint64_t(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4),
+                                   idesc_qk, kk > 0);
+                    tc::commit(&s.k_empty[st]);
+                    tc::commit(&s.bar_s[it & 1]);
+                }
+            }
+            if (!ok) {
+                set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+                s.failed = 1;
+            }
+        }
+    } else if (warp == kWarpPV) {
+        // ------------------------------ O += P V issuer ------------------------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_pv = tc::idesc_f16(kRows, kHeadDim, false, true);
+            uint64_t v_desc[kVStages];
+#pragma unroll
+            for (int i = 0; i < kVStages; ++i) v_desc[i] = tc::smem_desc(smem_u32(s.v[i]), kTile * 128, 1024);
+            int b = 0, it = 0;
+            bool ok = true;
+            for (int pos = u_begin; pos < u_end && ok;) {
+                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+                pos += g.n_tiles;
+                for (int j = 0; j < g.n_tiles; ++j, ++it) {
+                    const int st = it % kVStages;
+                    if (!mbar_wait(&s.v_full[st], (it / kVStages) & 1)) { ok = false; break; }
+                    // P of a segment's first page is published after every thread has read the segment before's O
+                    if (!mbar_wait(&s.bar_p[it & 1], (it >> 1) & 1)) { ok = false; break; }
+                    tc::fence_after_sync();
+                    const uint64_t vd = st == 0 ? v_desc[0] : (st == 1 ? v_desc[1] : v_desc[2]);
+                    const uint32_t p_tmem = tmem + kColP + (it & 1) * 32;
+                    tc::mma_ts(tmem + kColO, p_tmem, vd, idesc_pv, j > 0);
+#pragma unroll
+                    for (int kk = 1; kk < 4; ++kk)
+                        tc::mma_ts(tmem + kColO, p_tmem + kk * 8, vd + uint64_t((kk * 16 * 128) >> 4), idesc_pv, 1);
+                    tc::commit(&s.v_empty[st]);
+                    tc::commit(&s.bar_pv[it & 1]);
+                }
+            }
+            if (!ok) {
+                set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+                s.failed = 1;
+            }
+        }
+    } else {
+        // ------------------------------ softmax warps ------------------------------
+        const int grp = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, quarter = warp >> 2;
+        const int r = quad * 32 + lane;                       // row of the tile = TMEM lane
+        const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {     // `ok` is the same in all lanes of a warp
+            if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+                set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+                ok = false;
+            }
+        };
+        int b = 0, it0 = 0;                                   // it0: pages of the segments before
+        for (int pos = u_begin; pos < u_end;) {
+            const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+            pos += g.n_tiles;
+            const int row = g.rt * kRows + r, node = row / G, hq = g.h * G + row - node * G;
+            const bool live = node < g.nodes;
+            const size_t flat = (size_t(g.b) * a.max_nodes + (live ? node : 0)) * a.n_q + hq;
+            // ---- Q -> tensor memory: 64 dims per thread, the row scaled to a largest magnitude in [128, 256) ----
+            float scale_log2 = a.scale * 1.4426950408889634f;
+            {
+                float x[64];
+                if (live) {
+                    load_q(x, a.q, a.q_type, flat * kHeadDim + quarter * 64);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) x[i] = 0.f;
+                }
+                float mx = 0.f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) mx = fmaxf(mx, fabsf(x[i]));
+                s.part[r][quarter] = mx;
+                named_bar_sync(9, kSoftmaxThreads);
+                const float4 m4 = *reinterpret_cast<const float4*>(s.part[r]);
+                mx = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+                const int e = int(__float_as_uint(mx) >> 23) - 127;
+                const int up = mx > 0.f && e < 128 ? min(max(7 - e, -120), 120) : 0;
+                const float f = __uint_as_float(uint32_t(127 + up) << 23);
+                scale_log2 *= __uint_as_float(uint32_t(127 - up) << 23);
+                uint32_t regs[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) regs[i] = pack_h2(x[2 * i] * f, x[2 * i + 1] * f);
+                tc::tmem_st32(lane_addr + kColQ + quarter * 32, regs);
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                mbar_arrive(&s.bar_q);
+            }
+            // ---- this row's visible nodes ----
+            unsigned long long seen = 0;
+            if ((g.j0 + g.n_tiles) * kTile > g.base) {        // the segment reaches the drafted rows
+                const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(g.b) * a.max_nodes : nullptr, g.nodes, lane, a.err);
+                seen = tree::of_node(w.lo, w.hi, node & 63);
+            }
+            const int last_pos = g.base + g.nodes - 1;
+            float m_known = kNoMax, l_part = 0.f;             // maxima are kept as the scores they are, unscaled
+            for (int j = (grp ^ it0) & 1; j < g.n_tiles; j += 2) {
+                const int it = it0 + j;                       // it & 1 == grp
+                const uint32_t par = (it >> 1) & 1;
+                wait(&s.bar_s[grp], par);
+                tc::fence_after_sync();
+                uint32_t raw[32];
+                if (ok) {
+                    tc::tmem_ld32(lane_addr + kColS + half * 32, raw);
+                    tc::tmem_wait_ld();
+                }
+                tc::fence_before_sync();
+                mbar_arrive(&s.bar_sfree[grp]);
+                const int tok0 = (g.j0 + j) * kTile;
+                if (last_pos + 1 - tok0 < kTile) {
+                    // V rows past the last node may hold anything (0 * NaN would poison O): clear them
+                    wait(&s.v_full[it % kVStages], (it / kVStages) & 1);
+                    const int first = last_pos + 1 - tok0;
+                    unsigned char* vt = s.v[it % kVStages];
+                    for (int idx = tid - grp * kGroupThreads; idx < (kTile - first) * 32; idx += kGroupThreads) {
+                        const int vr = first + (idx >> 5), c16 = idx & 31;
+                        *reinterpret_cast<uint4*>(vt + (c16 >> 3) * (kTile * 128) + vr * 128 + (c16 & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_async_smem();
+                }
+                float mx = kNoMax;
+                if (tok0 + kTile > g.base) {
+                    // bit i of `vis`: token tok0 + 32 half + i is committed, or a node that this row sees
+                    const int rel = tok0 + half * 32 - g.base;
+                    uint32_t vis;
+                    if (rel >= 0) vis = rel < 64 ? uint32_t(seen >> rel) : 0u;
+                    else vis = rel <= -32 ? 0xffffffffu : (uint32_t(seen << -rel) | ((1u << -rel) - 1));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (!(vis >> i & 1)) raw[i] = 0xff800000u;         // -inf
+                        mx = fmaxf(mx, __uint_as_float(raw[i]));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(raw[i]));
+                }
+                s.xch[grp][par][r][half] = mx;
+                named_bar_sync(1 + grp * 4 + quad, 64);
+                mx = fmaxf(mx, s.xch[grp][par][r][half ^ 1]);
+                float m_prev = kNoMax;
+                if (j > 0) {
+                    wait(&s.bar_m[grp ^ 1], ((it - 1) >> 1) & 1);
+                    m_prev = s.mrow[grp ^ 1][r];
+                }
+                float m_new = m_prev, alpha = 1.f;
+                if (mx > m_prev && (m_prev == kNoMax || (mx - m_prev) * scale_log2 > kRescaleThreshold)) {
+                    alpha = fast_exp2((m_prev - mx) * scale_log2);
+                    m_new = mx;
+                }
+                if (half == 0) s.mrow[grp][r] = m_new;
+                mbar_arrive(&s.bar_m[grp]);
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    wait(&s.bar_pv[grp ^ 1], ((it - 1) >> 1) & 1);         // O must not be in use
+                    tc::fence_after_sync();
+                    if (ok) {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < kHeadDim / 2; c0 += 32) {
+                            uint32_t o[32];
+                            tc::tmem_ld32(lane_addr + kColO + half * 128 + c0, o);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tc::tmem_st32(lane_addr + kColO + half * 128 + c0, o);
+                        }
+                        tc::tmem_wait_st();
+                    }
+                }
+                if (m_new != m_known) {
+                    l_part *= fast_exp2((m_known - m_new) * scale_log2);
+                    m_known = m_new;
+                }
+                // p = 2^((s - m) scale) as one FFMA and one EX2.  m scale is rounded, the same for the whole row; only
+                // where that rounding is itself a large exponent (|m scale| > 2^20) is the difference taken first.
+                float m_log2 = m_new == kNoMax ? 0.f : m_new * scale_log2;
+                if (__any_sync(0xffffffffu, fabsf(m_log2) > 1048576.f)) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) - m_new);
+                    m_log2 = 0.f;
+                }
+                uint32_t ph[16];
+                float lsum0 = 0.f, lsum1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p0 = fast_exp2(fmaf(__uint_as_float(raw[2 * i]), scale_log2, -m_log2));
+                    const float p1 = fast_exp2(fmaf(__uint_as_float(raw[2 * i + 1]), scale_log2, -m_log2));
+                    lsum0 += p0;
+                    lsum1 += p1;
+                    ph[i] = pack_h2(p0, p1);
+                }
+                l_part += lsum0 + lsum1;
+                if (it >= 2) wait(&s.bar_pv[grp], ((it - 2) >> 1) & 1);    // this P buffer's last reader
+                tc::fence_after_sync();
+                if (ok) {
+                    tc::tmem_st16(lane_addr + kColP + grp * 32 + half * 16, ph);
+                    tc::tmem_wait_st();
+                }
+                tc::fence_before_sync();
+                mbar_arrive(&s.bar_p[grp]);
+            }
+            // ---- end of the segment ----
+            it0 += g.n_tiles;
+            const int it_last = it0 - 1;
+            wait(&s.bar_m[it_last & 1], (it_last >> 1) & 1);
+            const float m_fin = s.mrow[it_last & 1][r];
+            s.part[r][quarter] = l_part * fast_exp2((m_known - m_fin) * scale_log2);
+            named_bar_sync(9, kSoftmaxThreads);
+            const float4 lp = *reinterpret_cast<const float4*>(s.part[r]);
+            const float l_run = (lp.x + lp.y) + (lp.z + lp.w);
+            wait(&s.bar_pv[it_last & 1], (it_last >> 1) & 1);              // every P.V of the segment is done
+            tc::fence_after_sync();
+            const bool whole = g.n_tiles == g.n_all;
+            const size_t slot = (size_t(blockIdx.x) + g.index) * kRows + r;
+            const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
+            const int col0 = quarter * 64;
+            if (ok && __all_sync(0xffffffffu, !*const_cast<volatile int*>(&s.failed))) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < 64; c0 += 32) {
+                    uint32_t raw[32];
+                    __syncwarp();
+                    tc::tmem_ld32(lane_addr + kColO + col0 + c0, raw);
+                    tc::tmem_wait_ld();
+                    if (!live) continue;
+                    float o[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(raw[i]) * inv;
+                    if (whole) {
+                        const float* gate = a.gate ? a.gate + (size_t(g.b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + col0 + c0
+                                                   : nullptr;
+                        store_o(a, flat * kHeadDim + col0 + c0, gate, o);
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(a.part_o + slot * kHeadDim + col0 + c0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+                if (!whole && live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
+            }
+            tc::fence_before_sync();
+            named_bar_sync(9, kSoftmaxThreads);               // O, Q and `part` may be rewritten
+        }
+    }
+    __syncthreads();
+    if (warp == kWarpQK) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+// Rows whose pages were divided: one warp per (node, query head), 2 x 4 dims per lane; log-sum-exp over the
+// row's slots (log2 domain), gate, rounding.  grid (ceil(max_nodes * n_q / 8), batch).
+__global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
+    __shared__ Prefix prefix;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
+    const int G = a.n_q / a.n_kv;
+    if (warp == 0) build_prefix(prefix, a, lane, nullptr);
+    __syncthreads();
+    griddep_wait();
+    const Seq q = sequence(a, b, nullptr);
+    const int row = blockIdx.x * 8 + warp, node = row / a.n_q, hq = row - node * a.n_q;
+    if (node >= q.nodes) return;
+    const int h = hq / G, tr = node * G + hq - h * G, hr = h * q.row_tiles + tr / kRows;
+    const int share = share_of(prefix.unit[a.batch], a);
+    const int u0 = prefix.unit[b] + hr * q.tiles;
+    const int first = u0 / share, last = (u0 + q.tiles - 1) / share;
+    if (first == last) return;                                // written by the CTA that held all of it
+    const size_t r0 = (size_t(first) + prefix.seg[b] + hr) * kRows + tr % kRows;
+    float mm = kNoMax;
+    for (int p = lane; p <= last - first; p += 32) mm = fmaxf(mm, a.part_ml[(r0 + size_t(p) * kRows) * 2]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+    float l = 0.f, x[8] = {};
+    for (int p = 0; p <= last - first; ++p) {
+        const size_t row_at = r0 + size_t(p) * kRows;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_at * 2);
+        const float4 o0 = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8));
+        const float4 o1 = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8 + 4));
+        const float w = fast_exp2(ml.x - mm);
+        l = fmaf(ml.y, w, l);
+        x[0] = fmaf(o0.x, w, x[0]); x[1] = fmaf(o0.y, w, x[1]); x[2] = fmaf(o0.z, w, x[2]); x[3] = fmaf(o0.w, w, x[3]);
+        x[4] = fmaf(o1.x, w, x[4]); x[5] = fmaf(o1.y, w, x[5]); x[6] = fmaf(o1.z, w, x[6]); x[7] = fmaf(o1.w, w, x[7]);
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inv;
+    if (a.gate) {
+        const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + lane * 8;
+        const float4 g0 = __ldcs(reinterpret_cast<const float4*>(gp)), g1 = __ldcs(reinterpret_cast<const float4*>(gp + 4));
+        x[0] *= sigmoid(g0.x); x[1] *= sigmoid(g0.y); x[2] *= sigmoid(g0.z); x[3] *= sigmoid(g0.w);
+        x[4] *= sigmoid(g1.x); x[5] *= sigmoid(g1.y); x[6] *= sigmoid(g1.z); x[7] *= sigmoid(g1.w);
+    }
+    const size_t at = ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + lane * 8;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at) =
+        a.o_type == 1 ? make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]))
+                      : make_uint4(pack_b2(x[0], x[1]), pack_b2(x[2], x[3]), pack_b2(x[4], x[5]), pack_b2(x[6], x[7]));
+}
+
+size_t attn_tree_smem_bytes() { return sizeof(Smem) + 1024; }
+int attn_tree_rows() { return kRows; }
+int attn_tree_max_batch() { return kMaxBatch; }
+
+cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
+    attn_tree_kernel<<<a.grid, kThreads, attn_tree_smem_bytes(), st>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned((a.max_nodes * a.n_q + 7) / 8), unsigned(a.batch));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_tree_merge_kernel, a);
+}
+
+}  // namespace rl

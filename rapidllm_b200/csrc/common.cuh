@@ -15,6 +15,7 @@ enum DevErr : int {
     DEV_ERR_WORKSPACE = 3,     // more split-KV chunks than the workspace holds
     DEV_ERR_BAD_SLOT = 4,      // state-cache slot outside the cache
     DEV_ERR_BAD_LEN = 5,       // sequence length outside the page table
+    DEV_ERR_BAD_TREE = 6,      // draft tree: a parent, a node count or a leaf out of range
 };
 
 __device__ __forceinline__ void set_err(int* err, int code) {

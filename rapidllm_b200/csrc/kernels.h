@@ -274,4 +274,91 @@ void launch_conv1d_update(const ConvUpdateArgs& a, cudaStream_t st);
 void launch_conv1d_prefill(const float* x, const float* w, float* y, float* state_io, int seq,
                            int dim, int k, int use_state_in, cudaStream_t st);
 
+// ---- trees of drafted tokens (tree.cuh) ----------------------------------------------------------
+// parents int32 [batch][max_nodes] (null: a chain), n_nodes int32 [batch] (null: max_nodes everywhere)
+struct AttnQkAppendArgs {
+    __half* k_pool;
+    __half* v_pool;
+    const int32_t* page_table;
+    const int32_t* pos;          // [batch] cache position of row 0
+    const int32_t* parents;      // [batch][n_tok] or null: row t is at position pos + t
+    const int32_t* n_nodes;      // [batch] rows of each sequence, or null: n_tok
+    const float* qg;             // rows of [n_q][2 * 256] ([q | gate] per head), qg_stride floats apart
+    const float* k;              // rows of [n_kv][256]
+    const float* v;
+    const float* q_norm;         // [256] or null
+    const float* k_norm;
+    void* q_out;                 // [batch * n_tok][n_q][256] of q_type
+    float* gate_out;             // [batch * n_tok][n_q][256] or null
+    int* err;
+    size_t qg_stride, k_stride, v_stride;
+    int n_q, n_kv, n_tok, n_pages, max_pages_per_seq, rotary_dim, q_type;    // q_type: 0 fp32, 1 fp16, 2 bf16
+    float eps;
+    double inv_turn[256 / 2];   // turns of pair i per position: theta^(-i / pairs) / (2 pi)
+};
+void launch_attn_qk_append(const AttnQkAppendArgs& a, int batch, cudaStream_t st);
+
+struct KvTreeCommitArgs {
+    __half* k_pool;
+    __half* v_pool;
+    const int32_t* page_table;
+    const int32_t* base_len;     // [batch] committed tokens
+    const int32_t* parents;
+    const int32_t* leaf;         // [batch] last node of the path, -1: none
+    int32_t* n_accept;           // [batch] length of the path, or null
+    int* err;
+    int n_kv, max_nodes, n_pages, max_pages_per_seq;
+};
+void launch_kv_tree_commit(const KvTreeCommitArgs& a, int batch, cudaStream_t st);
+
+struct AttnTreeArgs {
+    const __half* k_pool;
+    const __half* v_pool;
+    const int32_t* page_table;   // [batch][max_pages_per_seq]
+    const int32_t* base_len;     // [batch] committed tokens
+    const int32_t* parents;
+    const int32_t* n_nodes;
+    const void* q;               // [batch][max_nodes][n_q][256] of q_type (as above)
+    const float* gate;           // or null; element (row, head, d) at row * gate_row + head * gate_head + d
+    void* o;                     // [batch][max_nodes][n_q][256]; o_type 1 fp16, 2 bf16
+    float* part_o;               // [grid + segments][128][256]
+    float* part_ml;              // [grid + segments][128][2] (maximum in log2 units, sum)
+    int* err;
+    size_t gate_row, gate_head;
+    int batch, max_nodes, n_q, n_kv, n_pages, max_pages_per_seq, q_type, o_type;
+    int max_len;                 // host-side bound of base_len + nodes: the workspace is sized for it
+    int grid, min_share;         // CTAs; least units a CTA takes
+    float scale;
+};
+size_t attn_tree_smem_bytes();
+int attn_tree_rows();
+int attn_tree_max_batch();
+__global__ void attn_tree_kernel(AttnTreeArgs a);
+cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st);
+
+struct GdnTreeArgs {
+    const float* S;              // [n_slots][n_v][128][128]
+    float* S_out;                // commit: the same array
+    const float* conv;           // windows [n_slots][conv_dim][4]
+    float* conv_out;             // commit: the same array
+    const int32_t* conv_phase;   // [n_slots] ring position (gdn_decode.cu), or null: shifted windows
+    const int32_t* slot_ids;     // [batch] or null
+    const int32_t* parents;
+    const int32_t* n_nodes;
+    const int32_t* leaf;         // commit: [batch], -1: none
+    const float* x;              // [batch][max_nodes] rows of conv_dim channels, x_stride floats apart
+    const float* w;              // [conv_dim][4]
+    const float* beta;           // [batch][max_nodes][n_v]
+    const float* g_log;
+    float* o;                    // [batch][max_nodes][n_v][128]
+    int* err;
+    size_t x_stride;
+    int batch, max_nodes, n_v, n_qk, n_slots, head_map, conv_dim;
+    float eps_l2;
+};
+size_t gdn_tree_smem_bytes();
+const void* gdn_tree_kernel_ptr();
+void launch_gdn_tree(const GdnTreeArgs& a, cudaStream_t st);
+cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st);
+
 }  // namespace rl

@@ -23,7 +23,7 @@ from ._lib import DeltaRecurrentParams, check, lib
 
 def _matmul(x, w):
     if w.dtype == torch.float32:
-        return x @ w.t()
+        return x.float() @ w.t()
     return (x.to(w.dtype) @ w.t()).float()
 
 
@@ -100,6 +100,31 @@ class DeltaNetMixer:
         return x + _matmul(og.view(T, zd), self.W_out)
 
 
+    def verify_tree(self, x, parents, n_nodes=None, slot_ids=None):
+        """Every node of a draft tree along its own path: x fp32 [batch][nodes][hidden] -> the nodes' new hidden
+        states, and what commit_tree needs to keep one path.  The slots' state and windows are only read.
+        parents int32 [batch][nodes], n_nodes int32 [batch] or None (ops.gdn_tree); rows behind a sequence's
+        last node come back unspecified."""
+        B, n, hidden = x.shape
+        cd, zd, nv = self.conv_dim, self.zdim, self.n_v
+        rows = x.reshape(B * n, hidden)
+        proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in)
+        qkv = proj.view(B, n, -1)[..., :cd]                  # read where the projection left it
+        z = proj[:, cd:cd + zd].contiguous()
+        beta, g = ops.delta_gates(proj[:, cd + zd:cd + zd + nv].contiguous(), proj[:, cd + zd + nv:].contiguous(),
+                                  self.A_log, self.dt_bias)
+        pending = (qkv, beta.view(B, n, nv), g.view(B, n, nv))
+        o = ops.gdn_tree(self.S, self.conv_state, None, pending[0], self.conv_w, pending[1], pending[2], parents, self.n_k,
+                         n_nodes=n_nodes, slot_ids=slot_ids, head_map=self.head_map)
+        og = ops.gated_rmsnorm(o.view(B * n, nv, self.dv), z.view(B * n, nv, self.dv), self.gnorm, 1e-6)
+        return (rows + _matmul(og.view(B * n, zd), self.W_out)).view(B, n, hidden), pending
+
+    def commit_tree(self, pending, parents, leaf, slot_ids=None):
+        """Advance the slots by the path to node leaf[b] (-1: nothing) of the tree that verify_tree ran."""
+        ops.gdn_tree_commit(self.S, self.conv_state, None, pending[0], self.conv_w, pending[1], pending[2], parents, leaf,
+                            self.n_k, slot_ids=slot_ids, head_map=self.head_map)
+
+
 class GatedAttentionMixer:
     """w: rms_w [hidden], Wq [n_q*2*hd, hidden] ([q | gate] rows per head), Wk, Wv [n_kv*hd, hidden],
     Wo [hidden, n_q*hd], q_norm, k_norm [hd].  The KV cache is paged F16 (k_pool, v_pool)."""
@@ -128,6 +153,28 @@ class GatedAttentionMixer:
         ops.kv_append(self.k_pool, self.v_pool, page_table, k.unsqueeze(1), v.unsqueeze(1), pos=pos)
         o = ops.attn_decode(q, self.k_pool, self.v_pool, page_table, pos + 1, gate)
         return x + _matmul(o.view(B, qn), self.W_out)
+
+
+    def verify_tree(self, x, page_table, base_len, parents, n_nodes=None):
+        """Every node of a draft tree: x fp32 [batch][nodes][hidden] -> the nodes' new hidden states.  Node i's K and V
+        go to cache position base_len[b] + i (int32 [batch], the committed tokens); commit_tree moves one path's
+        rows together.  The query meets the tensor cores as fp16, as K does."""
+        B, n, hidden = x.shape
+        qn, kn = self.n_q * self.hd, self.n_kv * self.hd
+        rows = x.reshape(B * n, hidden)
+        proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in).view(B, n, -1)
+        qg = proj[..., :2 * qn].view(B, n, self.n_q, 2 * self.hd)
+        k = proj[..., 2 * qn:2 * qn + kn].view(B, n, self.n_kv, self.hd)
+        v = proj[..., 2 * qn + kn:].view(B, n, self.n_kv, self.hd)
+        q, _ = ops.attn_qk_append(qg, k, v, self.k_pool, self.v_pool, page_table, base_len, self.q_norm, self.k_norm,
+                                  parents=parents, n_nodes=n_nodes, rotary_dim=self.rotary_dim, theta=self.theta,
+                                  eps=self.eps, q_dtype=torch.float16, want_gate=False)
+        o = ops.attn_tree(q, self.k_pool, self.v_pool, page_table, base_len, parents, n_nodes=n_nodes, gate=qg[..., self.hd:])
+        return (rows + _matmul(o.view(B * n, qn), self.W_out)).view(B, n, hidden)
+
+    def commit_tree(self, page_table, base_len, parents, leaf):
+        """Keep the path to node leaf[b] (-1: nothing); returns the paths' lengths, by which base_len grows."""
+        return ops.kv_tree_commit(self.k_pool, self.v_pool, page_table, base_len, parents, leaf)
 
 
 class MixerStack:
@@ -160,6 +207,31 @@ class MixerStack:
             else:
                 x = layer.decode(x, slot_ids)
         return x
+
+    def verify_tree(self, x, page_table, base_len, parents, n_nodes=None, slot_ids=None):
+        """One verify pass over a draft tree: x fp32 [batch][nodes][hidden] -> hidden states after the last mixer, and
+        what commit_tree needs.  parents int32 [batch][nodes] (< own index, -1 = continues the committed tokens),
+        n_nodes int32 [batch] or None, base_len int32 [batch] committed tokens, all on the device."""
+        pending = []
+        for layer in self.layers:
+            if isinstance(layer, GatedAttentionMixer):
+                x = layer.verify_tree(x, page_table, base_len, parents, n_nodes)
+                pending.append(None)
+            else:
+                x, kept = layer.verify_tree(x, parents, n_nodes, slot_ids)
+                pending.append(kept)
+        return x, pending
+
+    def commit_tree(self, pending, page_table, base_len, parents, leaf, slot_ids=None):
+        """Keep the path to node leaf[b] (int32 [batch], -1: nothing) in every layer; returns the paths' lengths,
+        int32 [batch] (the caller adds them to base_len), or None without an attention layer."""
+        taken = None
+        for layer, kept in zip(self.layers, pending):
+            if isinstance(layer, GatedAttentionMixer):
+                taken = layer.commit_tree(page_table, base_len, parents, leaf)
+            else:
+                layer.commit_tree(kept, parents, leaf, slot_ids)
+        return taken
 
 
 def _attn_prefill(self, x, page_table_row, pos0):

@@ -387,3 +387,221 @@ def conv_ring_export(conv_ring, conv_phase):
     check(lib().rl_conv_ring_export(_p(conv_ring), _p(conv_phase), _p(out), 1, conv_ring.shape[0], -1,
                                     conv_ring.shape[1], _stream()))
     return out
+
+
+# ---- trees of drafted tokens: append, verify, commit (rl_b200.h has the format of parents, n_nodes, leaf) ----
+
+_TYPES = {torch.float32: _lib.RL_TYPE_F32, torch.float16: _lib.RL_TYPE_F16, torch.bfloat16: _lib.RL_TYPE_BF16}
+
+
+def _here(**tensors):
+    """Every tensor is on the current CUDA device (the one whose current stream the call goes to)."""
+    dev = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise _lib.RlError(6, f"{name}: need a tensor on the current device cuda:{dev}, got one on {t.device}")
+
+
+def _shape(t, shape, name):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise _lib.RlError(6, f"{name}: need shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _rows(t, name):
+    """fp32 [batch][rows]..., dense inside a row, rows at one distance: that distance in floats."""
+    if t.dtype != torch.float32:
+        raise _lib.RlError(6, f"{name}: need fp32")
+    inner = 1
+    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+        if size > 1 and stride != inner:
+            raise _lib.RlError(6, f"{name}: a row must be contiguous")
+        inner *= size
+    B, T = t.shape[:2]
+    row = t.stride(1) if T > 1 else (t.stride(0) if B > 1 else inner)
+    if B > 1 and T > 1 and t.stride(0) != T * row:
+        raise _lib.RlError(6, f"{name}: the rows of all sequences must be at one distance")
+    return row
+
+
+def _tree(parents, n_nodes, batch, nodes):
+    _need(parents, torch.int32, "parents")
+    _need(n_nodes, torch.int32, "n_nodes")
+    _shape(parents, (batch, nodes), "parents")
+    _shape(n_nodes, (batch,), "n_nodes")
+
+
+def _pools(k_pool, v_pool, page_table, batch):
+    _need(k_pool, torch.float16, "k_pool")
+    _need(v_pool, torch.float16, "v_pool")
+    _need(page_table, torch.int32, "page_table")
+    _shape(v_pool, k_pool.shape, "v_pool")
+    if k_pool.dim() != 3 or k_pool.shape[2] != PAGE_TOKENS * HEAD_DIM:
+        raise _lib.RlError(6, "k_pool: need [n_pages][n_kv][64 * 256] (new_pool)")
+    if page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise _lib.RlError(6, f"page_table: need [{batch}][max_pages]")
+
+
+def attn_qk_append(qg, k, v, k_pool, v_pool, page_table, pos, q_norm=None, k_norm=None, parents=None, n_nodes=None,
+                   rotary_dim=64, theta=1e7, eps=1e-6, q_dtype=torch.float32, want_gate=True, q_out=None, gate_out=None):
+    """From the projections to the operands of the attention in one pass: q/gate split, head RMSNorm
+    (1 + gamma), rotation, K and V rows into the paged F16 cache at pos[b] + t.
+
+    qg fp32 [batch][n_tok][n_q][512] ([q | gate] per head), k, v fp32 [batch][n_tok][n_kv][256], column
+    ranges of one projection or dense; pos int32 [batch].  Row t is rotated by pos[b] + t, with parents
+    [batch][n_tok] (n_tok <= 64) by pos[b] + the node's depth.  Returns q of q_dtype (or of q_out) and the
+    gate, None without want_gate.  Rows behind n_nodes[b] are left as they are."""
+    batch, n_tok, n_q, two_hd = qg.shape
+    n_kv = k_pool.shape[1]
+    _here(qg=qg, k=k, v=v, k_pool=k_pool, v_pool=v_pool, page_table=page_table, pos=pos, q_norm=q_norm, k_norm=k_norm,
+          parents=parents, n_nodes=n_nodes, q_out=q_out, gate_out=gate_out)
+    _pools(k_pool, v_pool, page_table, batch)
+    _need(pos, torch.int32, "pos")
+    _shape(pos, (batch,), "pos")
+    _shape(k, (batch, n_tok, n_kv, HEAD_DIM), "k")
+    _shape(v, (batch, n_tok, n_kv, HEAD_DIM), "v")
+    _tree(parents, n_nodes, batch, n_tok)
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        _need(t, torch.float32, name)
+        _shape(t, (HEAD_DIM,), name)
+    if two_hd != 2 * HEAD_DIM:
+        raise _lib.RlError(4, f"qg: rows of {two_hd} per head, only 512")
+    if q_out is None:
+        q_out = torch.empty(batch, n_tok, n_q, HEAD_DIM, dtype=q_dtype, device=qg.device)
+    if q_out.dtype not in _TYPES:
+        raise _lib.RlError(4, f"q_out: {q_out.dtype} unknown")
+    _need(q_out, q_out.dtype, "q_out")
+    _shape(q_out, (batch, n_tok, n_q, HEAD_DIM), "q_out")
+    if not want_gate:
+        gate_out = None
+    elif gate_out is None:
+        gate_out = torch.empty(batch, n_tok, n_q, HEAD_DIM, dtype=torch.float32, device=qg.device)
+    _need(gate_out, torch.float32, "gate_out")
+    _shape(gate_out, (batch, n_tok, n_q, HEAD_DIM), "gate_out")
+    p = _lib.AttnQkAppendParams(n_q, n_kv, HEAD_DIM, rotary_dim, batch, n_tok, PAGE_TOKENS, k_pool.shape[0],
+                                page_table.shape[1], _TYPES[q_out.dtype], theta, eps, _rows(qg, "qg"), _rows(k, "k"),
+                                _rows(v, "v"))
+    check(lib().rl_attn_qk_append(_p(k_pool), _p(v_pool), _p(page_table), _p(pos), _p(parents), _p(n_nodes), _p(qg),
+                                  _p(k), _p(v), _p(q_norm), _p(k_norm), _p(q_out), _p(gate_out), C.byref(p), _stream()))
+    return q_out, gate_out
+
+
+def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=None, gate=None, max_seq_len=None, out=None,
+              out_dtype=None, workspace=None):
+    """Attention of every node of a draft tree over the paged F16 cache: node i of sequence b sees the rows
+    [0, base_len[b]) and base_len[b] + j for its ancestors j and itself; o *= sigmoid(gate).
+
+    q fp32, fp16 or bf16 [batch][nodes][n_q][256]; gate fp32 of that shape, dense or strided (qg[..., 256:] as
+    it lies); out fp16 or bf16 (default: q's type, fp16 for fp32).  parents None = chains."""
+    batch, nodes, n_q, hd = q.shape
+    n_kv = k_pool.shape[1]
+    _here(q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, base_len=base_len, parents=parents, n_nodes=n_nodes,
+          gate=gate, out=out, workspace=workspace)
+    _pools(k_pool, v_pool, page_table, batch)
+    _tree(parents, n_nodes, batch, nodes)
+    _need(base_len, torch.int32, "base_len")
+    _shape(base_len, (batch,), "base_len")
+    if q.dtype not in _TYPES:
+        raise _lib.RlError(4, f"q: {q.dtype} unknown")
+    _need(q, q.dtype, "q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or (torch.float16 if q.dtype == torch.float32 else q.dtype), device=q.device)
+    if out.dtype not in _TYPES:
+        raise _lib.RlError(4, f"out: {out.dtype} unknown")
+    _need(out, out.dtype, "out")
+    _shape(out, q.shape, "out")
+    row = head = 0
+    if gate is not None:
+        _shape(gate, q.shape, "gate")
+        if gate.dtype != torch.float32 or gate.stride(3) != 1:
+            raise _lib.RlError(6, "gate: need fp32, contiguous inside a head")
+        head = gate.stride(2) if n_q > 1 else hd
+        row = gate.stride(1) if nodes > 1 else (gate.stride(0) if batch > 1 else 0)
+        if batch > 1 and nodes > 1 and gate.stride(0) != nodes * row:
+            raise _lib.RlError(6, "gate: the rows of all sequences must be at one distance")
+    p = _lib.AttnTreeParams(n_q, n_kv, hd, batch, nodes, PAGE_TOKENS, k_pool.shape[0], page_table.shape[1],
+                            page_table.shape[1] * PAGE_TOKENS if max_seq_len is None else max_seq_len, _TYPES[q.dtype],
+                            _TYPES[out.dtype], row, head)
+    need = lib().rl_attn_tree_workspace_bytes(C.byref(p))
+    if need == 0:
+        raise _lib.RlError(6, lib().rl_last_error().decode())
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    check(lib().rl_attn_tree(_p(k_pool), _p(v_pool), _p(page_table), _p(base_len), _p(parents), _p(n_nodes), _p(q),
+                             _p(gate), _p(out), _p(workspace), workspace.numel() * workspace.element_size(), C.byref(p),
+                             _stream()))
+    return out
+
+
+def kv_tree_commit(k_pool, v_pool, page_table, base_len, parents, leaf):
+    """Keep the path to node leaf[b] (int32 [batch], -1 = nothing) of each sequence's tree: its K and V rows move
+    to positions base_len[b], base_len[b] + 1, ...  Returns the paths' lengths, int32 [batch].  parents int32
+    [batch][nodes], or the number of nodes for chains."""
+    batch = leaf.shape[0]
+    nodes = parents if isinstance(parents, int) else parents.shape[1]
+    parents = None if isinstance(parents, int) else parents
+    _here(k_pool=k_pool, v_pool=v_pool, page_table=page_table, base_len=base_len, parents=parents, leaf=leaf)
+    _pools(k_pool, v_pool, page_table, batch)
+    _tree(parents, None, batch, nodes)
+    for t, name in ((base_len, "base_len"), (leaf, "leaf")):
+        _need(t, torch.int32, name)
+        _shape(t, (batch,), name)
+    n_accept = torch.empty(batch, dtype=torch.int32, device=leaf.device)
+    p = _lib.KvTreeCommitParams(k_pool.shape[1], HEAD_DIM, batch, nodes, PAGE_TOKENS, k_pool.shape[0], page_table.shape[1])
+    check(lib().rl_kv_tree_commit(_p(k_pool), _p(v_pool), _p(page_table), _p(base_len), _p(parents), _p(leaf),
+                                  _p(n_accept), C.byref(p), _stream()))
+    return n_accept
+
+
+def _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_nodes, n_qk, slot_ids, head_map,
+                     eps_l2, **more):
+    n_slots, n_v, dk, dv = S.shape
+    batch, nodes, dim = qkv.shape
+    _here(S=S, conv_window=conv_window, conv_phase=conv_phase, qkv=qkv, conv_w=conv_w, beta=beta, g_log=g_log,
+          parents=parents, n_nodes=n_nodes, slot_ids=slot_ids, **more)
+    for t, n in ((S, "S"), (conv_window, "conv_window"), (conv_w, "conv_w"), (beta, "beta"), (g_log, "g_log")):
+        _need(t, torch.float32, n)
+    _tree(parents, n_nodes, batch, nodes)
+    if dim != 2 * n_qk * dk + n_v * dv:
+        raise _lib.RlError(6, f"qkv: rows of {dim} channels, {n_qk} key and {n_v} value heads need {2 * n_qk * dk + n_v * dv}")
+    _shape(conv_window, (n_slots, dim, 4), "conv_window")
+    _shape(conv_w, (dim, 4), "conv_w")
+    _shape(beta, (batch, nodes, n_v), "beta")
+    _shape(g_log, (batch, nodes, n_v), "g_log")
+    _need(conv_phase, torch.int32, "conv_phase")
+    _shape(conv_phase, (n_slots,), "conv_phase")
+    _need(slot_ids, torch.int32, "slot_ids")
+    _shape(slot_ids, (batch,), "slot_ids")
+    if slot_ids is None and batch > n_slots:
+        raise _lib.RlError(6, f"{batch} sequences in {n_slots} slots")
+    if head_map is None:
+        head_map = _lib.RL_HEADS_PER_VALUE if n_qk == n_v else _lib.RL_HEADS_GROUPED
+    return _lib.GdnTreeParams(n_v, n_qk, dk, dv, 4, batch, nodes, n_slots, head_map, eps_l2, _rows(qkv, "qkv"))
+
+
+def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk, n_nodes=None, slot_ids=None,
+             head_map=None, eps_l2=1e-6, out=None):
+    """The Gated DeltaNet step of every node of a draft tree, each along its own path; S [n_slots][n_v][128][128]
+    and conv_window [n_slots][conv_dim][4] are only read.  conv_phase int32 [n_slots] (rings, see gdn_decode) or
+    None (shifted windows, conv1d_update's state).  qkv fp32 [batch][nodes][conv_dim] (rows may be a column range),
+    beta, g_log [batch][nodes][n_v].  Returns o fp32 [batch][nodes][n_v][128]."""
+    p = _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_nodes, n_qk, slot_ids, head_map,
+                         eps_l2, out=out)
+    shape = (qkv.shape[0], qkv.shape[1], S.shape[1], S.shape[3])
+    o = torch.empty(shape, dtype=torch.float32, device=S.device) if out is None else out
+    _need(o, torch.float32, "out")
+    _shape(o, shape, "out")
+    check(lib().rl_gdn_tree(_p(S), _p(conv_window), _p(conv_phase), _p(slot_ids), _p(parents), _p(n_nodes), _p(qkv),
+                            _p(conv_w), _p(beta), _p(g_log), _p(o), C.byref(p), _stream()))
+    return o
+
+
+def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, n_qk, slot_ids=None,
+                    head_map=None, eps_l2=1e-6):
+    """Advance S and conv_window of each sequence's slot by the path to node leaf[b] (-1 = nothing), in place, with
+    gdn_tree's inputs; conv_phase stays.  slot_ids must be distinct."""
+    p = _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, None, n_qk, slot_ids, head_map,
+                         eps_l2, leaf=leaf)
+    _need(leaf, torch.int32, "leaf")
+    _shape(leaf, (qkv.shape[0],), "leaf")
+    check(lib().rl_gdn_tree_commit(_p(S), _p(conv_window), _p(conv_phase), _p(slot_ids), _p(parents), _p(leaf), _p(qkv),
+                                   _p(conv_w), _p(beta), _p(g_log), C.byref(p), _stream()))
