@@ -119,8 +119,7 @@ int dev_info(DevInfo** out) {
                                      int(rl::attn_decode_tq_smem_bytes())));
         RL_CUDA(cudaFuncSetAttribute(rl::attn_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      int(rl::attn_tree_smem_bytes())));
-        RL_CUDA(cudaFuncSetAttribute(rl::gdn_tree_kernel_ptr(), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     int(rl::gdn_tree_smem_bytes())));
+        RL_CUDA(rl::gdn_tree_setup());
         d.ready = true;
     }
     *out = &d;
@@ -1674,7 +1673,9 @@ int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_ph
     if (!aligned16(o)) return fail(RL_ERR_RANGE, "o must be 16-byte aligned");
     a.n_nodes = n_nodes;
     a.o = o;
-    rl::launch_gdn_tree(a, as_stream(stream));
+    DevInfo* d;
+    if (int st = dev_info(&d)) return st;
+    rl::launch_gdn_tree(a, d->sms, as_stream(stream));
     RL_CUDA(cudaGetLastError());
     return RL_OK;
 }

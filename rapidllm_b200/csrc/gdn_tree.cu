@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "tcgen05.cuh"
 #include "tree.cuh"
 
 namespace rl {
@@ -96,106 +97,444 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float acc) {
     return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, acc))));
 }
 
+// ---- packed pairs of fp32 ----
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// x0, x1 as fp16 pairs: hi, and what hi leaves
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack_h2(x0 - f.x, x1 - f.y);
+}
+// the power of two that brings a largest magnitude mx into [2^14, 2^15), and its inverse
+__device__ __forceinline__ float lift(float mx, float& back) {
+    const int e = int(__float_as_uint(mx) >> 23) - 127;
+    const int up = mx > 0.f && e < 128 ? min(max(14 - e, -112), 112) : 0;
+    back = __uint_as_float(uint32_t(127 - up) << 23);
+    return __uint_as_float(uint32_t(127 + up) << 23);
+}
+// scale of the unit vectors k, q and of the coefficients (all at most 1) under their split
+constexpr float kLift = 4096.f, kBack = 1.f / 4096.f;
+
+constexpr int kThreads = 256, kHalf = kThreads / 2;
+
+// The triangular coefficients of the solve, by columns: entry (j, i), i > j, at off(j) + i; a column starts at
+// a multiple of four.
+template <int NB>
+__host__ __device__ constexpr int low_off(int j) {
+    const int g = j >> 2;
+    return 4 * (NB * g - 2 * g * (g - 1)) + (j & 3) * (NB - 4 * g) - 4 * g;
+}
+template <int NB>
 struct TreeSmem {
-    float q[kMaxNodes][kDk], k[kMaxNodes][kDk], u[kMaxNodes][kDv];
-    float low[kMaxNodes][kMaxNodes], mix[kMaxNodes][kMaxNodes];      // coefficients of u_j in u_i and in o_i
-    float decay[kMaxNodes], beta[kMaxNodes];                          // c_i
+    static constexpr int kSub = 2 * NB * 128;                 // 64 dims of the rows [k; q], 128 bytes each
+    alignas(1024) unsigned char kq[4][kSub];                  // hi dims 0-63, 64-127, lo dims 0-63, 64-127
+    alignas(1024) unsigned char mix[2][NB * 128];             // coefficients of u_j in o_i: hi, lo
+    alignas(16) float low[4 * (NB * NB / 4 - 2 * (NB / 4) * (NB / 4 - 1))];
+    float gram[NB][NB + 1];                                   // [i][j], j < i: k_i . k_j; [j][i], j <= i: q_i . k_j
+    float decay[NB], grow[NB], beta[NB], in[NB];              // c_i, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
+    float amax[2][kDv], back[kDv], uback[kDv];
     unsigned long long word[kMaxNodes];
     int parents[kMaxNodes];
-    int4 src[kMaxNodes];
+    int4 src[NB];
+    uint64_t bar_gram, bar_half, bar_in, bar_out;
+    uint32_t tmem_base;
 };
+template <int NB>
+constexpr size_t tree_smem_bytes() {
+    // the Gram product takes its A operand as 128 rows, past the last tile's where there are fewer
+    return (sizeof(TreeSmem<NB>) > 3 * TreeSmem<NB>::kSub + 128 * 128 ? sizeof(TreeSmem<NB>) : 3 * TreeSmem<NB>::kSub + 128 * 128) + 1024;
+}
 
-constexpr int kThreads = 128;
+// byte offset of fp16 element (row, d < 64) in a tile of 128-byte rows under the 128-byte swizzle
+__device__ __forceinline__ int tile_at(int row, int d) { return row * 128 + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2; }
 
 }  // namespace
 
-// grid (n_v, batch): one CTA per (sequence, value head), thread = column of the state.
-__global__ void __launch_bounds__(kThreads) gdn_tree_kernel(GdnTreeArgs a) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    TreeSmem& s = *reinterpret_cast<TreeSmem*>(smem_raw);
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
+// One CTA per (key head, sequence) with that key head's value heads one after the other (a.heads > 1), or per
+// (value head, sequence).  Node count rounded up to NB.
+//
+// S0^T k and S0^T q of all nodes are one product per value head, D[v][row] = sum_d S0[d][v] [k; q][row][d],
+// with the state as the A operand in tensor memory (a thread reads column v of the state with coalesced loads
+// and stores it as TMEM lane v) and the rows [k; q] as the K-major B operand in shared memory; so is the last
+// term of o, with A = u.  Both must keep fp32's precision: operands are split into two fp16 terms (22 bits,
+// rows scaled by powers of two so that neither term leaves fp16's range) and hi lo + lo hi + hi hi accumulate
+// in fp32, the small ones first.  The solve between them is triangular: thread v keeps column v of
+// u in registers and, once u_j is known, takes it out of all later rows (right-looking, so the fused
+// multiply-adds of a step are independent; two rows per packed instruction).
+template <int NB>
+__global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
+    using Smem = TreeSmem<NB>;
+    extern __shared__ unsigned char smem_raw[];
+    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // tensor memory: A (32 columns hi, 32 lo: half the state's dims, later u), then D
+    constexpr uint32_t kColA = 0, kColD = 64;
+    constexpr uint32_t kCols = 64 + 2 * NB <= 128 ? 128 : 256;
+    const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int grp = warp >> 2;                                // half of the state's dims; 0: solves
+    const int v = tid & (kDv - 1);                            // column of the state = TMEM lane
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
+    const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
     if (slot < 0 || slot >= a.n_slots) {
         if (tid == 0) set_err(a.err, DEV_ERR_BAD_SLOT);
         return;
     }
     if (n == 0) return;
+    const int ratio = a.n_v / a.n_qk;
+    const int h0 = a.heads == 1 ? int(blockIdx.x) : (a.head_map == 1 ? int(blockIdx.x) * ratio : int(blockIdx.x));
+    const int h_step = a.head_map == 1 ? 1 : a.n_qk;
+    const int hs = a.heads == 1 ? key_head_of(h0, a.n_v, a.n_qk, a.head_map) : int(blockIdx.x);
+
+    // the first head's half column of the state, on its way while the rows are prepared
+    float st[kDk / 2];
+    auto fetch = [&](int h) {
+        const float* S = a.S + (size_t(slot) * a.n_v + h) * (kDk * kDv) + size_t(grp) * (kDk / 2) * kDv + v;
+#pragma unroll
+        for (int d = 0; d < kDk / 2; ++d) st[d] = __ldcs(S + d * kDv);
+    };
+
     if (warp == 0) {
         const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, n, lane, a.err);
         s.word[lane] = w.lo;
         s.word[lane + 32] = w.hi;
         s.parents[lane] = w.parent_lo;
         s.parents[lane + 32] = w.parent_hi;
+        __syncwarp();
+        for (int i = lane; i < n; i += 32) s.src[i] = conv_sources(i, s.parents);
+    } else if (warp == 1) {
+        tc::tmem_alloc(&s.tmem_base, kCols);
+    } else if (tid == 64) {
+        mbar_init(&s.bar_gram, 1);
+        mbar_init(&s.bar_half, 1);
+        mbar_init(&s.bar_in, 1);
+        mbar_init(&s.bar_out, 1);
+        mbar_fence_init();
     }
+    tc::fence_before_sync();
     __syncthreads();
-    if (tid < n) {
-        s.src[tid] = conv_sources(tid, s.parents);
-        float c = 0.f;
-        for (unsigned long long m = s.word[tid]; m; m &= m - 1)
-            c += a.g_log[(size_t(b) * a.max_nodes + (__ffsll(m) - 1)) * a.n_v + h];
-        s.decay[tid] = c;
-        s.beta[tid] = a.beta[(size_t(b) * a.max_nodes + tid) * a.n_v + h];
-    }
-    __syncthreads();
-    const int hs = key_head_of(h, a.n_v, a.n_qk, a.head_map);
+    tc::fence_after_sync();
+    const uint32_t tmem = s.tmem_base, lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {         // `ok` is the same in all lanes of a warp
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+            set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+            ok = false;
+        }
+    };
     const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride;
+
+    // ---- k and q of all nodes: conv, SiLU, unit length, split; a warp per node, 4 dims per lane ----
 #pragma unroll 1
-    for (int role = 0; role < 3; ++role) {
-        const int c0 = (role == 0 ? hs * kDk : (role == 1 ? (a.n_qk + hs) * kDk : 2 * a.n_qk * kDk + h * kDv)) + lane * 4;
+    for (int role = 0; role < 2; ++role) {                    // 0: k, 1: q
+        const int c0 = (role == 0 ? (a.n_qk + hs) * kDk : hs * kDk) + lane * 4;
         Conv4 cv;
         cv.load(a, slot, c0);
-        for (int i = warp; i < n; i += kThreads / 32) {
-            float4 y = conv_node(cv, x + c0, a.x_stride, s.src[i]);
-            if (role == 0) y = unit(y, a.eps_l2, 1.f / sqrtf(float(kDk)));
-            if (role == 1) y = unit(y, a.eps_l2, 1.f);
-            *reinterpret_cast<float4*>(role == 0 ? &s.q[i][lane * 4] : (role == 1 ? &s.k[i][lane * 4] : &s.u[i][lane * 4])) = y;
+        for (int i = warp; i < NB; i += kThreads / 32) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < n) y = unit(conv_node(cv, x + c0, a.x_stride, s.src[i]), a.eps_l2, kLift);
+            uint2 hi, lo;
+            split2(y.x, y.y, hi.x, lo.x);
+            split2(y.z, y.w, hi.y, lo.y);
+            const int at = tile_at(role * NB + i, (lane * 4) & 63);
+            *reinterpret_cast<uint2*>(s.kq[lane >> 4] + at) = hi;
+            *reinterpret_cast<uint2*>(s.kq[2 + (lane >> 4)] + at) = lo;
         }
     }
+    fetch(h0);
+    tc::fence_async_smem();
     __syncthreads();
-    for (int p = tid; p < n * n; p += kThreads) {
-        const int i = p / n, j = p - i * n;
-        if (!(s.word[i] >> j & 1)) continue;
-        float kk = 0.f, qk = 0.f;
-        for (int d = 0; d < kDk; d += 4) {
-            const float4 kj = *reinterpret_cast<const float4*>(&s.k[j][d]);
-            kk = dot4(*reinterpret_cast<const float4*>(&s.k[i][d]), kj, kk);
-            qk = dot4(*reinterpret_cast<const float4*>(&s.q[i][d]), kj, qk);
-        }
-        const float e = expf(s.decay[i] - s.decay[j]);
-        s.low[i][j] = s.beta[i] * e * kk;
-        s.mix[i][j] = e * qk;
-    }
-    __syncthreads();
-    const float* S = a.S + (size_t(slot) * a.n_v + h) * (kDk * kDv) + tid;
-    constexpr int kStep = 8;
-    for (int i0 = 0; i0 < n; i0 += kStep) {
-        float ks[kStep] = {}, qs[kStep] = {};
-        for (int d = 0; d < kDk; ++d) {
-            const float sv = S[d * kDv];
+    auto kq_desc = [&](int part) { return tc::smem_desc(smem_u32(s.kq[part]), 16, 1024); };
+    if (tid == 0) {
+        // [k; q] k^T, lane = row
+        constexpr uint32_t idesc = tc::idesc_f16(128, NB, false, false);
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int pa = pass == 0 ? 2 : 0, pb = pass == 1 ? 2 : 0;     // lo hi, hi lo, hi hi
 #pragma unroll
-            for (int r = 0; r < kStep; ++r) {
-                const int i = min(i0 + r, n - 1);
-                ks[r] = fmaf(s.k[i][d], sv, ks[r]);
-                qs[r] = fmaf(s.q[i][d], sv, qs[r]);
+            for (int kk = 0; kk < 8; ++kk)
+                tc::mma_ss(tmem + kColD, kq_desc(pa + (kk >> 2)) + (kk & 3) * 2, kq_desc(pb + (kk >> 2)) + (kk & 3) * 2, idesc,
+                           pass > 0 || kk > 0);
+        }
+        tc::commit(&s.bar_gram);
+    }
+    wait(&s.bar_gram, 0);
+    tc::fence_after_sync();
+    {
+        const bool is_q = v >= NB;
+        const int i = is_q ? v - NB : v;
+#pragma unroll
+        for (int c = 0; c < NB / 2; c += 8) {
+            const int j0 = grp * (NB / 2) + c;
+            uint32_t g[8];
+            tc::tmem_ld8(lanes + kColD + j0, g);
+            tc::tmem_wait_ld();
+            if (v < 2 * NB) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = j0 + e;
+                    const float f = __uint_as_float(g[e]) * (kBack * kBack);
+                    if (!is_q && j < i) s.gram[i][j] = f;
+                    if (is_q && j <= i) s.gram[j][i] = f;
+                }
+            }
+            __syncwarp();
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+
+#pragma unroll 1
+    for (int hi = 0; hi < a.heads; ++hi) {
+        const int h = h0 + hi * h_step;
+        const uint32_t par = hi & 1;
+        // ---- decays along the paths ----
+        if (warp == 4) {
+            const size_t at = size_t(b) * a.max_nodes * a.n_v + h;
+            float c0 = lane < n ? a.g_log[at + size_t(lane) * a.n_v] : 0.f;
+            float c1 = NB > 32 && lane + 32 < n ? a.g_log[at + size_t(lane + 32) * a.n_v] : 0.f;
+            const float b0 = lane < n ? a.beta[at + size_t(lane) * a.n_v] : 0.f;
+            const float b1 = NB > 32 && lane + 32 < n ? a.beta[at + size_t(lane + 32) * a.n_v] : 0.f;
+            int j0 = s.parents[lane], j1 = s.parents[lane + 32];
+            while (__any_sync(0xffffffffu, j0 >= 0 || j1 >= 0)) {
+                const float x0 = tree::of_node(c0, c1, j0 & 63), x1 = tree::of_node(c0, c1, j1 & 63);
+                const int y0 = tree::of_node(j0, j1, j0 & 63), y1 = tree::of_node(j0, j1, j1 & 63);
+                if (j0 >= 0) {
+                    c0 += x0;
+                    j0 = y0;
+                }
+                if (j1 >= 0) {
+                    c1 += x1;
+                    j1 = y1;
+                }
+            }
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int i = lane + 32 * z;
+                if (i >= NB) break;
+                const float c = z ? c1 : c0, bt = z ? b1 : b0, e = expf(c);
+                s.decay[i] = c;
+                s.grow[i] = e;
+                s.beta[i] = bt;
+                s.in[i] = -bt * e * kBack;
             }
         }
+        // ---- the state's column -> A, 64 dims at a time ----
+        {
+            float mx = 0.f;
 #pragma unroll
-        for (int r = 0; r < kStep; ++r) {
-            const int i = i0 + r;
-            if (i >= n) break;
-            const float e = expf(s.decay[i]);
-            float u = s.beta[i] * (s.u[i][tid] - e * ks[r]), o = e * qs[r];
-            for (unsigned long long m = s.word[i] & ~(1ull << i); m; m &= m - 1) {
-                const int j = __ffsll(m) - 1;
-                const float uj = s.u[j][tid];
-                u = fmaf(-s.low[i][j], uj, u);
-                o = fmaf(s.mix[i][j], uj, o);
-            }
-            s.u[i][tid] = u;
-            a.o[((size_t(b) * a.max_nodes + i) * a.n_v + h) * kDv + tid] = fmaf(s.mix[i][i], u, o);
+            for (int d = 0; d < kDk / 2; ++d) mx = fmaxf(mx, fabsf(st[d]));
+            s.amax[grp][v] = mx;
         }
+        __syncthreads();
+        float back;
+        const float f = lift(fmaxf(s.amax[0][v], s.amax[1][v]), back);
+        if (grp == 0) s.back[v] = back;
+        if (grp == 1) wait(&s.bar_half, par);                 // the first half's products are done with A
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+            uint32_t h8[8], l8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) split2(st[2 * (c + e)] * f, st[2 * (c + e) + 1] * f, h8[e], l8[e]);
+            tc::tmem_st8(lanes + kColA + c, h8);
+            tc::tmem_st8(lanes + kColA + 32 + c, l8);
+        }
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        named_bar_sync(1 + grp, kHalf);
+        if ((tid & (kHalf - 1)) == 0) {
+            tc::fence_after_sync();
+            constexpr uint32_t idesc = tc::idesc_f16(128, 2 * NB, false, false);
+#pragma unroll 1
+            for (int pass = 0; pass < 3; ++pass) {
+                const uint32_t acol = tmem + kColA + (pass == 0 ? 32 : 0);
+                const uint64_t bd = kq_desc((pass == 1 ? 2 : 0) + grp);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    tc::mma_ts(tmem + kColD, acol + kk * 8, bd + kk * 2, idesc, grp > 0 || pass > 0 || kk > 0);
+            }
+            tc::commit(grp ? &s.bar_in : &s.bar_half);
+        }
+        unsigned long long u[NB / 2];                         // rows 2p, 2p + 1 of column v
+        if (grp == 0) {
+            // ---- beta v of all nodes: the conv of channel v, all taps of four nodes in flight ----
+            const int c = 2 * a.n_qk * kDk + h * kDv + v;
+            const float4 w = reinterpret_cast<const float4*>(a.w)[c];
+            float4 win = reinterpret_cast<const float4*>(a.conv)[size_t(slot) * a.conv_dim + c];
+            const int ph = a.conv_phase ? a.conv_phase[slot] & 3 : 0;
+            if (ph & 1) win = make_float4(win.y, win.z, win.w, win.x);
+            if (ph & 2) win = make_float4(win.z, win.w, win.x, win.y);
+            const float* xv = x + c;
+#pragma unroll
+            for (int i0 = 0; i0 < NB; i0 += 4) {
+                float y[4];
+                if (i0 < n) {
+                    float t[4][4];
+                    int4 src[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        src[e] = s.src[min(i0 + e, n - 1)];
+                        t[e][3] = xv[src[e].x * a.x_stride];
+                        t[e][2] = xv[max(src[e].y, 0) * a.x_stride];
+                        t[e][1] = xv[max(src[e].z, 0) * a.x_stride];
+                        t[e][0] = xv[max(src[e].w, 0) * a.x_stride];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (src[e].w < 0) {                   // near a root: taps from the window
+                            t[e][0] = comp(win, ~src[e].w);
+                            if (src[e].z < 0) t[e][1] = comp(win, ~src[e].z);
+                            if (src[e].y < 0) t[e][2] = comp(win, ~src[e].y);
+                        }
+                        const float r = fmaf(w.w, t[e][3], fmaf(w.z, t[e][2], fmaf(w.y, t[e][1], w.x * t[e][0])));
+                        y[e] = i0 + e < n ? s.beta[i0 + e] * __fdividef(r, 1.f + expf(-r)) : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = 0.f;
+                }
+                u[i0 / 2] = pair(y[0], y[1]);
+                u[i0 / 2 + 1] = pair(y[2], y[3]);
+            }
+        } else {
+            // ---- coefficients of this head: rows i, eight columns j per step ----
+            for (int idx = v; idx < NB * (NB / 8); idx += kHalf) {
+                const int i = idx % NB, j0 = (idx / NB) * 8;
+                const unsigned long long word = i < n ? s.word[i] : 0ull;
+                const float ci = s.decay[i], bi = s.beta[i];
+                float m[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = j0 + e;
+                    m[e] = 0.f;
+                    float l = 0.f;
+                    if (word >> j & 1) {
+                        const float d = expf(ci - s.decay[j]);
+                        m[e] = d * s.gram[j][i] * (kLift * 0.08838834764831845f);       // 1 / sqrt(128)
+                        if (j < i) l = -bi * d * s.gram[i][j];
+                    }
+                    if (i >= (j & ~3)) s.low[low_off<NB>(j) + i] = l;
+                }
+                uint4 mh, ml;
+                split2(m[0], m[1], mh.x, ml.x);
+                split2(m[2], m[3], mh.y, ml.y);
+                split2(m[4], m[5], mh.z, ml.z);
+                split2(m[6], m[7], mh.w, ml.w);
+                const int at = tile_at(i, j0);
+                *reinterpret_cast<uint4*>(s.mix[0] + at) = mh;
+                *reinterpret_cast<uint4*>(s.mix[1] + at) = ml;
+            }
+            tc::fence_async_smem();
+        }
+        __syncthreads();
+        if (grp == 0) {
+            wait(&s.bar_in, par);
+            tc::fence_after_sync();
+            // ---- right-hand side: beta v - beta e^c S0^T k ----
+#pragma unroll
+            for (int c = 0; c < NB; c += 16) {
+                uint32_t d[16];
+                tc::tmem_ld16(lanes + kColD + c, d);
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float2 in = *reinterpret_cast<const float2*>(&s.in[c + e]);
+                    u[(c + e) / 2] = fma2(pair(__uint_as_float(d[e]) * back, __uint_as_float(d[e + 1]) * back), pair(in.x, in.y), u[(c + e) / 2]);
+                }
+            }
+            // ---- solve ----
+#pragma unroll
+            for (int j = 0; j < NB - 1; ++j) {
+                if (j % 4 == 0 && j >= n) break;
+                const float2 uu = halves(u[j / 2]);
+                const float uj = j & 1 ? uu.y : uu.x;
+                const unsigned long long u2 = pair(uj, uj);
+#pragma unroll
+                for (int i = j & ~3; i < NB; i += 4) {
+                    if (i + 3 <= j) continue;
+                    const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(&s.low[low_off<NB>(j) + i]);
+                    if (i + 1 > j) u[i / 2] = fma2(l.x, u2, u[i / 2]);
+                    u[i / 2 + 1] = fma2(l.y, u2, u[i / 2 + 1]);
+                }
+            }
+            // ---- u -> A ----
+            float mx = 0.f;
+#pragma unroll
+            for (int p = 0; p < NB / 2; ++p) {
+                const float2 x2 = halves(u[p]);
+                mx = fmaxf(mx, fmaxf(fabsf(x2.x), fabsf(x2.y)));
+            }
+            float uback;
+            const float uf = lift(mx, uback);
+            s.uback[v] = uback;
+#pragma unroll
+            for (int c = 0; c < NB / 2; c += 8) {
+                uint32_t h8[8], l8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 x2 = halves(u[c + e]);
+                    split2(x2.x * uf, x2.y * uf, h8[e], l8[e]);
+                }
+                tc::tmem_st8(lanes + kColA + c, h8);
+                tc::tmem_st8(lanes + kColA + 32 + c, l8);
+            }
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            named_bar_sync(1, kHalf);
+            if (tid == 0) {
+                tc::fence_after_sync();
+                // the last term of o, over D's k columns, which every thread of this group has read
+                constexpr uint32_t idesc = tc::idesc_f16(128, NB, false, false);
+#pragma unroll 1
+                for (int pass = 0; pass < 3; ++pass) {
+                    const uint32_t acol = tmem + kColA + (pass == 0 ? 32 : 0);
+                    const uint64_t bd = tc::smem_desc(smem_u32(s.mix[pass == 1 ? 1 : 0]), 16, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < NB / 16; ++kk) tc::mma_ts(tmem + kColD, acol + kk * 8, bd + kk * 2, idesc, pass > 0 || kk > 0);
+                }
+                tc::commit(&s.bar_out);
+            }
+        }
+        if (hi + 1 < a.heads) fetch(h + h_step);
+        __syncthreads();                                      // uback
+        wait(&s.bar_out, par);
+        tc::fence_after_sync();
+        // ---- o = e^c S0^T q / sqrt(128) + sum mix u: half the nodes per group ----
+        const float qs = s.back[v] * (kBack * 0.08838834764831845f), us = s.uback[v] * kBack;
+        float* o = a.o + (size_t(b) * a.max_nodes * a.n_v + h) * kDv + v;
+#pragma unroll
+        for (int c = 0; c < NB / 2; c += 8) {
+            const int i0 = grp * (NB / 2) + c;
+            if (i0 >= n) break;
+            uint32_t dq[8], du[8];
+            tc::tmem_ld8(lanes + kColD + NB + i0, dq);
+            tc::tmem_ld8(lanes + kColD + i0, du);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (ok && i0 + e < n)
+                    __stcs(o + size_t(i0 + e) * a.n_v * kDv,
+                           fmaf(__uint_as_float(dq[e]) * qs, s.grow[i0 + e], __uint_as_float(du[e]) * us));
+        }
+        tc::fence_before_sync();
+        __syncthreads();                                      // D, A and the head's tables may be rewritten
+        tc::fence_after_sync();
     }
+    if (warp == 1) tc::tmem_dealloc(tmem, kCols);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -392,11 +731,34 @@ __global__ void __launch_bounds__(256) gdn_tree_window_kernel(GdnTreeArgs a) {
     *ring = make_float4(out[0], out[1], out[2], out[3]);
 }
 
-size_t gdn_tree_smem_bytes() { return sizeof(TreeSmem); }
-const void* gdn_tree_kernel_ptr() { return reinterpret_cast<const void*>(&gdn_tree_kernel); }
+namespace {
+template <int NB>
+cudaError_t set_attr() {
+    return cudaFuncSetAttribute(gdn_tree_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tree_smem_bytes<NB>()));
+}
+template <int NB>
+void launch(const GdnTreeArgs& a, cudaStream_t st) {
+    gdn_tree_kernel<NB><<<dim3(unsigned(a.n_v / a.heads), unsigned(a.batch)), kThreads, tree_smem_bytes<NB>(), st>>>(a);
+}
+}  // namespace
 
-void launch_gdn_tree(const GdnTreeArgs& a, cudaStream_t st) {
-    gdn_tree_kernel<<<dim3(unsigned(a.n_v), unsigned(a.batch)), kThreads, gdn_tree_smem_bytes(), st>>>(a);
+cudaError_t gdn_tree_setup() {
+    cudaError_t e = set_attr<16>();
+    if (e == cudaSuccess) e = set_attr<32>();
+    if (e == cudaSuccess) e = set_attr<48>();
+    if (e == cudaSuccess) e = set_attr<64>();
+    return e;
+}
+
+void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
+    // one CTA per value head while that leaves SMs without a second CTA; else a key head's value heads share
+    // the preparation of its k and q rows
+    const int ratio = a.n_v / a.n_qk;
+    a.heads = a.batch * a.n_v <= 2 * sms ? 1 : ratio;
+    if (a.max_nodes <= 16) launch<16>(a, st);
+    else if (a.max_nodes <= 32) launch<32>(a, st);
+    else if (a.max_nodes <= 48) launch<48>(a, st);
+    else launch<64>(a, st);
 }
 
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st) {

@@ -354,11 +354,11 @@ struct GdnTreeArgs {
     int* err;
     size_t x_stride;
     int batch, max_nodes, n_v, n_qk, n_slots, head_map, conv_dim;
+    int heads;                   // verify: value heads of a CTA, 1 or n_v / n_qk (set by the launch)
     float eps_l2;
 };
-size_t gdn_tree_smem_bytes();
-const void* gdn_tree_kernel_ptr();
-void launch_gdn_tree(const GdnTreeArgs& a, cudaStream_t st);
+cudaError_t gdn_tree_setup();    // kernel attributes, once per device
+void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st);
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st);
 
 }  // namespace rl
