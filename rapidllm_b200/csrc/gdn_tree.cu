@@ -44,27 +44,45 @@ struct Conv4 {
 };
 __device__ __forceinline__ float comp(const float4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
-// SiLU(conv) of channels c0 .. c0+3 at a node: taps are the node, its parent, ... (src[0..3]; src[k] < 0:
-// that tap is window entry ~src[k]).
-__device__ __forceinline__ float4 conv_node(const Conv4& cv, const float* x, size_t row_stride, int4 src) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int s[4] = {src.w, src.z, src.y, src.x};       // oldest first
+// hardware exponential and quotient: within 2^-21 for the magnitudes that matter, 2 instructions instead of 20
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+
+// SiLU(conv) of channels c0 .. c0+3 at M nodes, all their taps requested before the first is used: taps are the
+// node, its parent, ... (src.x .. src.w; negative: window entry ~src).
+template <int M>
+__device__ __forceinline__ void conv_nodes(const Conv4& cv, const float* x, size_t row_stride, const int4 (&src)[M], float4 (&y)[M]) {
+    float4 t[M][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float4 t;
-        if (s[k] >= 0) {
-            t = *reinterpret_cast<const float4*>(x + s[k] * row_stride);
-        } else {
-            const int j = ~s[k];
-            t = make_float4(comp(cv.win[0], j), comp(cv.win[1], j), comp(cv.win[2], j), comp(cv.win[3], j));
-        }
-        acc[0] = fmaf(comp(cv.w[0], k), t.x, acc[0]);
-        acc[1] = fmaf(comp(cv.w[1], k), t.y, acc[1]);
-        acc[2] = fmaf(comp(cv.w[2], k), t.z, acc[2]);
-        acc[3] = fmaf(comp(cv.w[3], k), t.w, acc[3]);
+    for (int m = 0; m < M; ++m) {
+        t[m][3] = *reinterpret_cast<const float4*>(x + src[m].x * row_stride);
+        t[m][2] = *reinterpret_cast<const float4*>(x + max(src[m].y, 0) * row_stride);
+        t[m][1] = *reinterpret_cast<const float4*>(x + max(src[m].z, 0) * row_stride);
+        t[m][0] = *reinterpret_cast<const float4*>(x + max(src[m].w, 0) * row_stride);
     }
-    auto silu = [](float v) { return v / (1.f + expf(-v)); };
-    return make_float4(silu(acc[0]), silu(acc[1]), silu(acc[2]), silu(acc[3]));
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        if (src[m].w < 0) {                                   // near a root
+            const int s[3] = {src[m].w, src[m].z, src[m].y};
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                if (s[k] < 0) t[m][k] = make_float4(comp(cv.win[0], ~s[k]), comp(cv.win[1], ~s[k]), comp(cv.win[2], ~s[k]), comp(cv.win[3], ~s[k]));
+        }
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[0] = fmaf(comp(cv.w[0], k), t[m][k].x, a[0]);
+            a[1] = fmaf(comp(cv.w[1], k), t[m][k].y, a[1]);
+            a[2] = fmaf(comp(cv.w[2], k), t[m][k].z, a[2]);
+            a[3] = fmaf(comp(cv.w[3], k), t[m][k].w, a[3]);
+        }
+        y[m] = make_float4(silu(a[0]), silu(a[1]), silu(a[2]), silu(a[3]));
+    }
+}
+__device__ __forceinline__ float4 conv_node(const Conv4& cv, const float* x, size_t row_stride, int4 src) {
+    const int4 s[1] = {src};
+    float4 y[1];
+    conv_nodes(cv, x, row_stride, s, y);
+    return y[0];
 }
 
 // taps of a node: itself and its next three ancestors, then the window from its newest entry (3) down
@@ -97,22 +115,6 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float acc) {
     return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, acc))));
 }
 
-// ---- packed pairs of fp32 ----
-__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 halves(unsigned long long p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-    return f;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
 // x0, x1 as fp16 pairs: hi, and what hi leaves
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x0, x1);
@@ -132,32 +134,101 @@ constexpr float kLift = 4096.f, kBack = 1.f / 4096.f;
 
 constexpr int kThreads = 256, kHalf = kThreads / 2;
 
-// The triangular coefficients of the solve, by columns: entry (j, i), i > j, at off(j) + i; a column starts at
-// a multiple of four.
-template <int NB>
-__host__ __device__ constexpr int low_off(int j) {
-    const int g = j >> 2;
-    return 4 * (NB * g - 2 * g * (g - 1)) + (j & 3) * (NB - 4 * g) - 4 * g;
-}
 template <int NB>
 struct TreeSmem {
     static constexpr int kSub = 2 * NB * 128;                 // 64 dims of the rows [k; q], 128 bytes each
+    static constexpr int kPitch = NB + 4;                     // of the fp32 triangle: 16-byte rows on all banks
     alignas(1024) unsigned char kq[4][kSub];                  // hi dims 0-63, 64-127, lo dims 0-63, 64-127
-    alignas(1024) unsigned char mix[2][NB * 128];             // coefficients of u_j in o_i: hi, lo
-    alignas(16) float low[4 * (NB * NB / 4 - 2 * (NB / 4) * (NB / 4 - 1))];
-    float gram[NB][NB + 1];                                   // [i][j], j < i: k_i . k_j; [j][i], j <= i: q_i . k_j
+    union {
+        float v[NB][kDv];                                     // first: v of all nodes
+        struct {
+            alignas(1024) unsigned char inv[2][NB * 128];     // then: scratch of the inversion; T as tiles, hi and lo
+            union {
+                float tri[NB][kPitch];                        // L, inverted in place
+                alignas(1024) unsigned char mix[2][NB * 128]; // then: coefficients of u_j in o_i as tiles
+            };
+        };
+    };
     float decay[NB], grow[NB], beta[NB], in[NB];              // c_i, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
-    float amax[2][kDv], back[kDv], uback[kDv];
+    float amax[2][kDv];
     unsigned long long word[kMaxNodes];
     int parents[kMaxNodes];
     int4 src[NB];
-    uint64_t bar_gram, bar_half, bar_in, bar_out;
+    uint64_t bar_gram, bar_half, bar_in, bar_u, bar_out;
     uint32_t tmem_base;
 };
 template <int NB>
 constexpr size_t tree_smem_bytes() {
     // the Gram product takes its A operand as 128 rows, past the last tile's where there are fewer
     return (sizeof(TreeSmem<NB>) > 3 * TreeSmem<NB>::kSub + 128 * 128 ? sizeof(TreeSmem<NB>) : 3 * TreeSmem<NB>::kSub + 128 * 128) + 1024;
+}
+
+// t = (I + t)^-1 in place, t unit lower triangular with its strict lower part given; what lies above the 16 x 16
+// blocks of the diagonal is neither read nor written.  x: scratch of NB / 2 * 32 floats.  All threads; ends synchronised.
+//   [T1 0; -T2 L T1, T2] joins the inverses T1, T2 of two diagonal blocks with L below the first.
+template <int NB, int P>
+__device__ __forceinline__ float4 row_times(const float (&)[NB][P], const float* arow, const float* b, int b_pitch, int k0, int k1) {
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = k0; k < k1; k += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(arow + k);
+        const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float4 y = *reinterpret_cast<const float4*>(b + (k + e) * b_pitch);
+            c.x = fmaf(xs[e], y.x, c.x); c.y = fmaf(xs[e], y.y, c.y); c.z = fmaf(xs[e], y.z, c.z); c.w = fmaf(xs[e], y.w, c.w);
+        }
+    }
+    return c;
+}
+template <int NB, int P>
+__device__ __forceinline__ void invert_triangle(float (&t)[NB][P], float* x, int tid) {
+    if (tid < (NB + 31) / 32 * 32) {                          // a thread per column of a diagonal block
+        const int r0 = min(tid, NB - 1) & ~15, c = tid & 15;
+        float y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float r = i == c ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < i; j += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(&t[r0 + i][r0 + j]);
+                r = fmaf(-l.x, y[j], r);
+                if (j + 1 < i) r = fmaf(-l.y, y[j + 1], r);
+                if (j + 2 < i) r = fmaf(-l.z, y[j + 2], r);
+                if (j + 3 < i) r = fmaf(-l.w, y[j + 3], r);
+            }
+            y[i] = r;
+        }
+        __syncwarp();
+        if (tid < NB) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[r0 + i][r0 + c] = y[i];
+        }
+    }
+    __syncthreads();
+    if constexpr (NB >= 32) {                                 // 16 + 16
+        const int p = tid >> 6, i = (tid & 63) >> 2, j = (tid & 3) * 4, c0 = 32 * p, r0 = c0 + 16;
+        const bool mine = p < NB / 32;
+        if (mine) *reinterpret_cast<float4*>(x + p * 256 + i * 16 + j) = row_times(t, &t[r0 + i][c0], &t[c0][c0 + j], P, 0, 16);
+        __syncthreads();
+        if (mine) {
+            const float4 r = row_times(t, &t[r0 + i][r0], x + p * 256 + j, 16, 0, 16);
+            *reinterpret_cast<float4*>(&t[r0 + i][c0 + j]) = make_float4(-r.x, -r.y, -r.z, -r.w);
+        }
+        __syncthreads();
+    }
+    if constexpr (NB > 32) {                                  // 32 + the rest
+        constexpr int kRest = NB - 32;
+        const int i = tid >> 3, j = (tid & 7) * 4;
+        const bool mine = i < kRest;
+        if (mine) *reinterpret_cast<float4*>(x + i * 32 + j) = row_times(t, &t[32 + i][0], &t[0][j], P, j & ~15, 32);
+        __syncthreads();
+        if (mine) {
+            const float4 r = row_times(t, &t[32 + i][32], x + j, 32, 0, i < 16 ? 16 : kRest);
+            *reinterpret_cast<float4*>(&t[32 + i][j]) = make_float4(-r.x, -r.y, -r.z, -r.w);
+        }
+        __syncthreads();
+    }
 }
 
 // byte offset of fp16 element (row, d < 64) in a tile of 128-byte rows under the 128-byte swizzle
@@ -170,22 +241,24 @@ __device__ __forceinline__ int tile_at(int row, int d) { return row * 128 + (((d
 //
 // S0^T k and S0^T q of all nodes are one product per value head, D[v][row] = sum_d S0[d][v] [k; q][row][d],
 // with the state as the A operand in tensor memory (a thread reads column v of the state with coalesced loads
-// and stores it as TMEM lane v) and the rows [k; q] as the K-major B operand in shared memory; so is the last
-// term of o, with A = u.  Both must keep fp32's precision: operands are split into two fp16 terms (22 bits,
-// rows scaled by powers of two so that neither term leaves fp16's range) and hi lo + lo hi + hi hi accumulate
-// in fp32, the small ones first.  The solve between them is triangular: thread v keeps column v of
-// u in registers and, once u_j is known, takes it out of all later rows (right-looking, so the fused
-// multiply-adds of a step are independent; two rows per packed instruction).
+// and stores it as TMEM lane v) and the rows [k; q] as the K-major B operand in shared memory.  With
+// W = beta (V - e^c S0^T k) and T = (I + L)^-1, U = T W and the last term of o are products of the same form.
+// All must keep fp32's precision: operands are split into two fp16 terms (22 bits, rows scaled by powers of two
+// so that neither term leaves fp16's range) and hi lo + lo hi + hi hi accumulate in fp32, the small ones first.
+// T is formed in fp32 (16 x 16 blocks by substitution, then joined): n^3 / 6 products once instead of n^2 / 2
+// for each of the 128 columns, and no thread walks 64 dependent steps.  Its entries are k_i^T (a product of
+// contractions) k_j beta, at most max beta in magnitude, so a fixed scale serves them.
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     using Smem = TreeSmem<NB>;
     extern __shared__ unsigned char smem_raw[];
     Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    // tensor memory: A (32 columns hi, 32 lo: half the state's dims, later u), then D
-    constexpr uint32_t kColA = 0, kColD = 64;
-    constexpr uint32_t kCols = 64 + 2 * NB <= 128 ? 128 : 256;
+    // tensor memory: A (32 columns hi, 32 lo: half the state's dims, later W and U), D, and [k; q] k^T (lane = row)
+    constexpr uint32_t kColA = 0, kColD = 64, kColG = 64 + 2 * NB;
+    constexpr uint32_t kCols = 64 + 3 * NB <= 128 ? 128 : 256;
+    constexpr int kMine = NB / 2;                             // nodes of a thread's group
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int grp = warp >> 2;                                // half of the state's dims; 0: solves
+    const int grp = warp >> 2;                                // which half of the state's dims, of the nodes
     const int v = tid & (kDv - 1);                            // column of the state = TMEM lane
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
     const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
@@ -221,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         mbar_init(&s.bar_gram, 1);
         mbar_init(&s.bar_half, 1);
         mbar_init(&s.bar_in, 1);
+        mbar_init(&s.bar_u, 1);
         mbar_init(&s.bar_out, 1);
         mbar_fence_init();
     }
@@ -243,15 +317,24 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         const int c0 = (role == 0 ? (a.n_qk + hs) * kDk : hs * kDk) + lane * 4;
         Conv4 cv;
         cv.load(a, slot, c0);
-        for (int i = warp; i < NB; i += kThreads / 32) {
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (i < n) y = unit(conv_node(cv, x + c0, a.x_stride, s.src[i]), a.eps_l2, kLift);
-            uint2 hi, lo;
-            split2(y.x, y.y, hi.x, lo.x);
-            split2(y.z, y.w, hi.y, lo.y);
-            const int at = tile_at(role * NB + i, (lane * 4) & 63);
-            *reinterpret_cast<uint2*>(s.kq[lane >> 4] + at) = hi;
-            *reinterpret_cast<uint2*>(s.kq[2 + (lane >> 4)] + at) = lo;
+        for (int i0 = warp; i0 < NB; i0 += 2 * (kThreads / 32)) {
+            int4 src[2];
+            float4 y[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) src[m] = s.src[min(i0 + m * (kThreads / 32), n - 1)];
+            conv_nodes(cv, x + c0, a.x_stride, src, y);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int i = i0 + m * (kThreads / 32);
+                y[m] = unit(y[m], a.eps_l2, kLift);
+                if (i >= n) y[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+                uint2 hi, lo;
+                split2(y[m].x, y[m].y, hi.x, lo.x);
+                split2(y[m].z, y[m].w, hi.y, lo.y);
+                const int at = tile_at(role * NB + i, (lane * 4) & 63);
+                *reinterpret_cast<uint2*>(s.kq[lane >> 4] + at) = hi;
+                *reinterpret_cast<uint2*>(s.kq[2 + (lane >> 4)] + at) = lo;
+            }
         }
     }
     fetch(h0);
@@ -266,36 +349,12 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             const int pa = pass == 0 ? 2 : 0, pb = pass == 1 ? 2 : 0;     // lo hi, hi lo, hi hi
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-                tc::mma_ss(tmem + kColD, kq_desc(pa + (kk >> 2)) + (kk & 3) * 2, kq_desc(pb + (kk >> 2)) + (kk & 3) * 2, idesc,
+                tc::mma_ss(tmem + kColG, kq_desc(pa + (kk >> 2)) + (kk & 3) * 2, kq_desc(pb + (kk >> 2)) + (kk & 3) * 2, idesc,
                            pass > 0 || kk > 0);
         }
         tc::commit(&s.bar_gram);
     }
     wait(&s.bar_gram, 0);
-    tc::fence_after_sync();
-    {
-        const bool is_q = v >= NB;
-        const int i = is_q ? v - NB : v;
-#pragma unroll
-        for (int c = 0; c < NB / 2; c += 8) {
-            const int j0 = grp * (NB / 2) + c;
-            uint32_t g[8];
-            tc::tmem_ld8(lanes + kColD + j0, g);
-            tc::tmem_wait_ld();
-            if (v < 2 * NB) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = j0 + e;
-                    const float f = __uint_as_float(g[e]) * (kBack * kBack);
-                    if (!is_q && j < i) s.gram[i][j] = f;
-                    if (is_q && j <= i) s.gram[j][i] = f;
-                }
-            }
-            __syncwarp();
-        }
-    }
-    tc::fence_before_sync();
-    __syncthreads();
     tc::fence_after_sync();
 
 #pragma unroll 1
@@ -343,7 +402,6 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         __syncthreads();
         float back;
         const float f = lift(fmaxf(s.amax[0][v], s.amax[1][v]), back);
-        if (grp == 0) s.back[v] = back;
         if (grp == 1) wait(&s.bar_half, par);                 // the first half's products are done with A
 #pragma unroll
         for (int c = 0; c < 32; c += 8) {
@@ -369,156 +427,158 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             }
             tc::commit(grp ? &s.bar_in : &s.bar_half);
         }
-        unsigned long long u[NB / 2];                         // rows 2p, 2p + 1 of column v
-        if (grp == 0) {
-            // ---- beta v of all nodes: the conv of channel v, all taps of four nodes in flight ----
-            const int c = 2 * a.n_qk * kDk + h * kDv + v;
-            const float4 w = reinterpret_cast<const float4*>(a.w)[c];
-            float4 win = reinterpret_cast<const float4*>(a.conv)[size_t(slot) * a.conv_dim + c];
-            const int ph = a.conv_phase ? a.conv_phase[slot] & 3 : 0;
-            if (ph & 1) win = make_float4(win.y, win.z, win.w, win.x);
-            if (ph & 2) win = make_float4(win.z, win.w, win.x, win.y);
-            const float* xv = x + c;
+        // ---- v of all nodes: conv and SiLU by rows (a warp per node), handed over by columns ----
+        {
+            const int c0 = 2 * a.n_qk * kDk + h * kDv + lane * 4;
+            Conv4 cv;
+            cv.load(a, slot, c0);
+            for (int i0 = warp; i0 < n; i0 += 2 * (kThreads / 32)) {
+                int4 src[2];
+                float4 y[2];
 #pragma unroll
-            for (int i0 = 0; i0 < NB; i0 += 4) {
-                float y[4];
-                if (i0 < n) {
-                    float t[4][4];
-                    int4 src[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        src[e] = s.src[min(i0 + e, n - 1)];
-                        t[e][3] = xv[src[e].x * a.x_stride];
-                        t[e][2] = xv[max(src[e].y, 0) * a.x_stride];
-                        t[e][1] = xv[max(src[e].z, 0) * a.x_stride];
-                        t[e][0] = xv[max(src[e].w, 0) * a.x_stride];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (src[e].w < 0) {                   // near a root: taps from the window
-                            t[e][0] = comp(win, ~src[e].w);
-                            if (src[e].z < 0) t[e][1] = comp(win, ~src[e].z);
-                            if (src[e].y < 0) t[e][2] = comp(win, ~src[e].y);
-                        }
-                        const float r = fmaf(w.w, t[e][3], fmaf(w.z, t[e][2], fmaf(w.y, t[e][1], w.x * t[e][0])));
-                        y[e] = i0 + e < n ? s.beta[i0 + e] * __fdividef(r, 1.f + expf(-r)) : 0.f;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = 0.f;
-                }
-                u[i0 / 2] = pair(y[0], y[1]);
-                u[i0 / 2 + 1] = pair(y[2], y[3]);
+                for (int m = 0; m < 2; ++m) src[m] = s.src[min(i0 + m * (kThreads / 32), n - 1)];
+                conv_nodes(cv, x + c0, a.x_stride, src, y);
+                *reinterpret_cast<float4*>(&s.v[i0][lane * 4]) = y[0];
+                if (i0 + kThreads / 32 < n) *reinterpret_cast<float4*>(&s.v[i0 + kThreads / 32][lane * 4]) = y[1];
             }
-        } else {
-            // ---- coefficients of this head: rows i, eight columns j per step ----
-            for (int idx = v; idx < NB * (NB / 8); idx += kHalf) {
-                const int i = idx % NB, j0 = (idx / NB) * 8;
-                const unsigned long long word = i < n ? s.word[i] : 0ull;
-                const float ci = s.decay[i], bi = s.beta[i];
-                float m[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = j0 + e;
-                    m[e] = 0.f;
-                    float l = 0.f;
-                    if (word >> j & 1) {
-                        const float d = expf(ci - s.decay[j]);
-                        m[e] = d * s.gram[j][i] * (kLift * 0.08838834764831845f);       // 1 / sqrt(128)
-                        if (j < i) l = -bi * d * s.gram[i][j];
-                    }
-                    if (i >= (j & ~3)) s.low[low_off<NB>(j) + i] = l;
-                }
-                uint4 mh, ml;
-                split2(m[0], m[1], mh.x, ml.x);
-                split2(m[2], m[3], mh.y, ml.y);
-                split2(m[4], m[5], mh.z, ml.z);
-                split2(m[6], m[7], mh.w, ml.w);
-                const int at = tile_at(i, j0);
-                *reinterpret_cast<uint4*>(s.mix[0] + at) = mh;
-                *reinterpret_cast<uint4*>(s.mix[1] + at) = ml;
-            }
-            tc::fence_async_smem();
         }
         __syncthreads();
-        if (grp == 0) {
-            wait(&s.bar_in, par);
-            tc::fence_after_sync();
-            // ---- right-hand side: beta v - beta e^c S0^T k ----
+        float u[kMine];                                       // column v of W, later of U, at this group's nodes
 #pragma unroll
-            for (int c = 0; c < NB; c += 16) {
-                uint32_t d[16];
-                tc::tmem_ld16(lanes + kColD + c, d);
+        for (int e = 0; e < kMine; ++e) {
+            const int i = grp * kMine + e;
+            u[e] = i < n ? s.v[i][v] * s.beta[i] : 0.f;
+        }
+        __syncthreads();
+        // ---- this head's coefficients, half a row of [k; q] k^T per thread: L to shared memory, those of o kept ----
+        float m[kMine];
+        {
+            const bool is_q = v >= NB;
+            const int i = is_q ? v - NB : v;
+            const bool row = v < 2 * NB && i < n;
+            const unsigned long long word = row ? s.word[i] : 0ull;
+            const float ci = row ? s.decay[i] : 0.f;
+            const float f_ = is_q ? kBack * 0.08838834764831845f : (row ? s.beta[i] * kBack * kBack : 0.f);      // 1 / sqrt(128)
+#pragma unroll
+            for (int c = 0; c < kMine; c += 8) {
+                const int j0 = grp * kMine + c;
+                uint32_t g[8];
+                tc::tmem_ld8(lanes + kColG + j0, g);
                 tc::tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float2 in = *reinterpret_cast<const float2*>(&s.in[c + e]);
-                    u[(c + e) / 2] = fma2(pair(__uint_as_float(d[e]) * back, __uint_as_float(d[e + 1]) * back), pair(in.x, in.y), u[(c + e) / 2]);
+                for (int e = 0; e < 8; ++e) {
+                    const bool on = (word >> (j0 + e) & 1) && (is_q || j0 + e < i);
+                    m[c + e] = on ? expf(ci - s.decay[j0 + e]) * f_ * __uint_as_float(g[e]) : 0.f;
                 }
-            }
-            // ---- solve ----
-#pragma unroll
-            for (int j = 0; j < NB - 1; ++j) {
-                if (j % 4 == 0 && j >= n) break;
-                const float2 uu = halves(u[j / 2]);
-                const float uj = j & 1 ? uu.y : uu.x;
-                const unsigned long long u2 = pair(uj, uj);
-#pragma unroll
-                for (int i = j & ~3; i < NB; i += 4) {
-                    if (i + 3 <= j) continue;
-                    const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(&s.low[low_off<NB>(j) + i]);
-                    if (i + 1 > j) u[i / 2] = fma2(l.x, u2, u[i / 2]);
-                    u[i / 2 + 1] = fma2(l.y, u2, u[i / 2 + 1]);
+                if (v < NB) {
+                    *reinterpret_cast<float4*>(&s.tri[i][j0]) = make_float4(m[c], m[c + 1], m[c + 2], m[c + 3]);
+                    *reinterpret_cast<float4*>(&s.tri[i][j0 + 4]) = make_float4(m[c + 4], m[c + 5], m[c + 6], m[c + 7]);
                 }
+                __syncwarp();
             }
-            // ---- u -> A ----
+        }
+        __syncthreads();
+        invert_triangle<NB>(s.tri, reinterpret_cast<float*>(s.inv[0]), tid);
+        // ---- T -> tiles; W = beta v - beta e^c S0^T k -> A ----
+        for (int idx = tid; idx < NB * (NB / 8); idx += kThreads) {
+            const int i = idx % NB, j0 = (idx / NB) * 8;
+            float r[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(&s.tri[i][j0 + e]);
+                r[e] = q.x; r[e + 1] = q.y; r[e + 2] = q.z; r[e + 3] = q.w;
+            }
+            uint32_t th[4], tl[4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                split2(j0 + e <= i ? r[e] * kLift : 0.f, j0 + e + 1 <= i ? r[e + 1] * kLift : 0.f, th[e / 2], tl[e / 2]);
+            const int at = tile_at(i, j0);
+            *reinterpret_cast<uint4*>(s.inv[0] + at) = make_uint4(th[0], th[1], th[2], th[3]);
+            *reinterpret_cast<uint4*>(s.inv[1] + at) = make_uint4(tl[0], tl[1], tl[2], tl[3]);
+        }
+        tc::fence_async_smem();
+        wait(&s.bar_in, par);
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < kMine; c += 8) {
+            uint32_t d[8];
+            tc::tmem_ld8(lanes + kColD + grp * kMine + c, d);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[c + e] = fmaf(__uint_as_float(d[e]) * back, s.in[grp * kMine + c + e], u[c + e]);
+        }
+        // column v of W or U, both halves' largest magnitude scaled into place -> A; returns the scale's inverse
+        auto store_column = [&]() {
             float mx = 0.f;
 #pragma unroll
-            for (int p = 0; p < NB / 2; ++p) {
-                const float2 x2 = halves(u[p]);
-                mx = fmaxf(mx, fmaxf(fabsf(x2.x), fabsf(x2.y)));
-            }
-            float uback;
-            const float uf = lift(mx, uback);
-            s.uback[v] = uback;
+            for (int e = 0; e < kMine; ++e) mx = fmaxf(mx, fabsf(u[e]));
+            s.amax[grp][v] = mx;
+            __syncthreads();
+            float bk;
+            const float sc = lift(fmaxf(s.amax[0][v], s.amax[1][v]), bk);
 #pragma unroll
-            for (int c = 0; c < NB / 2; c += 8) {
-                uint32_t h8[8], l8[8];
+            for (int c = 0; c < kMine / 2; c += 4) {
+                uint32_t h4[4], l4[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 x2 = halves(u[c + e]);
-                    split2(x2.x * uf, x2.y * uf, h8[e], l8[e]);
-                }
-                tc::tmem_st8(lanes + kColA + c, h8);
-                tc::tmem_st8(lanes + kColA + 32 + c, l8);
+                for (int e = 0; e < 4; ++e) split2(u[2 * (c + e)] * sc, u[2 * (c + e) + 1] * sc, h4[e], l4[e]);
+                tc::tmem_st4(lanes + kColA + grp * (kMine / 2) + c, h4);
+                tc::tmem_st4(lanes + kColA + 32 + grp * (kMine / 2) + c, l4);
             }
             tc::tmem_wait_st();
             tc::fence_before_sync();
-            named_bar_sync(1, kHalf);
-            if (tid == 0) {
-                tc::fence_after_sync();
-                // the last term of o, over D's k columns, which every thread of this group has read
-                constexpr uint32_t idesc = tc::idesc_f16(128, NB, false, false);
+            __syncthreads();
+            return bk;
+        };
+        // D's k columns = A x tiles, both split: lo hi, hi lo, hi hi
+        auto product = [&](const unsigned char (&tiles)[2][NB * 128], uint64_t* done) {
+            tc::fence_after_sync();
+            constexpr uint32_t idesc = tc::idesc_f16(128, NB, false, false);
 #pragma unroll 1
-                for (int pass = 0; pass < 3; ++pass) {
-                    const uint32_t acol = tmem + kColA + (pass == 0 ? 32 : 0);
-                    const uint64_t bd = tc::smem_desc(smem_u32(s.mix[pass == 1 ? 1 : 0]), 16, 1024);
+            for (int pass = 0; pass < 3; ++pass) {
+                const uint32_t acol = tmem + kColA + (pass == 0 ? 32 : 0);
+                const uint64_t bd = tc::smem_desc(smem_u32(tiles[pass == 1 ? 1 : 0]), 16, 1024);
 #pragma unroll
-                    for (int kk = 0; kk < NB / 16; ++kk) tc::mma_ts(tmem + kColD, acol + kk * 8, bd + kk * 2, idesc, pass > 0 || kk > 0);
-                }
-                tc::commit(&s.bar_out);
+                for (int kk = 0; kk < NB / 16; ++kk) tc::mma_ts(tmem + kColD, acol + kk * 8, bd + kk * 2, idesc, pass > 0 || kk > 0);
+            }
+            tc::commit(done);
+        };
+        const float wback = store_column() * kBack;
+        if (tid == 0) product(s.inv, &s.bar_u);
+        if (v >= NB && v < 2 * NB) {
+#pragma unroll
+            for (int c = 0; c < kMine; c += 8) {
+                uint32_t mh[4], ml[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split2(m[c + 2 * e], m[c + 2 * e + 1], mh[e], ml[e]);
+                const int at = tile_at(v - NB, grp * kMine + c);
+                *reinterpret_cast<uint4*>(s.mix[0] + at) = make_uint4(mh[0], mh[1], mh[2], mh[3]);
+                *reinterpret_cast<uint4*>(s.mix[1] + at) = make_uint4(ml[0], ml[1], ml[2], ml[3]);
             }
         }
+        tc::fence_async_smem();
+        __syncwarp();
+        wait(&s.bar_u, par);
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < kMine; c += 8) {
+            uint32_t d[8];
+            tc::tmem_ld8(lanes + kColD + grp * kMine + c, d);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[c + e] = __uint_as_float(d[e]) * wback;
+        }
+        const float uback = store_column() * kBack;
+        if (tid == 0) product(s.mix, &s.bar_out);
         if (hi + 1 < a.heads) fetch(h + h_step);
-        __syncthreads();                                      // uback
+        __syncwarp();
         wait(&s.bar_out, par);
         tc::fence_after_sync();
-        // ---- o = e^c S0^T q / sqrt(128) + sum mix u: half the nodes per group ----
-        const float qs = s.back[v] * (kBack * 0.08838834764831845f), us = s.uback[v] * kBack;
+        // ---- o = e^c S0^T q / sqrt(128) + sum mix u ----
+        const float qs = back * (kBack * 0.08838834764831845f);
         float* o = a.o + (size_t(b) * a.max_nodes * a.n_v + h) * kDv + v;
 #pragma unroll
-        for (int c = 0; c < NB / 2; c += 8) {
-            const int i0 = grp * (NB / 2) + c;
+        for (int c = 0; c < kMine; c += 8) {
+            const int i0 = grp * kMine + c;
             if (i0 >= n) break;
             uint32_t dq[8], du[8];
             tc::tmem_ld8(lanes + kColD + NB + i0, dq);
@@ -528,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             for (int e = 0; e < 8; ++e)
                 if (ok && i0 + e < n)
                     __stcs(o + size_t(i0 + e) * a.n_v * kDv,
-                           fmaf(__uint_as_float(dq[e]) * qs, s.grow[i0 + e], __uint_as_float(du[e]) * us));
+                           fmaf(__uint_as_float(dq[e]) * qs, s.grow[i0 + e], __uint_as_float(du[e]) * uback));
         }
         tc::fence_before_sync();
         __syncthreads();                                      // D, A and the head's tables may be rewritten
