@@ -1637,6 +1637,7 @@ static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_w
     a->conv_dim = 2 * p->n_qk * p->dk + p->n_v * p->dv;
     if (!row_stride(p->qkv_stride, a->conv_dim, &a->x_stride))
         return fail(RL_ERR_RANGE, "qkv_stride %lld: at least a row, a multiple of 4", p->qkv_stride);
+    if (a->x_stride > 0x7fffffff / RL_TREE_MAX_NODES) return fail(RL_ERR_RANGE, "qkv_stride %lld: rows too far apart", p->qkv_stride);
     if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
     if (!S || !conv_window || !qkv || !conv_w || !beta || !g_log) return fail(RL_ERR_RANGE, "NULL pointer argument");
     if (!aligned16(S) || !aligned16(conv_window) || !aligned16(qkv) || !aligned16(conv_w))

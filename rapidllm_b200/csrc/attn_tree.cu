@@ -192,7 +192,8 @@ __device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const 
 
 __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) {
     extern __shared__ unsigned char smem_raw[];
-    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // (aligned by an offset, not by integer arithmetic on the pointer: the compiler keeps the loads shared-space ones)
+    Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.n_q / a.n_kv;
     griddep_launch();

@@ -48,16 +48,16 @@ __device__ __forceinline__ float comp(const float4& v, int i) { return i == 0 ? 
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + __expf(-v)); }
 
 // SiLU(conv) of channels c0 .. c0+3 at M nodes, all their taps requested before the first is used: taps are the
-// node, its parent, ... (src.x .. src.w; negative: window entry ~src).
+// node, its parent, ... (src.x .. src.w: offsets of their rows in floats; negative: window entry ~src).
 template <int M>
-__device__ __forceinline__ void conv_nodes(const Conv4& cv, const float* x, size_t row_stride, const int4 (&src)[M], float4 (&y)[M]) {
+__device__ __forceinline__ void conv_nodes(const Conv4& cv, const float* x, const int4 (&src)[M], float4 (&y)[M]) {
     float4 t[M][4];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-        t[m][3] = *reinterpret_cast<const float4*>(x + src[m].x * row_stride);
-        t[m][2] = *reinterpret_cast<const float4*>(x + max(src[m].y, 0) * row_stride);
-        t[m][1] = *reinterpret_cast<const float4*>(x + max(src[m].z, 0) * row_stride);
-        t[m][0] = *reinterpret_cast<const float4*>(x + max(src[m].w, 0) * row_stride);
+        t[m][3] = *reinterpret_cast<const float4*>(x + src[m].x);
+        t[m][2] = *reinterpret_cast<const float4*>(x + max(src[m].y, 0));
+        t[m][1] = *reinterpret_cast<const float4*>(x + max(src[m].z, 0));
+        t[m][0] = *reinterpret_cast<const float4*>(x + max(src[m].w, 0));
     }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
@@ -78,21 +78,21 @@ __device__ __forceinline__ void conv_nodes(const Conv4& cv, const float* x, size
         y[m] = make_float4(silu(a[0]), silu(a[1]), silu(a[2]), silu(a[3]));
     }
 }
-__device__ __forceinline__ float4 conv_node(const Conv4& cv, const float* x, size_t row_stride, int4 src) {
+__device__ __forceinline__ float4 conv_node(const Conv4& cv, const float* x, int4 src) {
     const int4 s[1] = {src};
     float4 y[1];
-    conv_nodes(cv, x, row_stride, s, y);
+    conv_nodes(cv, x, s, y);
     return y[0];
 }
 
 // taps of a node: itself and its next three ancestors, then the window from its newest entry (3) down
-__device__ __forceinline__ int4 conv_sources(int i, const int* parents) {
+__device__ __forceinline__ int4 conv_sources(int i, const int* parents, int row_stride) {
     int s[4];
     int at = i, past = 3;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (at >= 0) {
-            s[k] = at;
+            s[k] = at * row_stride;
             at = parents[at];
         } else {
             s[k] = ~past;
@@ -108,7 +108,7 @@ __device__ __forceinline__ float sum_warp(float v) {
     return v;
 }
 __device__ __forceinline__ float4 unit(float4 y, float eps, float extra) {
-    const float inv = extra / sqrtf(sum_warp(y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w) + eps);
+    const float inv = extra * rsqrtf(sum_warp(y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w) + eps);
     return make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float acc) {
@@ -149,7 +149,7 @@ struct TreeSmem {
             };
         };
     };
-    float decay[NB], grow[NB], beta[NB], in[NB];              // c_i, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
+    float decay[NB], grow[NB], beta[NB], in[NB];              // c_i log2 e, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
     float amax[2][kDv];
     unsigned long long word[kMaxNodes];
     int parents[kMaxNodes];
@@ -252,11 +252,14 @@ template <int NB>
 __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     using Smem = TreeSmem<NB>;
     extern __shared__ unsigned char smem_raw[];
-    Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // (aligned by an offset, not by integer arithmetic on the pointer: the compiler keeps the loads shared-space ones)
+    Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     // tensor memory: A (32 columns hi, 32 lo: half the state's dims, later W and U), D, and [k; q] k^T (lane = row)
     constexpr uint32_t kColA = 0, kColD = 64, kColG = 64 + 2 * NB;
     constexpr uint32_t kCols = 64 + 3 * NB <= 128 ? 128 : 256;
     constexpr int kMine = NB / 2;                             // nodes of a thread's group
+    constexpr int kConv = NB <= 16 ? 2 : 4;                   // nodes a warp has in flight
+    constexpr int kWarps = kThreads / 32;
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int grp = warp >> 2;                                // which half of the state's dims, of the nodes
     const int v = tid & (kDv - 1);                            // column of the state = TMEM lane
@@ -280,6 +283,20 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         for (int d = 0; d < kDk / 2; ++d) st[d] = __ldcs(S + d * kDv);
     };
 
+    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride;
+    // all that this CTA will read starts on its way into L2: the stages below wait for it one after the other
+    {
+        auto line = [](const float* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); };
+        const int rows = 2 + a.heads;                         // segments of 128 channels: q, k, v of the heads
+        auto channel = [&](int r) { return r == 0 ? hs * kDk : (r == 1 ? (a.n_qk + hs) * kDk : 2 * a.n_qk * kDk + (h0 + (r - 2) * h_step) * kDv); };
+        for (int i = tid; i < rows * n * 4; i += kThreads) line(x + (i >> 2) % n * a.x_stride + channel((i >> 2) / n) + (i & 3) * 32);
+        for (int i = tid; i < rows * 16; i += kThreads) {
+            line(a.w + size_t(channel(i >> 4)) * kTaps + (i & 15) * 32);
+            line(a.conv + (size_t(slot) * a.conv_dim + channel(i >> 4)) * kTaps + (i & 15) * 32);
+        }
+        for (int i = tid; i < a.heads * 512; i += kThreads)
+            line(a.S + (size_t(slot) * a.n_v + h0 + (i >> 9) * h_step) * (kDk * kDv) + (i & 511) * 32);
+    }
     if (warp == 0) {
         const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, n, lane, a.err);
         s.word[lane] = w.lo;
@@ -287,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         s.parents[lane] = w.parent_lo;
         s.parents[lane + 32] = w.parent_hi;
         __syncwarp();
-        for (int i = lane; i < n; i += 32) s.src[i] = conv_sources(i, s.parents);
+        for (int i = lane; i < n; i += 32) s.src[i] = conv_sources(i, s.parents, int(a.x_stride));
     } else if (warp == 1) {
         tc::tmem_alloc(&s.tmem_base, kCols);
     } else if (tid == 64) {
@@ -309,7 +326,6 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             ok = false;
         }
     };
-    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride;
 
     // ---- k and q of all nodes: conv, SiLU, unit length, split; a warp per node, 4 dims per lane ----
 #pragma unroll 1
@@ -317,15 +333,16 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         const int c0 = (role == 0 ? (a.n_qk + hs) * kDk : hs * kDk) + lane * 4;
         Conv4 cv;
         cv.load(a, slot, c0);
-        for (int i0 = warp; i0 < NB; i0 += 2 * (kThreads / 32)) {
-            int4 src[2];
-            float4 y[2];
+        for (int i0 = warp; i0 < NB; i0 += kConv * kWarps) {
+            int4 src[kConv];
+            float4 y[kConv];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) src[m] = s.src[min(i0 + m * (kThreads / 32), n - 1)];
-            conv_nodes(cv, x + c0, a.x_stride, src, y);
+            for (int m = 0; m < kConv; ++m) src[m] = s.src[min(i0 + m * kWarps, n - 1)];
+            conv_nodes(cv, x + c0, src, y);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int i = i0 + m * (kThreads / 32);
+            for (int m = 0; m < kConv; ++m) {
+                const int i = i0 + m * kWarps;
+                if (i >= NB) break;
                 y[m] = unit(y[m], a.eps_l2, kLift);
                 if (i >= n) y[m] = make_float4(0.f, 0.f, 0.f, 0.f);
                 uint2 hi, lo;
@@ -385,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             for (int z = 0; z < 2; ++z) {
                 const int i = lane + 32 * z;
                 if (i >= NB) break;
-                const float c = z ? c1 : c0, bt = z ? b1 : b0, e = expf(c);
+                const float c = (z ? c1 : c0) * 1.4426950408889634f, bt = z ? b1 : b0, e = fast_exp2(c);
                 s.decay[i] = c;
                 s.grow[i] = e;
                 s.beta[i] = bt;
@@ -432,14 +449,15 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             const int c0 = 2 * a.n_qk * kDk + h * kDv + lane * 4;
             Conv4 cv;
             cv.load(a, slot, c0);
-            for (int i0 = warp; i0 < n; i0 += 2 * (kThreads / 32)) {
-                int4 src[2];
-                float4 y[2];
+            for (int i0 = warp; i0 < n; i0 += kConv * kWarps) {
+                int4 src[kConv];
+                float4 y[kConv];
 #pragma unroll
-                for (int m = 0; m < 2; ++m) src[m] = s.src[min(i0 + m * (kThreads / 32), n - 1)];
-                conv_nodes(cv, x + c0, a.x_stride, src, y);
-                *reinterpret_cast<float4*>(&s.v[i0][lane * 4]) = y[0];
-                if (i0 + kThreads / 32 < n) *reinterpret_cast<float4*>(&s.v[i0 + kThreads / 32][lane * 4]) = y[1];
+                for (int m = 0; m < kConv; ++m) src[m] = s.src[min(i0 + m * kWarps, n - 1)];
+                conv_nodes(cv, x + c0, src, y);
+#pragma unroll
+                for (int m = 0; m < kConv; ++m)
+                    if (i0 + m * kWarps < n) *reinterpret_cast<float4*>(&s.v[i0 + m * kWarps][lane * 4]) = y[m];
             }
         }
         __syncthreads();
@@ -468,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const bool on = (word >> (j0 + e) & 1) && (is_q || j0 + e < i);
-                    m[c + e] = on ? expf(ci - s.decay[j0 + e]) * f_ * __uint_as_float(g[e]) : 0.f;
+                    m[c + e] = on ? fast_exp2(ci - s.decay[j0 + e]) * f_ * __uint_as_float(g[e]) : 0.f;
                 }
                 if (v < NB) {
                     *reinterpret_cast<float4*>(&s.tri[i][j0]) = make_float4(m[c], m[c + 1], m[c + 2], m[c + 3]);
@@ -658,16 +676,16 @@ __global__ void __launch_bounds__(kCommitThreads) gdn_tree_commit_kernel(GdnTree
         const int m = min(kChunk, len - t0);
         if (warp < m) {
             const int i = s.path[t0 + warp];
-            const int4 src = conv_sources(i, s.parents);
+            const int4 src = conv_sources(i, s.parents, int(a.x_stride));
             const int ck = (a.n_qk + hs) * kDk + lane * 4;
             Conv4 cv;
             cv.load(a, slot, ck);
-            const float4 y = unit(conv_node(cv, x + ck, a.x_stride, src), a.eps_l2, 1.f);
+            const float4 y = unit(conv_node(cv, x + ck, src), a.eps_l2, 1.f);
             *reinterpret_cast<float4*>(&s.k[warp][lane * 4]) = y;
             if (lane < kSliceCols / 4) {
                 const int c = 2 * a.n_qk * kDk + h * kDv + slice * kSliceCols + lane * 4;
                 cv.load(a, slot, c);
-                *reinterpret_cast<float4*>(&s.v[warp][lane * 4]) = conv_node(cv, x + c, a.x_stride, src);
+                *reinterpret_cast<float4*>(&s.v[warp][lane * 4]) = conv_node(cv, x + c, src);
             } else if (lane == 31) {
                 s.g[warp] = a.g_log[(size_t(b) * a.max_nodes + i) * a.n_v + h];
                 s.beta[warp] = a.beta[(size_t(b) * a.max_nodes + i) * a.n_v + h];
