@@ -7,6 +7,7 @@ raises RlError on a bad argument.  No CPU path exists here.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -390,55 +391,63 @@ def conv_ring_export(conv_ring, conv_phase):
 
 
 # ---- trees of drafted tokens: append, verify, commit (rl_b200.h has the format of parents, n_nodes, leaf) ----
+#
+# These calls take microseconds on the device, so their host side is kept short: one test per tensor, addresses
+# passed as plain integers.
 
 _TYPES = {torch.float32: _lib.RL_TYPE_F32, torch.float16: _lib.RL_TYPE_F16, torch.bfloat16: _lib.RL_TYPE_BF16}
+_F32, _I32 = torch.float32, torch.int32
 
 
-def _here(**tensors):
-    """Every tensor is on the current CUDA device (the one whose current stream the call goes to)."""
-    dev = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != dev):
-            raise _lib.RlError(6, f"{name}: need a tensor on the current device cuda:{dev}, got one on {t.device}")
+def _stream_of(dev):
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _shape(t, shape, name):
-    if t is not None and tuple(t.shape) != tuple(shape):
-        raise _lib.RlError(6, f"{name}: need shape {tuple(shape)}, got {tuple(t.shape)}")
+def _arg(t, dtype, shape, dev, name):
+    """Address of a contiguous tensor of that type and shape on device `dev` (the current one, whose current stream
+    the call goes to); None for None."""
+    if t is None:
+        return None
+    if t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    raise _lib.RlError(6, f"{name}: need a contiguous {dtype} tensor of shape {tuple(shape)} on the current device cuda:{dev}, "
+                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _rows(t, name):
-    """fp32 [batch][rows]..., dense inside a row, rows at one distance: that distance in floats."""
-    if t.dtype != torch.float32:
-        raise _lib.RlError(6, f"{name}: need fp32")
-    inner = 1
-    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
-        if size > 1 and stride != inner:
+def _needed(t, *rest):
+    if t is None:
+        raise _lib.RlError(6, f"{rest[-1]}: is None")
+    return _arg(t, *rest)
+
+
+def _rows(t, shape, dev, name):
+    """Address of fp32 [batch][rows]..., dense inside a row, rows at one distance; and that distance in floats."""
+    if t is None or t.get_device() != dev or t.dtype is not _F32 or t.shape != shape:
+        raise _lib.RlError(6, f"{name}: need a {_F32} tensor of shape {tuple(shape)} on the current device cuda:{dev}")
+    strides, inner = t.stride(), 1
+    for d in range(len(shape) - 1, 1, -1):
+        if shape[d] > 1 and strides[d] != inner:
             raise _lib.RlError(6, f"{name}: a row must be contiguous")
-        inner *= size
-    B, T = t.shape[:2]
-    row = t.stride(1) if T > 1 else (t.stride(0) if B > 1 else inner)
-    if B > 1 and T > 1 and t.stride(0) != T * row:
+        inner *= shape[d]
+    return t.data_ptr(), _row_distance(shape, strides, inner, name)
+
+
+def _row_distance(shape, strides, inner, name):
+    row = strides[1] if shape[1] > 1 else (strides[0] if shape[0] > 1 else inner)
+    if shape[0] > 1 and shape[1] > 1 and strides[0] != shape[1] * row:
         raise _lib.RlError(6, f"{name}: the rows of all sequences must be at one distance")
     return row
 
 
-def _tree(parents, n_nodes, batch, nodes):
-    _need(parents, torch.int32, "parents")
-    _need(n_nodes, torch.int32, "n_nodes")
-    _shape(parents, (batch, nodes), "parents")
-    _shape(n_nodes, (batch,), "n_nodes")
-
-
-def _pools(k_pool, v_pool, page_table, batch):
-    _need(k_pool, torch.float16, "k_pool")
-    _need(v_pool, torch.float16, "v_pool")
-    _need(page_table, torch.int32, "page_table")
-    _shape(v_pool, k_pool.shape, "v_pool")
-    if k_pool.dim() != 3 or k_pool.shape[2] != PAGE_TOKENS * HEAD_DIM:
+def _pools(k_pool, v_pool, page_table, batch, dev):
+    shape = k_pool.shape
+    if len(shape) != 3 or shape[2] != PAGE_TOKENS * HEAD_DIM:
         raise _lib.RlError(6, "k_pool: need [n_pages][n_kv][64 * 256] (new_pool)")
-    if page_table.dim() != 2 or page_table.shape[0] != batch:
+    if page_table.dim() != 2:
         raise _lib.RlError(6, f"page_table: need [{batch}][max_pages]")
+    pages = page_table.shape[1]
+    return (shape[0], shape[1], pages, _needed(k_pool, torch.float16, shape, dev, "k_pool"),
+            _needed(v_pool, torch.float16, shape, dev, "v_pool"), _needed(page_table, _I32, (batch, pages), dev, "page_table"))
 
 
 def attn_qk_append(qg, k, v, k_pool, v_pool, page_table, pos, q_norm=None, k_norm=None, parents=None, n_nodes=None,
@@ -450,39 +459,40 @@ def attn_qk_append(qg, k, v, k_pool, v_pool, page_table, pos, q_norm=None, k_nor
     ranges of one projection or dense; pos int32 [batch].  Row t is rotated by pos[b] + t, with parents
     [batch][n_tok] (n_tok <= 64) by pos[b] + the node's depth.  Returns q of q_dtype (or of q_out) and the
     gate, None without want_gate.  Rows behind n_nodes[b] are left as they are."""
+    dev = torch.cuda.current_device()
     batch, n_tok, n_q, two_hd = qg.shape
-    n_kv = k_pool.shape[1]
-    _here(qg=qg, k=k, v=v, k_pool=k_pool, v_pool=v_pool, page_table=page_table, pos=pos, q_norm=q_norm, k_norm=k_norm,
-          parents=parents, n_nodes=n_nodes, q_out=q_out, gate_out=gate_out)
-    _pools(k_pool, v_pool, page_table, batch)
-    _need(pos, torch.int32, "pos")
-    _shape(pos, (batch,), "pos")
-    _shape(k, (batch, n_tok, n_kv, HEAD_DIM), "k")
-    _shape(v, (batch, n_tok, n_kv, HEAD_DIM), "v")
-    _tree(parents, n_nodes, batch, n_tok)
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _need(t, torch.float32, name)
-        _shape(t, (HEAD_DIM,), name)
     if two_hd != 2 * HEAD_DIM:
         raise _lib.RlError(4, f"qg: rows of {two_hd} per head, only 512")
+    n_pages, n_kv, pages, kp, vp, table = _pools(k_pool, v_pool, page_table, batch, dev)
+    qg_p, qg_row = _rows(qg, qg.shape, dev, "qg")
+    k_p, k_row = _rows(k, (batch, n_tok, n_kv, HEAD_DIM), dev, "k")
+    v_p, v_row = _rows(v, (batch, n_tok, n_kv, HEAD_DIM), dev, "v")
+    shape = (batch, n_tok, n_q, HEAD_DIM)
     if q_out is None:
-        q_out = torch.empty(batch, n_tok, n_q, HEAD_DIM, dtype=q_dtype, device=qg.device)
+        q_out = torch.empty(shape, dtype=q_dtype, device=qg.device)
     if q_out.dtype not in _TYPES:
         raise _lib.RlError(4, f"q_out: {q_out.dtype} unknown")
-    _need(q_out, q_out.dtype, "q_out")
-    _shape(q_out, (batch, n_tok, n_q, HEAD_DIM), "q_out")
     if not want_gate:
         gate_out = None
     elif gate_out is None:
-        gate_out = torch.empty(batch, n_tok, n_q, HEAD_DIM, dtype=torch.float32, device=qg.device)
-    _need(gate_out, torch.float32, "gate_out")
-    _shape(gate_out, (batch, n_tok, n_q, HEAD_DIM), "gate_out")
-    p = _lib.AttnQkAppendParams(n_q, n_kv, HEAD_DIM, rotary_dim, batch, n_tok, PAGE_TOKENS, k_pool.shape[0],
-                                page_table.shape[1], _TYPES[q_out.dtype], theta, eps, _rows(qg, "qg"), _rows(k, "k"),
-                                _rows(v, "v"))
-    check(lib().rl_attn_qk_append(_p(k_pool), _p(v_pool), _p(page_table), _p(pos), _p(parents), _p(n_nodes), _p(qg),
-                                  _p(k), _p(v), _p(q_norm), _p(k_norm), _p(q_out), _p(gate_out), C.byref(p), _stream()))
+        gate_out = torch.empty(shape, dtype=_F32, device=qg.device)
+    p = _lib.AttnQkAppendParams(n_q, n_kv, HEAD_DIM, rotary_dim, batch, n_tok, PAGE_TOKENS, n_pages, pages,
+                                _TYPES[q_out.dtype], theta, eps, qg_row, k_row, v_row)
+    check(lib().rl_attn_qk_append(kp, vp, table, _needed(pos, _I32, (batch,), dev, "pos"),
+                                  _arg(parents, _I32, (batch, n_tok), dev, "parents"), _arg(n_nodes, _I32, (batch,), dev, "n_nodes"),
+                                  qg_p, k_p, v_p, _arg(q_norm, _F32, (HEAD_DIM,), dev, "q_norm"),
+                                  _arg(k_norm, _F32, (HEAD_DIM,), dev, "k_norm"), _arg(q_out, q_out.dtype, shape, dev, "q_out"),
+                                  _arg(gate_out, _F32, shape, dev, "gate_out"), p, _stream_of(dev)))
     return q_out, gate_out
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_tree_plan(dev, *fields):
+    p = _lib.AttnTreeParams(*fields)
+    need = lib().rl_attn_tree_workspace_bytes(p)
+    if need == 0:
+        raise _lib.RlError(6, lib().rl_last_error().decode())
+    return p, need
 
 
 def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=None, gate=None, max_seq_len=None, out=None,
@@ -492,43 +502,34 @@ def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=Non
 
     q fp32, fp16 or bf16 [batch][nodes][n_q][256]; gate fp32 of that shape, dense or strided (qg[..., 256:] as
     it lies); out fp16 or bf16 (default: q's type, fp16 for fp32).  parents None = chains."""
-    batch, nodes, n_q, hd = q.shape
-    n_kv = k_pool.shape[1]
-    _here(q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, base_len=base_len, parents=parents, n_nodes=n_nodes,
-          gate=gate, out=out, workspace=workspace)
-    _pools(k_pool, v_pool, page_table, batch)
-    _tree(parents, n_nodes, batch, nodes)
-    _need(base_len, torch.int32, "base_len")
-    _shape(base_len, (batch,), "base_len")
+    dev = torch.cuda.current_device()
+    shape = q.shape
+    batch, nodes, n_q, hd = shape
+    n_pages, n_kv, pages, kp, vp, table = _pools(k_pool, v_pool, page_table, batch, dev)
     if q.dtype not in _TYPES:
         raise _lib.RlError(4, f"q: {q.dtype} unknown")
-    _need(q, q.dtype, "q")
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or (torch.float16 if q.dtype == torch.float32 else q.dtype), device=q.device)
+        out = torch.empty(shape, dtype=out_dtype or (torch.float16 if q.dtype is _F32 else q.dtype), device=q.device)
     if out.dtype not in _TYPES:
         raise _lib.RlError(4, f"out: {out.dtype} unknown")
-    _need(out, out.dtype, "out")
-    _shape(out, q.shape, "out")
     row = head = 0
+    gate_p = None
     if gate is not None:
-        _shape(gate, q.shape, "gate")
-        if gate.dtype != torch.float32 or gate.stride(3) != 1:
-            raise _lib.RlError(6, "gate: need fp32, contiguous inside a head")
-        head = gate.stride(2) if n_q > 1 else hd
-        row = gate.stride(1) if nodes > 1 else (gate.stride(0) if batch > 1 else 0)
-        if batch > 1 and nodes > 1 and gate.stride(0) != nodes * row:
-            raise _lib.RlError(6, "gate: the rows of all sequences must be at one distance")
-    p = _lib.AttnTreeParams(n_q, n_kv, hd, batch, nodes, PAGE_TOKENS, k_pool.shape[0], page_table.shape[1],
-                            page_table.shape[1] * PAGE_TOKENS if max_seq_len is None else max_seq_len, _TYPES[q.dtype],
-                            _TYPES[out.dtype], row, head)
-    need = lib().rl_attn_tree_workspace_bytes(C.byref(p))
-    if need == 0:
-        raise _lib.RlError(6, lib().rl_last_error().decode())
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(lib().rl_attn_tree(_p(k_pool), _p(v_pool), _p(page_table), _p(base_len), _p(parents), _p(n_nodes), _p(q),
-                             _p(gate), _p(out), _p(workspace), workspace.numel() * workspace.element_size(), C.byref(p),
-                             _stream()))
+        strides = gate.stride()
+        if gate.get_device() != dev or gate.dtype is not _F32 or gate.shape != shape or strides[3] != 1:
+            raise _lib.RlError(6, f"gate: need a {_F32} tensor of shape {tuple(shape)} on the current device cuda:{dev}, contiguous inside a head")
+        head = strides[2] if n_q > 1 else hd
+        row = _row_distance(shape, strides, head * n_q, "gate")
+        gate_p = gate.data_ptr()
+    p, need = _attn_tree_plan(dev, n_q, n_kv, hd, batch, nodes, PAGE_TOKENS, n_pages, pages,
+                              pages * PAGE_TOKENS if max_seq_len is None else max_seq_len, _TYPES[q.dtype], _TYPES[out.dtype], row, head)
+    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if size < need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    check(lib().rl_attn_tree(kp, vp, table, _needed(base_len, _I32, (batch,), dev, "base_len"),
+                             _arg(parents, _I32, (batch, nodes), dev, "parents"), _arg(n_nodes, _I32, (batch,), dev, "n_nodes"),
+                             _arg(q, q.dtype, shape, dev, "q"), gate_p, _arg(out, out.dtype, shape, dev, "out"),
+                             _arg(workspace, workspace.dtype, workspace.shape, dev, "workspace"), size, p, _stream_of(dev)))
     return out
 
 
@@ -536,46 +537,37 @@ def kv_tree_commit(k_pool, v_pool, page_table, base_len, parents, leaf):
     """Keep the path to node leaf[b] (int32 [batch], -1 = nothing) of each sequence's tree: its K and V rows move
     to positions base_len[b], base_len[b] + 1, ...  Returns the paths' lengths, int32 [batch].  parents int32
     [batch][nodes], or the number of nodes for chains."""
+    dev = torch.cuda.current_device()
     batch = leaf.shape[0]
-    nodes = parents if isinstance(parents, int) else parents.shape[1]
-    parents = None if isinstance(parents, int) else parents
-    _here(k_pool=k_pool, v_pool=v_pool, page_table=page_table, base_len=base_len, parents=parents, leaf=leaf)
-    _pools(k_pool, v_pool, page_table, batch)
-    _tree(parents, None, batch, nodes)
-    for t, name in ((base_len, "base_len"), (leaf, "leaf")):
-        _need(t, torch.int32, name)
-        _shape(t, (batch,), name)
-    n_accept = torch.empty(batch, dtype=torch.int32, device=leaf.device)
-    p = _lib.KvTreeCommitParams(k_pool.shape[1], HEAD_DIM, batch, nodes, PAGE_TOKENS, k_pool.shape[0], page_table.shape[1])
-    check(lib().rl_kv_tree_commit(_p(k_pool), _p(v_pool), _p(page_table), _p(base_len), _p(parents), _p(leaf),
-                                  _p(n_accept), C.byref(p), _stream()))
+    chain = isinstance(parents, int)
+    nodes = parents if chain else parents.shape[1]
+    n_pages, n_kv, pages, kp, vp, table = _pools(k_pool, v_pool, page_table, batch, dev)
+    n_accept = torch.empty_like(leaf)
+    p = _lib.KvTreeCommitParams(n_kv, HEAD_DIM, batch, nodes, PAGE_TOKENS, n_pages, pages)
+    check(lib().rl_kv_tree_commit(kp, vp, table, _needed(base_len, _I32, (batch,), dev, "base_len"),
+                                  None if chain else _needed(parents, _I32, (batch, nodes), dev, "parents"),
+                                  _needed(leaf, _I32, (batch,), dev, "leaf"), n_accept.data_ptr(), p, _stream_of(dev)))
     return n_accept
 
 
-def _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_nodes, n_qk, slot_ids, head_map,
-                     eps_l2, **more):
+def _gdn_tree_args(dev, S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, third, name, n_qk, slot_ids, head_map,
+                   eps_l2):
     n_slots, n_v, dk, dv = S.shape
     batch, nodes, dim = qkv.shape
-    _here(S=S, conv_window=conv_window, conv_phase=conv_phase, qkv=qkv, conv_w=conv_w, beta=beta, g_log=g_log,
-          parents=parents, n_nodes=n_nodes, slot_ids=slot_ids, **more)
-    for t, n in ((S, "S"), (conv_window, "conv_window"), (conv_w, "conv_w"), (beta, "beta"), (g_log, "g_log")):
-        _need(t, torch.float32, n)
-    _tree(parents, n_nodes, batch, nodes)
     if dim != 2 * n_qk * dk + n_v * dv:
         raise _lib.RlError(6, f"qkv: rows of {dim} channels, {n_qk} key and {n_v} value heads need {2 * n_qk * dk + n_v * dv}")
-    _shape(conv_window, (n_slots, dim, 4), "conv_window")
-    _shape(conv_w, (dim, 4), "conv_w")
-    _shape(beta, (batch, nodes, n_v), "beta")
-    _shape(g_log, (batch, nodes, n_v), "g_log")
-    _need(conv_phase, torch.int32, "conv_phase")
-    _shape(conv_phase, (n_slots,), "conv_phase")
-    _need(slot_ids, torch.int32, "slot_ids")
-    _shape(slot_ids, (batch,), "slot_ids")
     if slot_ids is None and batch > n_slots:
         raise _lib.RlError(6, f"{batch} sequences in {n_slots} slots")
     if head_map is None:
         head_map = _lib.RL_HEADS_PER_VALUE if n_qk == n_v else _lib.RL_HEADS_GROUPED
-    return _lib.GdnTreeParams(n_v, n_qk, dk, dv, 4, batch, nodes, n_slots, head_map, eps_l2, _rows(qkv, "qkv"))
+    qkv_p, row = _rows(qkv, qkv.shape, dev, "qkv")
+    gates = (batch, nodes, n_v)
+    return (_lib.GdnTreeParams(n_v, n_qk, dk, dv, 4, batch, nodes, n_slots, head_map, eps_l2, row),
+            (_needed(S, _F32, S.shape, dev, "S"), _needed(conv_window, _F32, (n_slots, dim, 4), dev, "conv_window"),
+             _arg(conv_phase, _I32, (n_slots,), dev, "conv_phase"), _arg(slot_ids, _I32, (batch,), dev, "slot_ids"),
+             _arg(parents, _I32, (batch, nodes), dev, "parents"), _arg(third, _I32, (batch,), dev, name), qkv_p,
+             _needed(conv_w, _F32, (dim, 4), dev, "conv_w"), _needed(beta, _F32, gates, dev, "beta"),
+             _needed(g_log, _F32, gates, dev, "g_log")))
 
 
 def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk, n_nodes=None, slot_ids=None,
@@ -584,24 +576,23 @@ def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk
     and conv_window [n_slots][conv_dim][4] are only read.  conv_phase int32 [n_slots] (rings, see gdn_decode) or
     None (shifted windows, conv1d_update's state).  qkv fp32 [batch][nodes][conv_dim] (rows may be a column range),
     beta, g_log [batch][nodes][n_v].  Returns o fp32 [batch][nodes][n_v][128]."""
-    p = _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_nodes, n_qk, slot_ids, head_map,
-                         eps_l2, out=out)
+    dev = torch.cuda.current_device()
+    p, args = _gdn_tree_args(dev, S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_nodes, "n_nodes", n_qk,
+                             slot_ids, head_map, eps_l2)
     shape = (qkv.shape[0], qkv.shape[1], S.shape[1], S.shape[3])
-    o = torch.empty(shape, dtype=torch.float32, device=S.device) if out is None else out
-    _need(o, torch.float32, "out")
-    _shape(o, shape, "out")
-    check(lib().rl_gdn_tree(_p(S), _p(conv_window), _p(conv_phase), _p(slot_ids), _p(parents), _p(n_nodes), _p(qkv),
-                            _p(conv_w), _p(beta), _p(g_log), _p(o), C.byref(p), _stream()))
-    return o
+    if out is None:
+        out = torch.empty(shape, dtype=_F32, device=S.device)
+    check(lib().rl_gdn_tree(*args, _arg(out, _F32, shape, dev, "out"), p, _stream_of(dev)))
+    return out
 
 
 def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, n_qk, slot_ids=None,
                     head_map=None, eps_l2=1e-6):
     """Advance S and conv_window of each sequence's slot by the path to node leaf[b] (-1 = nothing), in place, with
     gdn_tree's inputs; conv_phase stays.  slot_ids must be distinct."""
-    p = _gdn_tree_params(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, None, n_qk, slot_ids, head_map,
-                         eps_l2, leaf=leaf)
-    _need(leaf, torch.int32, "leaf")
-    _shape(leaf, (qkv.shape[0],), "leaf")
-    check(lib().rl_gdn_tree_commit(_p(S), _p(conv_window), _p(conv_phase), _p(slot_ids), _p(parents), _p(leaf), _p(qkv),
-                                   _p(conv_w), _p(beta), _p(g_log), C.byref(p), _stream()))
+    dev = torch.cuda.current_device()
+    p, args = _gdn_tree_args(dev, S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, "leaf", n_qk, slot_ids,
+                             head_map, eps_l2)
+    if leaf is None:
+        raise _lib.RlError(6, "leaf: is None")
+    check(lib().rl_gdn_tree_commit(*args, p, _stream_of(dev)))
