@@ -471,7 +471,8 @@ size_t rl_attn_tree_workspace_bytes(const rl_attn_tree_params* p);
 /* rl_attn_decode for every node of a tree: node i of sequence b attends to the cache rows [0, base_len[b])
  * and to the rows base_len[b] + j of its ancestors j and itself (already appended), softmax scale 1/16,
  * o *= sigmoid(gate) when gate != NULL.  With parents == NULL this is the causal verify of a ragged batch.
- *   q [batch][max_nodes][n_q][256];  gate fp32, element (row, head, d) at row * gate_row + head * gate_head + d
+ *   q [batch][max_nodes][n_q][256];  gate fp32, element (row, head, d) at row * gate_row + head * gate_head + d;
+ *     q, o and workspace 32-byte aligned
  *   o [batch][max_nodes][n_q][256] in 16 bits: a mean of fp16 values times a gate in (0, 1), it fits fp16,
  *     and the probabilities meet V as fp16, so 32 bits would carry no more
  * The V rows of all nodes of a sequence must be finite (one that is not reaches its siblings too); K rows

@@ -1554,9 +1554,10 @@ int rl_attn_tree(const void* k_pool, const void* v_pool, const int32_t* page_tab
         return fail(RL_ERR_RANGE, "gate strides %lld %lld: at least a row and a head, multiples of 4", p->gate_row, p->gate_head);
     if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
     if (!k_pool || !v_pool || !page_table || !base_len || !q || !o || !workspace) return fail(RL_ERR_RANGE, "NULL pointer argument");
-    if (reinterpret_cast<uintptr_t>(k_pool) % 128 || reinterpret_cast<uintptr_t>(v_pool) % 128 || !aligned16(q) ||
-        !aligned16(gate) || !aligned16(o) || !aligned16(workspace))
-        return fail(RL_ERR_RANGE, "pools must be 128-byte aligned, q, gate, o and workspace 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(k_pool) % 128 || reinterpret_cast<uintptr_t>(v_pool) % 128 ||
+        reinterpret_cast<uintptr_t>(q) % 32 || reinterpret_cast<uintptr_t>(o) % 32 || reinterpret_cast<uintptr_t>(workspace) % 32 ||
+        !aligned16(gate))
+        return fail(RL_ERR_RANGE, "pools must be 128-byte aligned, q, o and workspace 32-byte, gate 16-byte");
     DevInfo* d;
     if (int st = dev_info(&d)) return st;
     const AttnTreePlan pl = attn_tree_plan(p, step_sms(d->sms));

@@ -41,8 +41,9 @@ constexpr int kSliceBytes = kPageTokens * kHeadDim * 2;
 constexpr int kGroupThreads = 256, kSoftmaxThreads = 512, kThreads = 608;
 constexpr int kWarpLoader = 16, kWarpQK = 17, kWarpPV = 18;
 constexpr uint32_t kTmemCols = 512;
-// tensor memory columns: S [0,64), two P buffers [64,128), O [128,384), Q (fp16 pairs) [384,512)
-constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kColQ = 384;
+// tensor memory columns: two S buffers [0,128), O [128,384), Q (fp16 pairs) [384,512).  The P of a page replaces the
+// first 32 columns of its own S, so that the next page's S is computed while this one is exponentiated.
+constexpr uint32_t kColS = 0, kColO = 128, kColQ = 384;
 constexpr float kRescaleThreshold = 8.f;          // log2 units
 constexpr float kNoMax = -1e30f;                   // of a row that has seen nothing; scores are below 2^8 * 65504 * 256
 constexpr int kMaxBatch = 512;
@@ -56,15 +57,16 @@ struct Segment {
 // units and segments of the sequences before b; entry `batch` holds the totals
 struct Prefix {
     int unit[kMaxBatch + 1], seg[kMaxBatch + 1];
+    int base[kMaxBatch], nodes[kMaxBatch];
 };
 
 struct Seq {
     int base, nodes, tiles, row_tiles;
 };
-__device__ __forceinline__ Seq sequence(const AttnTreeArgs& a, int b, int* err) {
+__device__ __forceinline__ Seq sequence(const AttnTreeArgs& a, int base, int nodes, int* err) {
     Seq q;
-    q.nodes = tree::node_count(a.n_nodes, b, a.max_nodes, err);
-    q.base = a.base_len[b];
+    q.nodes = nodes;
+    q.base = base;
     if (q.base < 0 || (long long)q.base + q.nodes > a.max_len) {
         set_err(err, DEV_ERR_BAD_LEN);
         q.nodes = 0;
@@ -80,7 +82,9 @@ __device__ __forceinline__ void build_prefix(Prefix& p, const AttnTreeArgs& a, i
         const int b = b0 + lane;
         int u = 0, g = 0;
         if (b < a.batch) {
-            const Seq q = sequence(a, b, err);
+            const Seq q = sequence(a, a.base_len[b], tree::node_count(a.n_nodes, b, a.max_nodes, err), err);
+            p.base[b] = q.base;
+            p.nodes[b] = q.nodes;
             g = a.n_kv * q.row_tiles;
             u = g * q.tiles;
         }
@@ -113,7 +117,7 @@ __device__ __forceinline__ int share_of(int units, const AttnTreeArgs& a) {
 __device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArgs& a, int pos, int end, int& b) {
     while (p.unit[b + 1] <= pos) ++b;
     Segment s;
-    const Seq q = sequence(a, b, nullptr);
+    const Seq q = sequence(a, p.base[b], p.nodes[b], nullptr);
     const int in = pos - p.unit[b], hr = in / q.tiles;
     s.b = b;
     s.h = hr / q.row_tiles;
@@ -132,7 +136,7 @@ struct Smem {
     alignas(1024) unsigned char v[kVStages][kSliceBytes];
     Prefix prefix;
     uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
-    uint64_t bar_s[2], bar_sfree[2], bar_p[2], bar_pv[2], bar_m[2], bar_q;
+    uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_m[2], bar_q;
     float xch[2][2][kRows][2];                    // [group][use parity] row maxima of the two column halves
     float mrow[2][kRows];                         // [page parity] running row maximum, in units of S
     alignas(16) float part[kRows][4];             // per row: the four threads' query maxima, later their sums
@@ -145,27 +149,40 @@ __device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
     __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&b);
 }
+// 32 bytes per thread: a whole sector of a row that is the thread's own
+__device__ __forceinline__ void ld_sector(const void* p, uint32_t (&r)[8]) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 // 64 query values of type q_type from src, as floats
 __device__ __forceinline__ void load_q(float (&x)[64], const void* q, int q_type, size_t at) {
     if (q_type == 0) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float4 f = __ldg(p + i);
-            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
-        }
-    } else {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at);
+        const float* p = static_cast<const float*>(q) + at;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint4 w = __ldg(p + i);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            uint32_t w[8];
+            ld_sector(p + 8 * i, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = q_type == 1 ? __half22float2(*reinterpret_cast<const __half2*>(&u[e]))
-                                             : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]));
-                x[8 * i + 2 * e] = f.x;
-                x[8 * i + 2 * e + 1] = f.y;
+            for (int e = 0; e < 8; ++e) x[8 * i + e] = __uint_as_float(w[e]);
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(q) + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w[8];
+            ld_sector(p + 16 * i, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 f = q_type == 1 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
+                                             : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
+                x[16 * i + 2 * e] = f.x;
+                x[16 * i + 2 * e + 1] = f.y;
             }
         }
     }
@@ -179,12 +196,14 @@ __device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const 
             o[i] *= sigmoid(g.x); o[i + 1] *= sigmoid(g.y); o[i + 2] *= sigmoid(g.z); o[i + 3] *= sigmoid(g.w);
         }
     }
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at);
+    uint16_t* dst = static_cast<uint16_t*>(a.o) + at;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float* x = o + 8 * i;
-        dst[i] = a.o_type == 1 ? make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]))
-                               : make_uint4(pack_b2(x[0], x[1]), pack_b2(x[2], x[3]), pack_b2(x[4], x[5]), pack_b2(x[6], x[7]));
+    for (int i = 0; i < 2; ++i) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            w[e] = a.o_type == 1 ? pack_h2(o[16 * i + 2 * e], o[16 * i + 2 * e + 1]) : pack_b2(o[16 * i + 2 * e], o[16 * i + 2 * e + 1]);
+        st_sector(dst + 16 * i, w);
     }
 }
 
@@ -209,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.bar_s[i], 1);
-            mbar_init(&s.bar_sfree[i], kGroupThreads);
             mbar_init(&s.bar_p[i], kGroupThreads);
             mbar_init(&s.bar_pv[i], 1);
             mbar_init(&s.bar_m[i], kGroupThreads);
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             uint64_t k_desc[kKStages];
 #pragma unroll
             for (int i = 0; i < kKStages; ++i) k_desc[i] = tc::smem_desc(smem_u32(s.k[i]), 16, 1024);
-            const uint32_t q_tmem = tmem + kColQ, s_tmem = tmem + kColS;
+            const uint32_t q_tmem = tmem + kColQ;
             int b = 0, it = 0, sg = 0;
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok; ++sg) {
@@ -273,9 +291,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
                     const int st = it % kKStages;
                     if (!mbar_wait(&s.k_full[st], (it / kKStages) & 1)) { ok = false; break; }
-                    // S is free once every thread of the group of the page before has read it out
-                    if (it >= 1 && !mbar_wait(&s.bar_sfree[(it - 1) & 1], ((it - 1) >> 1) & 1)) { ok = false; break; }
+                    // this S buffer held the P of two pages before
+                    if (it >= 2 && !mbar_wait(&s.bar_pv[it & 1], ((it - 2) >> 1) & 1)) { ok = false; break; }
                     tc::fence_after_sync();
+                    const uint32_t s_tmem = tmem + kColS + (it & 1) * 64;
                     const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[2]);
 #pragma unroll
                     for (int kk = 0; kk < 16; ++kk)
@@ -309,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     if (!mbar_wait(&s.bar_p[it & 1], (it >> 1) & 1)) { ok = false; break; }
                     tc::fence_after_sync();
                     const uint64_t vd = st == 0 ? v_desc[0] : (st == 1 ? v_desc[1] : v_desc[2]);
-                    const uint32_t p_tmem = tmem + kColP + (it & 1) * 32;
+                    const uint32_t p_tmem = tmem + kColS + (it & 1) * 64;
                     tc::mma_ts(tmem + kColO, p_tmem, vd, idesc_pv, j > 0);
 #pragma unroll
                     for (int kk = 1; kk < 4; ++kk)
@@ -386,11 +405,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 tc::fence_after_sync();
                 uint32_t raw[32];
                 if (ok) {
-                    tc::tmem_ld32(lane_addr + kColS + half * 32, raw);
+                    tc::tmem_ld32(lane_addr + kColS + grp * 64 + half * 32, raw);
                     tc::tmem_wait_ld();
                 }
-                tc::fence_before_sync();
-                mbar_arrive(&s.bar_sfree[grp]);
                 const int tok0 = (g.j0 + j) * kTile;
                 if (last_pos + 1 - tok0 < kTile) {
                     // V rows past the last node may hold anything (0 * NaN would poison O): clear them
@@ -473,10 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     ph[i] = pack_h2(p0, p1);
                 }
                 l_part += lsum0 + lsum1;
-                if (it >= 2) wait(&s.bar_pv[grp], ((it - 2) >> 1) & 1);    // this P buffer's last reader
-                tc::fence_after_sync();
-                if (ok) {
-                    tc::tmem_st16(lane_addr + kColP + grp * 32 + half * 16, ph);
+                if (ok) {                                     // both halves' scores left the buffer before the maxima met
+                    tc::tmem_st16(lane_addr + kColS + grp * 64 + half * 16, ph);
                     tc::tmem_wait_st();
                 }
                 tc::fence_before_sync();
@@ -513,9 +528,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                                                    : nullptr;
                         store_o(a, flat * kHeadDim + col0 + c0, gate, o);
                     } else {
-                        float4* dst = reinterpret_cast<float4*>(a.part_o + slot * kHeadDim + col0 + c0);
+                        float* dst = a.part_o + slot * kHeadDim + col0 + c0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e] = raw[8 * i + e];
+                            st_sector(dst + 8 * i, w);
+                        }
                     }
                 }
                 if (!whole && live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
@@ -537,7 +557,7 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
     if (warp == 0) build_prefix(prefix, a, lane, nullptr);
     __syncthreads();
     griddep_wait();
-    const Seq q = sequence(a, b, nullptr);
+    const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
     const int row = blockIdx.x * 8 + warp, node = row / a.n_q, hq = row - node * a.n_q;
     if (node >= q.nodes) return;
     const int h = hq / G, tr = node * G + hq - h * G, hr = h * q.row_tiles + tr / kRows;
@@ -551,15 +571,25 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
     float l = 0.f, x[8] = {};
-    for (int p = 0; p <= last - first; ++p) {
-        const size_t row_at = r0 + size_t(p) * kRows;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_at * 2);
-        const float4 o0 = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8));
-        const float4 o1 = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8 + 4));
-        const float w = fast_exp2(ml.x - mm);
-        l = fmaf(ml.y, w, l);
-        x[0] = fmaf(o0.x, w, x[0]); x[1] = fmaf(o0.y, w, x[1]); x[2] = fmaf(o0.z, w, x[2]); x[3] = fmaf(o0.w, w, x[3]);
-        x[4] = fmaf(o1.x, w, x[4]); x[5] = fmaf(o1.y, w, x[5]); x[6] = fmaf(o1.z, w, x[6]); x[7] = fmaf(o1.w, w, x[7]);
+    constexpr int kAhead = 4;                                 // slots whose loads are in flight together
+    for (int p0 = 0; p0 <= last - first; p0 += kAhead) {
+        float2 ml[kAhead];
+        float4 o0[kAhead], o1[kAhead];
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+            const size_t row_at = r0 + size_t(min(p0 + z, last - first)) * kRows;
+            ml[z] = *reinterpret_cast<const float2*>(a.part_ml + row_at * 2);
+            o0[z] = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8));
+            o1[z] = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8 + 4));
+        }
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+            if (p0 + z > last - first) break;
+            const float w = fast_exp2(ml[z].x - mm);
+            l = fmaf(ml[z].y, w, l);
+            x[0] = fmaf(o0[z].x, w, x[0]); x[1] = fmaf(o0[z].y, w, x[1]); x[2] = fmaf(o0[z].z, w, x[2]); x[3] = fmaf(o0[z].w, w, x[3]);
+            x[4] = fmaf(o1[z].x, w, x[4]); x[5] = fmaf(o1[z].y, w, x[5]); x[6] = fmaf(o1[z].z, w, x[6]); x[7] = fmaf(o1[z].w, w, x[7]);
+        }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
