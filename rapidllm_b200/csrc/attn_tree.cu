@@ -151,7 +151,7 @@ __device__ __forceinline__ uint32_t pack_b2(float lo, float hi) {
 }
 // 32 bytes per thread: a whole sector of a row that is the thread's own
 __device__ __forceinline__ void ld_sector(const void* p, uint32_t (&r)[8]) {
-    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "l"(p));
 }
@@ -246,33 +246,53 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
 
     if (warp == kWarpLoader) {
         // ------------------------------ page loader ------------------------------
-        if (lane == 0) {
-            int b = 0, it = 0;
-            bool ok = true;
-            for (int pos = u_begin; pos < u_end && ok;) {
-                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
-                pos += g.n_tiles;
-                const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq + g.j0;
-                for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
-                    const int ks = it % kKStages, vs = it % kVStages;
-                    int page = table[j];
-                    if (page < 0 || page >= a.n_pages) {
+        // The warp starts a segment's query rows (but the first's) and its sequence's parents on their way into L2
+        // when it starts on its pages, several pages ahead of the softmax warps; then lane 0 waits and copies.
+        int b = 0, it = 0;
+        bool ok = true;
+        for (int pos = u_begin; pos < u_end && ok;) {
+            const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+            if (pos > u_begin) {
+                const int row_bytes = kHeadDim * (a.q_type == 0 ? 4 : 2), lines = row_bytes / 128;
+                const int rows = min(kRows, g.nodes * G - g.rt * kRows);
+                for (int i = lane; i < rows * lines; i += 32) {
+                    const int row = g.rt * kRows + i / lines, node = row / G;
+                    const size_t flat = (size_t(g.b) * a.max_nodes + node) * a.n_q + g.h * G + row - node * G;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(a.q) + flat * row_bytes + (i % lines) * 128));
+                }
+                if (a.parents && lane < 2) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.parents + size_t(g.b) * a.max_nodes + min(lane * 32, a.max_nodes - 1)));
+            }
+            pos += g.n_tiles;
+            const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq + g.j0;
+            for (int j0 = 0; j0 < g.n_tiles && ok; j0 += 32) {
+                // 32 page ids at a time: the table's latency is paid once per 32 pages
+                int mine = 0;
+                if (j0 + lane < g.n_tiles) {
+                    mine = table[j0 + lane];
+                    if (mine < 0 || mine >= a.n_pages) {
                         set_err(a.err, DEV_ERR_BAD_PAGE);
-                        page = 0;
+                        mine = 0;
                     }
+                }
+                const int count = min(32, g.n_tiles - j0);
+                for (int j = 0; j < count; ++j, ++it) {
+                    const int page = __shfl_sync(0xffffffffu, mine, j);
+                    if (lane != 0 || !ok) continue;
+                    const int ks = it % kKStages, vs = it % kVStages;
                     const size_t slice = (size_t(page) * a.n_kv + g.h) * kv_slice_elems();
-                    if (!mbar_wait(&s.k_empty[ks], ((it / kKStages) & 1) ^ 1)) { ok = false; break; }
+                    if (!mbar_wait(&s.k_empty[ks], ((it / kKStages) & 1) ^ 1)) { ok = false; continue; }
                     mbar_arrive_expect_tx(&s.k_full[ks], kSliceBytes);
                     bulk_g2s(s.k[ks], a.k_pool + slice, kSliceBytes, &s.k_full[ks]);
-                    if (!mbar_wait(&s.v_empty[vs], ((it / kVStages) & 1) ^ 1)) { ok = false; break; }
+                    if (!mbar_wait(&s.v_empty[vs], ((it / kVStages) & 1) ^ 1)) { ok = false; continue; }
                     mbar_arrive_expect_tx(&s.v_full[vs], kSliceBytes);
                     bulk_g2s(s.v[vs], a.v_pool + slice, kSliceBytes, &s.v_full[vs]);
                 }
+                ok = __shfl_sync(0xffffffffu, int(ok), 0);
             }
-            if (!ok) {
-                set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
-                s.failed = 1;
-            }
+        }
+        if (!ok && lane == 0) {
+            set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
+            s.failed = 1;
         }
     } else if (warp == kWarpQK) {
         // ------------------------------ S = Q K^T issuer ------------------------------
@@ -509,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             wait(&s.bar_pv[it_last & 1], (it_last >> 1) & 1);              // every P.V of the segment is done
             tc::fence_after_sync();
             const bool whole = g.n_tiles == g.n_all;
-            const size_t slot = (size_t(blockIdx.x) + g.index) * kRows + r;
+            const size_t slot = size_t(blockIdx.x) + g.index;
             const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
             const int col0 = quarter * 64;
             if (ok && __all_sync(0xffffffffu, !*const_cast<volatile int*>(&s.failed))) {
@@ -528,17 +548,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                                                    : nullptr;
                         store_o(a, flat * kHeadDim + col0 + c0, gate, o);
                     } else {
-                        float* dst = a.part_o + slot * kHeadDim + col0 + c0;
+                        // [slot][dims / 8][row][8]: a warp's 32 rows of 32 bytes are contiguous
+                        float* dst = a.part_o + (slot * (kHeadDim / 8) + (col0 + c0) / 8) * (kRows * 8) + r * 8;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint32_t w[8];
 #pragma unroll
                             for (int e = 0; e < 8; ++e) w[e] = raw[8 * i + e];
-                            st_sector(dst + 8 * i, w);
+                            st_sector(dst + i * (kRows * 8), w);
                         }
                     }
                 }
-                if (!whole && live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
+                if (!whole && live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
             }
             tc::fence_before_sync();
             named_bar_sync(9, kSoftmaxThreads);               // O, Q and `part` may be rewritten
@@ -548,62 +569,74 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
     if (warp == kWarpQK) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
-// Rows whose pages were divided: one warp per (node, query head), 2 x 4 dims per lane; log-sum-exp over the
-// row's slots (log2 domain), gate, rounding.  grid (ceil(max_nodes * n_q / 8), batch).
+// Rows whose pages were divided: log-sum-exp over the row's slots (log2 domain), gate, rounding.  A block takes 16
+// rows of a row tile, a thread 16 dims of one row (lane = row: 32 bytes of 16 rows are contiguous in a slot); four
+// slots are in flight.  grid (n_kv * row tiles * 8, batch).
+constexpr int kMergeRows = 16, kAhead = 4;
 __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
     __shared__ Prefix prefix;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
+    const int tid = threadIdx.x, b = blockIdx.y;
     const int G = a.n_q / a.n_kv;
-    if (warp == 0) build_prefix(prefix, a, lane, nullptr);
+    if (tid < 32) build_prefix(prefix, a, tid, nullptr);
     __syncthreads();
-    griddep_wait();
     const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
-    const int row = blockIdx.x * 8 + warp, node = row / a.n_q, hq = row - node * a.n_q;
-    if (node >= q.nodes) return;
-    const int h = hq / G, tr = node * G + hq - h * G, hr = h * q.row_tiles + tr / kRows;
+    const int hr = blockIdx.x / (kRows / kMergeRows), r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + (tid & (kMergeRows - 1));
+    const int d0 = (tid / kMergeRows) * 16;
+    if (hr >= a.n_kv * q.row_tiles) return;
+    const int h = hr / q.row_tiles, tr = (hr - h * q.row_tiles) * kRows + r, node = tr / G, hq = h * G + tr - node * G;
     const int share = share_of(prefix.unit[a.batch], a);
     const int u0 = prefix.unit[b] + hr * q.tiles;
-    const int first = u0 / share, last = (u0 + q.tiles - 1) / share;
-    if (first == last) return;                                // written by the CTA that held all of it
-    const size_t r0 = (size_t(first) + prefix.seg[b] + hr) * kRows + tr % kRows;
-    float mm = kNoMax;
-    for (int p = lane; p <= last - first; p += 32) mm = fmaxf(mm, a.part_ml[(r0 + size_t(p) * kRows) * 2]);
+    const int first = u0 / share, parts = (u0 + q.tiles - 1) / share - first + 1;
+    if (node >= q.nodes || parts == 1) return;                // whole: written by the CTA that held all of it
+    uint32_t gate[2][8];
+    if (a.gate) {
+        const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
-    float l = 0.f, x[8] = {};
-    constexpr int kAhead = 4;                                 // slots whose loads are in flight together
-    for (int p0 = 0; p0 <= last - first; p0 += kAhead) {
-        float2 ml[kAhead];
-        float4 o0[kAhead], o1[kAhead];
-#pragma unroll
-        for (int z = 0; z < kAhead; ++z) {
-            const size_t row_at = r0 + size_t(min(p0 + z, last - first)) * kRows;
-            ml[z] = *reinterpret_cast<const float2*>(a.part_ml + row_at * 2);
-            o0[z] = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8));
-            o1[z] = __ldcs(reinterpret_cast<const float4*>(a.part_o + row_at * kHeadDim + lane * 8 + 4));
+        for (int i = 0; i < 4; ++i) {
+            const float4 g = __ldcs(reinterpret_cast<const float4*>(gp + 4 * i));
+            gate[i / 2][4 * (i & 1)] = __float_as_uint(g.x);
+            gate[i / 2][4 * (i & 1) + 1] = __float_as_uint(g.y);
+            gate[i / 2][4 * (i & 1) + 2] = __float_as_uint(g.z);
+            gate[i / 2][4 * (i & 1) + 3] = __float_as_uint(g.w);
         }
+    }
+    griddep_wait();
+    const size_t slot0 = size_t(first) + prefix.seg[b] + hr;
+    float m = kNoMax, l = 0.f, x[16] = {};
+    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+        float2 ml[kAhead];
+        uint32_t o[kAhead][2][8];
 #pragma unroll
         for (int z = 0; z < kAhead; ++z) {
-            if (p0 + z > last - first) break;
-            const float w = fast_exp2(ml[z].x - mm);
+            const size_t slot = slot0 + min(p0 + z, parts - 1);
+            ml[z] = *reinterpret_cast<const float2*>(a.part_ml + (slot * kRows + r) * 2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ld_sector(a.part_o + (slot * (kHeadDim / 8) + d0 / 8 + i) * (kRows * 8) + r * 8, o[z][i]);
+        }
+        float mx = m;
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) mx = fmaxf(mx, ml[z].x);
+        const float back = fast_exp2(m - mx);
+        m = mx;
+        l *= back;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= back;
+#pragma unroll
+        for (int z = 0; z < kAhead; ++z) {
+            if (p0 + z >= parts) break;
+            const float w = fast_exp2(ml[z].x - m);
             l = fmaf(ml[z].y, w, l);
-            x[0] = fmaf(o0[z].x, w, x[0]); x[1] = fmaf(o0[z].y, w, x[1]); x[2] = fmaf(o0[z].z, w, x[2]); x[3] = fmaf(o0[z].w, w, x[3]);
-            x[4] = fmaf(o1[z].x, w, x[4]); x[5] = fmaf(o1[z].y, w, x[5]); x[6] = fmaf(o1[z].z, w, x[6]); x[7] = fmaf(o1[z].w, w, x[7]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = fmaf(__uint_as_float(o[z][e / 8][e & 7]), w, x[e]);
         }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= inv;
-    if (a.gate) {
-        const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + lane * 8;
-        const float4 g0 = __ldcs(reinterpret_cast<const float4*>(gp)), g1 = __ldcs(reinterpret_cast<const float4*>(gp + 4));
-        x[0] *= sigmoid(g0.x); x[1] *= sigmoid(g0.y); x[2] *= sigmoid(g0.z); x[3] *= sigmoid(g0.w);
-        x[4] *= sigmoid(g1.x); x[5] *= sigmoid(g1.y); x[6] *= sigmoid(g1.z); x[7] *= sigmoid(g1.w);
-    }
-    const size_t at = ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + lane * 8;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at) =
-        a.o_type == 1 ? make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]))
-                      : make_uint4(pack_b2(x[0], x[1]), pack_b2(x[2], x[3]), pack_b2(x[4], x[5]), pack_b2(x[6], x[7]));
+    for (int e = 0; e < 16; ++e) x[e] *= a.gate ? inv * sigmoid(__uint_as_float(gate[e / 8][e & 7])) : inv;
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = a.o_type == 1 ? pack_h2(x[2 * e], x[2 * e + 1]) : pack_b2(x[2 * e], x[2 * e + 1]);
+    st_sector(static_cast<uint16_t*>(a.o) + ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + d0, w);
 }
 
 size_t attn_tree_smem_bytes() { return sizeof(Smem) + 1024; }
@@ -613,7 +646,8 @@ int attn_tree_max_batch() { return kMaxBatch; }
 cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
     attn_tree_kernel<<<a.grid, kThreads, attn_tree_smem_bytes(), st>>>(a);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((a.max_nodes * a.n_q + 7) / 8), unsigned(a.batch));
+    const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
+    cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * (kRows / kMergeRows)), unsigned(a.batch));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
