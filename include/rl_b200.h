@@ -515,10 +515,13 @@ int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_ph
 
 /* Keep one path: S and the conv window of each sequence's slot advance by the path's tokens, as that many
  * decode steps would (the sums are in another order).  The window's entries move and conv_phase stays, so no
- * rl_gdn_phase_advance follows.  The slots of a call must be distinct.  Takes rl_gdn_tree's inputs. */
+ * rl_gdn_phase_advance follows.  The slots of a call must be distinct.  Takes rl_gdn_tree's inputs and a
+ * workspace of rl_gdn_tree_commit_workspace_bytes() bytes, 16-byte aligned, for the path's k and v rows. */
+size_t rl_gdn_tree_commit_workspace_bytes(const rl_gdn_tree_params* p);
 int rl_gdn_tree_commit(float* S, float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
                        const int32_t* parents, const int32_t* leaf, const float* qkv, const float* conv_w,
-                       const float* beta, const float* g_log, const rl_gdn_tree_params* p, void* stream);
+                       const float* beta, const float* g_log, void* workspace, size_t workspace_bytes,
+                       const rl_gdn_tree_params* p, void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* Caches and the layer_types[] dispatch                                      */

@@ -1513,14 +1513,18 @@ static int attn_tree_check(const rl_attn_tree_params* p) {
     if (p->o_type != RL_TYPE_F16 && p->o_type != RL_TYPE_BF16)
         return fail(RL_ERR_UNSUPPORTED, "o_type %d: only RL_TYPE_F16 and RL_TYPE_BF16", p->o_type);
     const long long row_tiles = (1LL * p->max_nodes * (p->n_q / p->n_kv) + rl::attn_tree_rows() - 1) / rl::attn_tree_rows();
-    if (1LL * p->batch * p->n_kv * row_tiles * p->max_pages_per_seq > 0x3fffffff)
+    if (1LL * p->batch * p->n_kv * row_tiles * (p->max_pages_per_seq + 64LL) > 0x3fffffff)
         return fail(RL_ERR_RANGE, "batch %d, n_kv %d, max_pages_per_seq %d: too many pages in one call", p->batch, p->n_kv, p->max_pages_per_seq);
     return RL_OK;
 }
 
-// One persistent CTA per SM, fewer when the batch has less than kTreeMinShare pages for each.  Two pages are
-// the least that lets both softmax groups work.
-static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 2);
+// One persistent CTA per SM, fewer when the batch has less than kTreeMinShare pages for each: 8 nodes over 2 000
+// tokens take 20.7 us with 2 pages, 19.3 with 4, 21.4 with 6 (more CTAs leave more partials to merge).
+static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 4);
+// What a CTA pays to close one (sequence, head, row tile) and open the next (partial out, queries in, behind the pages
+// already requested), in pages.  16 trees of 21 over 16K: 161.5 us with 0, 157.0 with 6, 154.1 with 12, 149.6 with 18,
+// 150.4 with 26; 4 trees of 64 over 32K: 215.9, 210.3, 198.9, 201.1, 201.4.
+static const int kTreeBoundary = knob("RL_B200_TREE_BOUNDARY", 16);
 struct AttnTreePlan {
     int grid;
     size_t o_bytes, total_bytes;
@@ -1529,7 +1533,7 @@ static AttnTreePlan attn_tree_plan(const rl_attn_tree_params* p, int sms) {
     AttnTreePlan pl;
     const int rows = rl::attn_tree_rows();
     const long long segs = 1LL * p->batch * p->n_kv * ((p->max_nodes * (p->n_q / p->n_kv) + rows - 1) / rows);
-    const long long units = segs * ceil_div(p->max_seq_len, p->page_tokens);
+    const long long units = segs * (ceil_div(p->max_seq_len, p->page_tokens) + kTreeBoundary);
     pl.grid = int(std::max(1LL, std::min(1LL * sms, (units + kTreeMinShare - 1) / kTreeMinShare)));
     const size_t slots = size_t(pl.grid) + size_t(segs);
     pl.o_bytes = align_up(slots * rows * rl::kHeadDim * sizeof(float), 256);
@@ -1587,6 +1591,7 @@ int rl_attn_tree(const void* k_pool, const void* v_pool, const int32_t* page_tab
     a.o_type = p->o_type;
     a.grid = pl.grid;
     a.min_share = kTreeMinShare;
+    a.boundary = kTreeBoundary;
     a.scale = 1.f / sqrtf(float(p->head_dim));
     RL_CUDA(rl::launch_attn_tree(a, as_stream(stream)));
     RL_CUDA(cudaGetLastError());
@@ -1621,9 +1626,7 @@ int rl_kv_tree_commit(void* k_pool, void* v_pool, const int32_t* page_table, con
     return RL_OK;
 }
 
-static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_window, const int32_t* conv_phase,
-                         const int32_t* slot_ids, const int32_t* parents, const float* qkv, const float* conv_w,
-                         const float* beta, const float* g_log, const rl_gdn_tree_params* p) {
+static int gdn_tree_check(const rl_gdn_tree_params* p, rl::GdnTreeArgs* a) {
     if (!p) return fail(RL_ERR_RANGE, "params is NULL");
     if (p->dk != 128 || p->dv != 128 || p->conv_k != 4)
         return fail(RL_ERR_UNSUPPORTED, "dk %d dv %d conv_k %d: only 128 x 128, 4 taps", p->dk, p->dv, p->conv_k);
@@ -1639,6 +1642,12 @@ static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_w
     if (!row_stride(p->qkv_stride, a->conv_dim, &a->x_stride))
         return fail(RL_ERR_RANGE, "qkv_stride %lld: at least a row, a multiple of 4", p->qkv_stride);
     if (a->x_stride > 0x7fffffff / RL_TREE_MAX_NODES) return fail(RL_ERR_RANGE, "qkv_stride %lld: rows too far apart", p->qkv_stride);
+    return RL_OK;
+}
+static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_window, const int32_t* conv_phase,
+                         const int32_t* slot_ids, const int32_t* parents, const float* qkv, const float* conv_w,
+                         const float* beta, const float* g_log, const rl_gdn_tree_params* p) {
+    if (int st = gdn_tree_check(p, a)) return st;
     if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
     if (!S || !conv_window || !qkv || !conv_w || !beta || !g_log) return fail(RL_ERR_RANGE, "NULL pointer argument");
     if (!aligned16(S) || !aligned16(conv_window) || !aligned16(qkv) || !aligned16(conv_w))
@@ -1682,16 +1691,26 @@ int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_ph
     return RL_OK;
 }
 
+size_t rl_gdn_tree_commit_workspace_bytes(const rl_gdn_tree_params* p) {
+    rl::GdnTreeArgs a = {};
+    if (gdn_tree_check(p, &a)) return 0;
+    return std::max<size_t>(256, rl::gdn_tree_commit_workspace_bytes(p->batch, p->max_nodes, p->n_v, p->n_qk));
+}
+
 int rl_gdn_tree_commit(float* S, float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
                        const int32_t* parents, const int32_t* leaf, const float* qkv, const float* conv_w, const float* beta,
-                       const float* g_log, const rl_gdn_tree_params* p, void* stream) {
+                       const float* g_log, void* workspace, size_t workspace_bytes, const rl_gdn_tree_params* p, void* stream) {
     rl::GdnTreeArgs a = {};
     if (int st = gdn_tree_args(&a, S, conv_window, conv_phase, slot_ids, parents, qkv, conv_w, beta, g_log, p)) return st;
     if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
-    if (!leaf) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!leaf || !workspace) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(workspace)) return fail(RL_ERR_RANGE, "workspace must be 16-byte aligned");
+    const size_t need = rl::gdn_tree_commit_workspace_bytes(p->batch, p->max_nodes, p->n_v, p->n_qk);
+    if (workspace_bytes < need) return fail(RL_ERR_RANGE, "workspace %zu bytes < %zu required", workspace_bytes, need);
     a.leaf = leaf;
     a.S_out = S;
     a.conv_out = conv_window;
+    a.workspace = workspace;
     RL_CUDA(rl::launch_gdn_tree_commit(a, as_stream(stream)));
     RL_CUDA(cudaGetLastError());
     return RL_OK;

@@ -10,10 +10,11 @@
 //
 // Work division: the (sequence, KV head, row tile, page) units of the whole batch form one list, computed on
 // the device from base_len and n_nodes (a captured step may advance them), and every CTA of a persistent
-// grid takes an equal contiguous share, cut into segments at (sequence, head, row tile) boundaries.  The
-// page ring runs on across segments.  A segment that holds all pages of its rows writes the output, the
-// others write (unnormalised o, max, sum) to slot `CTA + segment index`, distinct because a CTA's last
-// segment is the next one's first at most; attn_tree_merge_kernel joins them.
+// grid takes a contiguous share of equal cost, cut into segments at (sequence, head, row tile) boundaries; a
+// boundary is charged as kBoundary pages.  The page ring runs on across segments.  A segment that holds all
+// pages of its rows writes the output, the others write (unnormalised o, max, sum) to slot `CTA + segment
+// index`, distinct because a CTA's last segment is the next one's first at most; attn_tree_merge_kernel joins
+// them.
 //
 // Inside a segment: S = Q K^T (M 128, N 64) and O += P V (M 128, N 256) with Q, P, S and O in tensor memory
 // and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
@@ -50,11 +51,12 @@ constexpr int kMaxBatch = 512;
 
 struct Segment {
     int b, h, rt, index;                          // index: running number of (b, h, rt)
-    int j0, n_tiles, n_all;                       // pages [j0, j0 + n_tiles) of n_all
+    int j0, n_tiles, n_all;                       // pages [j0, j0 + n_tiles) of n_all; n_tiles 0: only the charge
     int base, nodes;
+    int next;                                     // position of the next segment
 };
 
-// units and segments of the sequences before b; entry `batch` holds the totals
+// cost and segments of the sequences before b; entry `batch` holds the totals
 struct Prefix {
     int unit[kMaxBatch + 1], seg[kMaxBatch + 1];
     int base[kMaxBatch], nodes[kMaxBatch];
@@ -86,7 +88,7 @@ __device__ __forceinline__ void build_prefix(Prefix& p, const AttnTreeArgs& a, i
             p.base[b] = q.base;
             p.nodes[b] = q.nodes;
             g = a.n_kv * q.row_tiles;
-            u = g * q.tiles;
+            u = g * (q.tiles + a.boundary);
         }
         int su = u, sg = g;
 #pragma unroll
@@ -109,23 +111,25 @@ __device__ __forceinline__ void build_prefix(Prefix& p, const AttnTreeArgs& a, i
         p.seg[a.batch] = segs;
     }
 }
-// pages per CTA
+// cost per CTA
 __device__ __forceinline__ int share_of(int units, const AttnTreeArgs& a) {
     return max((units + a.grid - 1) / a.grid, a.min_share);
 }
-// the segment that starts at unit `pos` of a share that ends at `end`; b: a sequence at or before it
+// the segment at position `pos` of a share that ends at `end`; b: a sequence at or before it.  A (sequence, head, row
+// tile) spans `boundary` positions of charge, then its pages.
 __device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArgs& a, int pos, int end, int& b) {
     while (p.unit[b + 1] <= pos) ++b;
     Segment s;
     const Seq q = sequence(a, p.base[b], p.nodes[b], nullptr);
-    const int in = pos - p.unit[b], hr = in / q.tiles;
+    const int span = q.tiles + a.boundary, in = pos - p.unit[b], hr = in / span, at = in - hr * span - a.boundary;
     s.b = b;
     s.h = hr / q.row_tiles;
     s.rt = hr - s.h * q.row_tiles;
     s.index = p.seg[b] + hr;
-    s.j0 = in - hr * q.tiles;
+    s.j0 = max(at, 0);
     s.n_all = q.tiles;
-    s.n_tiles = min(q.tiles - s.j0, end - pos);
+    s.next = min(end, pos + q.tiles - at);
+    s.n_tiles = max(at + s.next - pos - s.j0, 0);
     s.base = q.base;
     s.nodes = q.nodes;
     return s;
@@ -252,7 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         bool ok = true;
         for (int pos = u_begin; pos < u_end && ok;) {
             const Segment g = segment_at(s.prefix, a, pos, u_end, b);
-            if (pos > u_begin) {
+            const bool first = pos == u_begin;
+            pos = g.next;
+            if (!g.n_tiles) continue;
+            if (!first) {
                 const int row_bytes = kHeadDim * (a.q_type == 0 ? 4 : 2), lines = row_bytes / 128;
                 const int rows = min(kRows, g.nodes * G - g.rt * kRows);
                 for (int i = lane; i < rows * lines; i += 32) {
@@ -262,7 +269,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 }
                 if (a.parents && lane < 2) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.parents + size_t(g.b) * a.max_nodes + min(lane * 32, a.max_nodes - 1)));
             }
-            pos += g.n_tiles;
             const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq + g.j0;
             for (int j0 = 0; j0 < g.n_tiles && ok; j0 += 32) {
                 // 32 page ids at a time: the table's latency is paid once per 32 pages
@@ -304,10 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             const uint32_t q_tmem = tmem + kColQ;
             int b = 0, it = 0, sg = 0;
             bool ok = true;
-            for (int pos = u_begin; pos < u_end && ok; ++sg) {
+            for (int pos = u_begin; pos < u_end && ok;) {
                 const Segment g = segment_at(s.prefix, a, pos, u_end, b);
-                pos += g.n_tiles;
+                pos = g.next;
+                if (!g.n_tiles) continue;
                 ok = mbar_wait(&s.bar_q, sg & 1);
+                ++sg;
                 for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
                     const int st = it % kKStages;
                     if (!mbar_wait(&s.k_full[st], (it / kKStages) & 1)) { ok = false; break; }
@@ -340,7 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok;) {
                 const Segment g = segment_at(s.prefix, a, pos, u_end, b);
-                pos += g.n_tiles;
+                pos = g.next;
+                if (!g.n_tiles) continue;
                 for (int j = 0; j < g.n_tiles; ++j, ++it) {
                     const int st = it % kVStages;
                     if (!mbar_wait(&s.v_full[st], (it / kVStages) & 1)) { ok = false; break; }
@@ -377,7 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         int b = 0, it0 = 0;                                   // it0: pages of the segments before
         for (int pos = u_begin; pos < u_end;) {
             const Segment g = segment_at(s.prefix, a, pos, u_end, b);
-            pos += g.n_tiles;
+            pos = g.next;
+            if (!g.n_tiles) continue;
             const int row = g.rt * kRows + r, node = row / G, hq = g.h * G + row - node * G;
             const bool live = node < g.nodes;
             const size_t flat = (size_t(g.b) * a.max_nodes + (live ? node : 0)) * a.n_q + hq;
@@ -585,7 +595,7 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
     if (hr >= a.n_kv * q.row_tiles) return;
     const int h = hr / q.row_tiles, tr = (hr - h * q.row_tiles) * kRows + r, node = tr / G, hq = h * G + tr - node * G;
     const int share = share_of(prefix.unit[a.batch], a);
-    const int u0 = prefix.unit[b] + hr * q.tiles;
+    const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
     const int first = u0 / share, parts = (u0 + q.tiles - 1) / share - first + 1;
     if (node >= q.nodes || parts == 1) return;                // whole: written by the CTA that held all of it
     uint32_t gate[2][8];

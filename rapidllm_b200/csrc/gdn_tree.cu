@@ -616,101 +616,196 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Commit: the path to the leaf, up to 8 tokens at a time in the closed form above with the state in
-// registers.  grid (4 slices of 32 columns, n_v, batch).
+// Commit, in two kernels.  The first (gdn_tree_path_kernel) walks the path to the leaf and leaves its tokens' k
+// (unit length), v, log decays and betas in the workspace, in path order; the second moves the state, 128 KiB in and
+// out per head, which is the bound, and rewrites the conv windows, which nothing reads any more.  Together in one
+// kernel every CTA waits for leaf, parents, rows and taps one after the other before it can touch the state (32
+// paths in trees of 32: 93 us).
 namespace {
 
-constexpr int kSliceCols = 32, kSlices = kDv / kSliceCols, kCommitThreads = 256, kChunk = 8;
+constexpr int kPathWarps = 4, kCommitThreads = 512, kChunk = 16;
 
 struct CommitSmem {
-    float k[kChunk][kDk], v[kChunk][kSliceCols];
-    float kk[kChunk][kChunk];
-    float g[kChunk], beta[kChunk];
-    float red[kCommitThreads / 32][kChunk][kSliceCols];
-    float u[kChunk][kSliceCols];
-    int parents[kMaxNodes];
-    int path[kMaxNodes];
-    int len;
+    float k[kChunk][kDk], v[kChunk][kDv];                     // v, then u
+    float low[kChunk][kChunk];                                // coefficient of u_j in u_i
+    float red[4][kChunk][kDv];                                // S0^T k by row blocks
+    float2 cb[kMaxNodes];                                     // log decay from the state to the path's token; beta
 };
+// workspace: path lengths, then the path's nodes [batch][max_nodes], (c, beta) [batch][n_v][max_nodes], k
+// [batch][max_nodes][n_qk][128], v [batch][max_nodes][n_v][128]
+struct CommitWorkspace {
+    int* len;
+    int* path;
+    float2* cb;
+    float *k, *v;
+    size_t bytes;
+};
+__host__ __device__ __forceinline__ CommitWorkspace commit_workspace(void* base, int batch, int max_nodes, int n_v, int n_qk) {
+    CommitWorkspace w;
+    size_t at = 0;
+    char* p = static_cast<char*>(base);
+    auto take = [&](size_t bytes) {
+        char* q = p + at;
+        at += (bytes + 255) / 256 * 256;
+        return q;
+    };
+    const size_t rows = size_t(batch) * max_nodes;
+    w.len = reinterpret_cast<int*>(take(size_t(batch) * 4));
+    w.path = reinterpret_cast<int*>(take(rows * 4));
+    w.cb = reinterpret_cast<float2*>(take(rows * n_v * 8));
+    w.k = reinterpret_cast<float*>(take(rows * n_qk * kDk * 4));
+    w.v = reinterpret_cast<float*>(take(rows * n_v * kDv * 4));
+    w.bytes = at;
+    return w;
+}
 
 }  // namespace
 
-__global__ void __launch_bounds__(kCommitThreads) gdn_tree_commit_kernel(GdnTreeArgs a) {
-    __shared__ CommitSmem s;
+// grid (ceil((n_qk + n_v) / 4), batch): a warp per key head (its k) or value head (its v, decays, betas).
+__global__ void __launch_bounds__(kPathWarps * 32) gdn_tree_path_kernel(GdnTreeArgs a) {
+    __shared__ int parents[kMaxNodes], path[kMaxNodes];
+    __shared__ int path_len;
     griddep_launch();
-    const int slice = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int slot = a.slot_ids ? a.slot_ids[b] : b;
-    if (slot < 0 || slot >= a.n_slots) {
-        if (tid == 0) set_err(a.err, DEV_ERR_BAD_SLOT);
+    const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int slot = a.slot_ids ? a.slot_ids[b] : b, leaf = a.leaf[b];
+    const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
+    const bool bad_slot = slot < 0 || slot >= a.n_slots, none = leaf < 0 || leaf >= a.max_nodes;
+    if (bad_slot || none) {
+        if (tid == 0) {
+            if (bad_slot) set_err(a.err, DEV_ERR_BAD_SLOT);
+            if (none && leaf != -1) set_err(a.err, DEV_ERR_BAD_TREE);
+            if (blockIdx.x == 0) ws.len[b] = 0;
+        }
         return;
     }
-    const int leaf = a.leaf[b];
-    if (leaf < 0 || leaf >= a.max_nodes) {
-        if (leaf != -1 && tid == 0) set_err(a.err, DEV_ERR_BAD_TREE);
-        return;
-    }
-    float* Sp = a.S_out + (size_t(slot) * a.n_v + h) * (kDk * kDv);
-    const int rg = tid >> 3, cg = tid & 7;               // rows 4rg.., slice columns 4cg..
-    const int col0 = slice * kSliceCols + cg * 4;
-    float4 st[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) st[r] = *reinterpret_cast<const float4*>(Sp + (4 * rg + r) * kDv + col0);
+    const int role = blockIdx.x * kPathWarps + warp;          // key heads, then value heads
+    const bool is_k = role < a.n_qk, is_v = !is_k && role < a.n_qk + a.n_v;
+    const int h = is_k ? role : role - a.n_qk;
+    const int ch = (is_k ? (a.n_qk + h) * kDk : 2 * a.n_qk * kDk + (is_v ? h : 0) * kDv) + lane * 4;
+    Conv4 cv;
+    cv.load(a, slot, ch);
     if (warp == 0) {
         const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, leaf + 1, lane, a.err);
-        s.parents[lane] = w.parent_lo;
-        s.parents[lane + 32] = w.parent_hi;
-        const unsigned long long path = tree::of_node(w.lo, w.hi, leaf);
+        parents[lane] = w.parent_lo;
+        parents[lane + 32] = w.parent_hi;
+        const unsigned long long on = tree::of_node(w.lo, w.hi, leaf);
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            const int i = lane + 32 * z;
-            if (path >> i & 1) s.path[__popcll(path & ((1ull << i) - 1))] = i;
+            const int i = lane + 32 * z, at = __popcll(on & ((1ull << i) - 1));
+            if (on >> i & 1) {
+                path[at] = i;
+                if (blockIdx.x == 0) ws.path[size_t(b) * a.max_nodes + at] = i;
+            }
         }
-        if (lane == 0) s.len = __popcll(path);
+        if (lane == 0) {
+            path_len = __popcll(on);
+            if (blockIdx.x == 0) ws.len[b] = path_len;
+        }
     }
     __syncthreads();
-    const int hs = key_head_of(h, a.n_v, a.n_qk, a.head_map);
+    if (!is_k && !is_v) return;
+    const int len = path_len;
     const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride;
-    const int len = s.len;
+    for (int t0 = 0; t0 < len; t0 += 4) {
+        int4 src[4];
+        float4 y[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) src[m] = conv_sources(path[min(t0 + m, len - 1)], parents, int(a.x_stride));
+        conv_nodes(cv, x + ch, src, y);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const size_t at = size_t(b) * a.max_nodes + t0 + m;
+            if (is_k) y[m] = unit(y[m], a.eps_l2, 1.f);
+            if (t0 + m < len) *reinterpret_cast<float4*>(is_k ? ws.k + (at * a.n_qk + h) * kDk + lane * 4 : ws.v + (at * a.n_v + h) * kDv + lane * 4) = y[m];
+        }
+    }
+    if (is_v) {
+        float carry = 0.f;
+        for (int t0 = 0; t0 < len; t0 += 32) {
+            const int t = t0 + lane;
+            const size_t at = t < len ? (size_t(b) * a.max_nodes + path[t]) * a.n_v + h : 0;
+            float g = t < len ? a.g_log[at] : 0.f;
+            const float bt = t < len ? a.beta[at] : 0.f;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const float up = __shfl_up_sync(0xffffffffu, g, off);
+                if (lane >= off) g += up;
+            }
+            if (t < len) ws.cb[(size_t(b) * a.n_v + h) * a.max_nodes + t] = make_float2(carry + g, bt);
+            carry += __shfl_sync(0xffffffffu, g, 31);
+        }
+    }
+}
+
+// grid (n_v + ceil(conv_dim / 512), batch).
+// x < n_v: the state of one value head, in registers: warp w holds rows 32 (w / 4) .. and columns 32 (w % 4) .., a
+// lane 8 rows x 4 columns, requested before the wait for the path kernel (only this kernel writes states).  Up to 16
+// tokens at a time in the closed form above.
+// The other blocks, a thread per channel: entry w (oldest first) of the new conv window is input len + w of the old
+// window followed by the path's rows.  The ring keeps its phase: rewriting the four taps of a channel is one 16-byte
+// store either way, and a phase that every block reads could only be advanced by another launch.
+__global__ void __launch_bounds__(kCommitThreads, 2) gdn_tree_commit_kernel(GdnTreeArgs a) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    CommitSmem& s = *reinterpret_cast<CommitSmem*>(smem_raw);
+    const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
+    const int slot = a.slot_ids ? a.slot_ids[b] : b;
+    if (slot < 0 || slot >= a.n_slots || a.leaf[b] < 0 || a.leaf[b] >= a.max_nodes) return;
+    if (int(blockIdx.x) >= a.n_v) {
+        const int c = (blockIdx.x - a.n_v) * kCommitThreads + tid;
+        griddep_wait();
+        if (c >= a.conv_dim) return;
+        const int len = ws.len[b], ph = a.conv_phase ? a.conv_phase[slot] & 3 : 0;
+        float4* ring = reinterpret_cast<float4*>(a.conv_out) + size_t(slot) * a.conv_dim + c;
+        const float4 old = *ring;
+        const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + c;
+        float out[kTaps];
+#pragma unroll
+        for (int w = 0; w < kTaps; ++w) {
+            const int t = len + w - kTaps;                    // of the path; negative: old entry len + w
+            const float y = t >= 0 ? x[ws.path[size_t(b) * a.max_nodes + t] * a.x_stride] : comp(old, (ph + len + w) & 3);
+#pragma unroll
+            for (int p = 0; p < kTaps; ++p)
+                if (((ph + w) & 3) == p) out[p] = y;
+        }
+        *ring = make_float4(out[0], out[1], out[2], out[3]);
+        return;
+    }
+    const int h = blockIdx.x;
+    float* Sh = a.S_out + (size_t(slot) * a.n_v + h) * (kDk * kDv);
+    const int row0 = (warp >> 2) * 32 + (lane >> 3) * 8, col0 = (warp & 3) * 32 + (lane & 7) * 4;
+    float4 st[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) st[r] = __ldcs(reinterpret_cast<const float4*>(Sh + (row0 + r) * kDv + col0));
+    griddep_wait();
+    const int len = ws.len[b], hs = key_head_of(h, a.n_v, a.n_qk, a.head_map);
+    if (tid < len) s.cb[tid] = ws.cb[(size_t(b) * a.n_v + h) * a.max_nodes + tid];
     for (int t0 = 0; t0 < len; t0 += kChunk) {
         const int m = min(kChunk, len - t0);
         if (warp < m) {
-            const int i = s.path[t0 + warp];
-            const int4 src = conv_sources(i, s.parents, int(a.x_stride));
-            const int ck = (a.n_qk + hs) * kDk + lane * 4;
-            Conv4 cv;
-            cv.load(a, slot, ck);
-            const float4 y = unit(conv_node(cv, x + ck, src), a.eps_l2, 1.f);
-            *reinterpret_cast<float4*>(&s.k[warp][lane * 4]) = y;
-            if (lane < kSliceCols / 4) {
-                const int c = 2 * a.n_qk * kDk + h * kDv + slice * kSliceCols + lane * 4;
-                cv.load(a, slot, c);
-                *reinterpret_cast<float4*>(&s.v[warp][lane * 4]) = conv_node(cv, x + c, src);
-            } else if (lane == 31) {
-                s.g[warp] = a.g_log[(size_t(b) * a.max_nodes + i) * a.n_v + h];
-                s.beta[warp] = a.beta[(size_t(b) * a.max_nodes + i) * a.n_v + h];
-            }
-        } else {
-            *reinterpret_cast<float4*>(&s.k[warp][lane * 4]) = make_float4(0.f, 0.f, 0.f, 0.f);
+            const size_t at = size_t(b) * a.max_nodes + t0 + warp;
+            *reinterpret_cast<float4*>(&s.k[warp][lane * 4]) = *reinterpret_cast<const float4*>(ws.k + (at * a.n_qk + hs) * kDk + lane * 4);
+            *reinterpret_cast<float4*>(&s.v[warp][lane * 4]) = *reinterpret_cast<const float4*>(ws.v + (at * a.n_v + h) * kDv + lane * 4);
         }
         __syncthreads();
-        // k_i . k_j for j < i (warp i), and S0^T k of all tokens: 4 rows x 4 columns per thread
-        if (warp < m) {
-            const float4 ki = *reinterpret_cast<const float4*>(&s.k[warp][lane * 4]);
-            for (int j = 0; j < warp; ++j) {
-                const float d = sum_warp(dot4(ki, *reinterpret_cast<const float4*>(&s.k[j][lane * 4]), 0.f));
-                if (lane == 0) s.kk[warp][j] = d;
-            }
+        const float c_in = t0 ? s.cb[t0 - 1].x : 0.f;         // decays are taken from the chunk's start
+        // coefficients: pair (i, j < i) per warp; S0^T k: 8 rows x 4 columns per thread
+        for (int p = warp; p < m * (m - 1) / 2; p += kCommitThreads / 32) {
+            int i = 1, j = p;
+            while (j >= i) j -= i++;
+            const float d = sum_warp(dot4(*reinterpret_cast<const float4*>(&s.k[i][lane * 4]), *reinterpret_cast<const float4*>(&s.k[j][lane * 4]), 0.f));
+            if (lane == 0) s.low[i][j] = s.cb[t0 + i].y * expf(s.cb[t0 + i].x - s.cb[t0 + j].x) * d;
         }
+#pragma unroll 2
+        for (int i = 0; i < m; ++i) {
+            const float4 ka = *reinterpret_cast<const float4*>(&s.k[i][row0]), kb = *reinterpret_cast<const float4*>(&s.k[i][row0 + 4]);
+            const float kr[8] = {ka.x, ka.y, ka.z, ka.w, kb.x, kb.y, kb.z, kb.w};
+            float4 kv = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            if (i >= m) break;
-            const float4 k4 = *reinterpret_cast<const float4*>(&s.k[i][4 * rg]);
-            float4 kv;
-            kv.x = st[0].x * k4.x + st[1].x * k4.y + st[2].x * k4.z + st[3].x * k4.w;
-            kv.y = st[0].y * k4.x + st[1].y * k4.y + st[2].y * k4.z + st[3].y * k4.w;
-            kv.z = st[0].z * k4.x + st[1].z * k4.y + st[2].z * k4.z + st[3].z * k4.w;
-            kv.w = st[0].w * k4.x + st[1].w * k4.y + st[2].w * k4.z + st[3].w * k4.w;
+            for (int r = 0; r < 8; ++r) {
+                kv.x = fmaf(st[r].x, kr[r], kv.x); kv.y = fmaf(st[r].y, kr[r], kv.y);
+                kv.z = fmaf(st[r].z, kr[r], kv.z); kv.w = fmaf(st[r].w, kr[r], kv.w);
+            }
 #pragma unroll
             for (int off = 8; off <= 16; off <<= 1) {
                 kv.x += __shfl_xor_sync(0xffffffffu, kv.x, off);
@@ -718,95 +813,45 @@ __global__ void __launch_bounds__(kCommitThreads) gdn_tree_commit_kernel(GdnTree
                 kv.z += __shfl_xor_sync(0xffffffffu, kv.z, off);
                 kv.w += __shfl_xor_sync(0xffffffffu, kv.w, off);
             }
-            if (lane < 8) *reinterpret_cast<float4*>(&s.red[warp][i][lane * 4]) = kv;
+            if (lane < 8) *reinterpret_cast<float4*>(&s.red[warp >> 2][i][col0]) = kv;
         }
         __syncthreads();
-        if (warp == 0) {
-            // the solve, one column per lane
-            float c = 0.f;
+        // the solve, one column per thread
+        if (tid < kDv) {
             for (int i = 0; i < m; ++i) {
-                c += s.g[i];
-                float t = 0.f;
-#pragma unroll
-                for (int w = 0; w < kCommitThreads / 32; ++w) t += s.red[w][i][lane];
-                float u = s.v[i][lane] - expf(c) * t;
-                float cj = 0.f;
-                for (int j = 0; j < i; ++j) {
-                    cj += s.g[j];
-                    u = fmaf(-expf(c - cj) * s.kk[i][j], s.u[j][lane], u);
-                }
-                s.u[i][lane] = s.beta[i] * u;
+                const float kv = (s.red[0][i][tid] + s.red[1][i][tid]) + (s.red[2][i][tid] + s.red[3][i][tid]);
+                float r = s.cb[t0 + i].y * (s.v[i][tid] - expf(s.cb[t0 + i].x - c_in) * kv);
+                for (int j = 0; j < i; ++j) r = fmaf(-s.low[i][j], s.v[j][tid], r);
+                s.v[i][tid] = r;
             }
         }
         __syncthreads();
-        float c = 0.f;
-        for (int i = 0; i < m; ++i) c += s.g[i];
-        const float e = expf(c);
+        const float c_out = s.cb[t0 + m - 1].x;
+        const float e = expf(c_out - c_in);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 8; ++r) {
             st[r].x *= e; st[r].y *= e; st[r].z *= e; st[r].w *= e;
         }
-        float ci = 0.f;
         for (int i = 0; i < m; ++i) {
-            ci += s.g[i];
-            const float f = expf(c - ci);
-            const float4 k4 = *reinterpret_cast<const float4*>(&s.k[i][4 * rg]);
-            const float4 u4 = *reinterpret_cast<const float4*>(&s.u[i][cg * 4]);
+            const float f = expf(c_out - s.cb[t0 + i].x);
+            const float4 ka = *reinterpret_cast<const float4*>(&s.k[i][row0]), kb = *reinterpret_cast<const float4*>(&s.k[i][row0 + 4]);
+            const float kr[8] = {ka.x, ka.y, ka.z, ka.w, kb.x, kb.y, kb.z, kb.w};
+            float4 u4 = *reinterpret_cast<const float4*>(&s.v[i][col0]);
+            u4.x *= f; u4.y *= f; u4.z *= f; u4.w *= f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float kr = comp(k4, r) * f;
-                st[r].x = fmaf(kr, u4.x, st[r].x);
-                st[r].y = fmaf(kr, u4.y, st[r].y);
-                st[r].z = fmaf(kr, u4.z, st[r].z);
-                st[r].w = fmaf(kr, u4.w, st[r].w);
+            for (int r = 0; r < 8; ++r) {
+                st[r].x = fmaf(kr[r], u4.x, st[r].x); st[r].y = fmaf(kr[r], u4.y, st[r].y);
+                st[r].z = fmaf(kr[r], u4.z, st[r].z); st[r].w = fmaf(kr[r], u4.w, st[r].w);
             }
         }
-        __syncthreads();                                 // k, u, red are rewritten by the next chunk
+        if (t0 + kChunk < len) __syncthreads();               // k, v, red are rewritten by the next chunk
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(Sp + (4 * rg + r) * kDv + col0) = st[r];
+    for (int r = 0; r < 8; ++r) __stcs(reinterpret_cast<float4*>(Sh + (row0 + r) * kDv + col0), st[r]);
 }
 
-// The conv windows after the path: entry w (oldest first) is input len + w of the old window followed by
-// the path's rows.  The ring keeps its phase: rewriting the four taps of a channel is one 16-byte store
-// either way, and a phase that every block reads could only be advanced by another launch.
-// grid (ceil(conv_dim / 256), batch), thread = channel; behind gdn_tree_commit_kernel, which reads the
-// windows.
-__global__ void __launch_bounds__(256) gdn_tree_window_kernel(GdnTreeArgs a) {
-    __shared__ int last[kTaps];                          // node of the new entry w, or ~(old entry)
-    griddep_wait();
-    const int b = blockIdx.y, lane = threadIdx.x & 31;
-    const int slot = a.slot_ids ? a.slot_ids[b] : b, leaf = a.leaf[b];
-    if (slot < 0 || slot >= a.n_slots || leaf < 0 || leaf >= a.max_nodes) return;
-    if (threadIdx.x < 32) {
-        const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, leaf + 1, lane, nullptr);
-        const unsigned long long path = tree::of_node(w.lo, w.hi, leaf);
-        const int len = __popcll(path);
-        if (lane < kTaps && len + lane < kTaps) last[lane] = ~(len + lane);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int i = lane + 32 * z;
-            const int at = __popcll(path & ((1ull << i) - 1)) + kTaps - len;     // entry this node becomes
-            if ((path >> i & 1) && at >= 0) last[at] = i;
-        }
-    }
-    __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.conv_dim) return;
-    const int ph = a.conv_phase ? a.conv_phase[slot] & 3 : 0;
-    float4* ring = reinterpret_cast<float4*>(a.conv_out) + size_t(slot) * a.conv_dim + c;
-    const float4 old = *ring;
-    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + c;
-    float out[4];
-#pragma unroll
-    for (int w = 0; w < kTaps; ++w) {
-        const int i = last[w];
-        const float v = i >= 0 ? x[i * a.x_stride] : comp(old, (ph + ~i) & 3);
-#pragma unroll
-        for (int p = 0; p < kTaps; ++p)
-            if (((ph + w) & 3) == p) out[p] = v;
-    }
-    *ring = make_float4(out[0], out[1], out[2], out[3]);
+size_t gdn_tree_commit_workspace_bytes(int batch, int max_nodes, int n_v, int n_qk) {
+    return commit_workspace(nullptr, batch, max_nodes, n_v, n_qk).bytes;
 }
 
 namespace {
@@ -825,6 +870,8 @@ cudaError_t gdn_tree_setup() {
     if (e == cudaSuccess) e = set_attr<32>();
     if (e == cudaSuccess) e = set_attr<48>();
     if (e == cudaSuccess) e = set_attr<64>();
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(gdn_tree_commit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(CommitSmem)));
     return e;
 }
 
@@ -840,17 +887,18 @@ void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
 }
 
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st) {
-    gdn_tree_commit_kernel<<<dim3(kSlices, unsigned(a.n_v), unsigned(a.batch)), kCommitThreads, 0, st>>>(a);
+    gdn_tree_path_kernel<<<dim3(unsigned((a.n_qk + a.n_v + kPathWarps - 1) / kPathWarps), unsigned(a.batch)), kPathWarps * 32, 0, st>>>(a);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((a.conv_dim + 255) / 256), unsigned(a.batch));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(unsigned(a.n_v + (a.conv_dim + kCommitThreads - 1) / kCommitThreads), unsigned(a.batch));
+    cfg.blockDim = dim3(kCommitThreads);
+    cfg.dynamicSmemBytes = sizeof(CommitSmem);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, gdn_tree_window_kernel, a);
+    return cudaLaunchKernelEx(&cfg, gdn_tree_commit_kernel, a);
 }
 
 }  // namespace rl

@@ -327,7 +327,8 @@ struct AttnTreeArgs {
     size_t gate_row, gate_head;
     int batch, max_nodes, n_q, n_kv, n_pages, max_pages_per_seq, q_type, o_type;
     int max_len;                 // host-side bound of base_len + nodes: the workspace is sized for it
-    int grid, min_share;         // CTAs; least units a CTA takes
+    int grid, min_share;         // CTAs; least cost a CTA takes
+    int boundary;                // charge of a (sequence, head, row tile), in pages
     float scale;
 };
 size_t attn_tree_smem_bytes();
@@ -355,10 +356,12 @@ struct GdnTreeArgs {
     size_t x_stride;
     int batch, max_nodes, n_v, n_qk, n_slots, head_map, conv_dim;
     int heads;                   // verify: value heads of a CTA, 1 or n_v / n_qk (set by the launch)
+    void* workspace;             // commit
     float eps_l2;
 };
 cudaError_t gdn_tree_setup();    // kernel attributes, once per device
 void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st);
+size_t gdn_tree_commit_workspace_bytes(int batch, int max_nodes, int n_v, int n_qk);
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st);
 
 }  // namespace rl

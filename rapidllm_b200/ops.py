@@ -587,7 +587,7 @@ def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk
 
 
 def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, n_qk, slot_ids=None,
-                    head_map=None, eps_l2=1e-6):
+                    head_map=None, eps_l2=1e-6, workspace=None):
     """Advance S and conv_window of each sequence's slot by the path to node leaf[b] (-1 = nothing), in place, with
     gdn_tree's inputs; conv_phase stays.  slot_ids must be distinct."""
     dev = torch.cuda.current_device()
@@ -595,4 +595,8 @@ def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parent
                              head_map, eps_l2)
     if leaf is None:
         raise _lib.RlError(6, "leaf: is None")
-    check(lib().rl_gdn_tree_commit(*args, p, _stream_of(dev)))
+    need = lib().rl_gdn_tree_commit_workspace_bytes(p)
+    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if size < need:
+        workspace, size = torch.empty(need, dtype=torch.uint8, device=S.device), need
+    check(lib().rl_gdn_tree_commit(*args, _arg(workspace, workspace.dtype, workspace.shape, dev, "workspace"), size, p, _stream_of(dev)))

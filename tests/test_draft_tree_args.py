@@ -41,8 +41,9 @@ def _gdn(commit=False, **kw):
     p = _lib.GdnTreeParams(n_v=48, n_qk=16, dk=128, dv=128, conv_k=4, batch=1, max_nodes=8, n_slots=1, head_map=1, eps_l2=1e-6)
     for k, v in kw.items():
         setattr(p, k, v)
-    f, n = (_lib.lib().rl_gdn_tree_commit, 10) if commit else (_lib.lib().rl_gdn_tree, 11)
-    return f(*[None] * n, C.byref(p), None)
+    if commit:
+        return _lib.lib().rl_gdn_tree_commit(*[None] * 11, 0, C.byref(p), None)
+    return _lib.lib().rl_gdn_tree(*[None] * 11, C.byref(p), None)
 
 
 @pytest.mark.parametrize("call,status,kw", [
@@ -72,7 +73,8 @@ def test_null_params_and_empty_calls():
     assert L.rl_attn_tree(*[None] * 10, 0, None, None) == RANGE
     assert L.rl_attn_tree_workspace_bytes(None) == 0
     assert L.rl_kv_tree_commit(*[None] * 9) == RANGE
-    assert L.rl_gdn_tree(*[None] * 13) == RANGE and L.rl_gdn_tree_commit(*[None] * 12) == RANGE
+    assert L.rl_gdn_tree(*[None] * 13) == RANGE and L.rl_gdn_tree_commit(*[None] * 11, 0, None, None) == RANGE
+    assert L.rl_gdn_tree_commit_workspace_bytes(None) == 0
     assert _append(batch=0) == 0 and _append(n_tok=0) == 0
     assert _attn(batch=0) == 0 and _attn(max_nodes=0) == 0
     assert _kv(batch=0) == 0
