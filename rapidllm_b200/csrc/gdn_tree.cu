@@ -623,12 +623,12 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
 // paths in trees of 32: 93 us).
 namespace {
 
-constexpr int kPathWarps = 4, kCommitThreads = 512, kChunk = 16;
+constexpr int kPathWarps = 4, kCommitThreads = 256, kCommitCols = 64, kParts = kDv / kCommitCols, kChunk = 16;
 
 struct CommitSmem {
-    float k[kChunk][kDk], v[kChunk][kDv];                     // v, then u
+    float k[kChunk][kDk], v[kChunk][kCommitCols];             // v, then u
     float low[kChunk][kChunk];                                // coefficient of u_j in u_i
-    float red[4][kChunk][kDv];                                // S0^T k by row blocks
+    float red[4][kChunk][kCommitCols];                        // S0^T k by row blocks
     float2 cb[kMaxNodes];                                     // log decay from the state to the path's token; beta
 };
 // workspace: path lengths, then the path's nodes [batch][max_nodes], (c, beta) [batch][n_v][max_nodes], k
@@ -737,22 +737,23 @@ __global__ void __launch_bounds__(kPathWarps * 32) gdn_tree_path_kernel(GdnTreeA
     }
 }
 
-// grid (n_v + ceil(conv_dim / 512), batch).
-// x < n_v: the state of one value head, in registers: warp w holds rows 32 (w / 4) .. and columns 32 (w % 4) .., a
-// lane 8 rows x 4 columns, requested before the wait for the path kernel (only this kernel writes states).  Up to 16
-// tokens at a time in the closed form above.
+// grid (2 n_v + ceil(conv_dim / 256), batch).
+// x < 2 n_v: 64 columns of one value head's state, in registers: warp w holds rows 32 (w / 2) .. and columns 32 (w % 2)
+// .., a lane 8 rows x 4 columns, requested before the wait for the path kernel (only this kernel writes states).  Four
+// such CTAs fit an SM, so that one's exchanges run under the others' loads and stores (two CTAs of 128 columns: 75
+// against 64 us).  Up to 16 tokens at a time in the closed form above.
 // The other blocks, a thread per channel: entry w (oldest first) of the new conv window is input len + w of the old
 // window followed by the path's rows.  The ring keeps its phase: rewriting the four taps of a channel is one 16-byte
 // store either way, and a phase that every block reads could only be advanced by another launch.
-__global__ void __launch_bounds__(kCommitThreads, 2) gdn_tree_commit_kernel(GdnTreeArgs a) {
+__global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnTreeArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     CommitSmem& s = *reinterpret_cast<CommitSmem*>(smem_raw);
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
     if (slot < 0 || slot >= a.n_slots || a.leaf[b] < 0 || a.leaf[b] >= a.max_nodes) return;
-    if (int(blockIdx.x) >= a.n_v) {
-        const int c = (blockIdx.x - a.n_v) * kCommitThreads + tid;
+    if (int(blockIdx.x) >= kParts * a.n_v) {
+        const int c = (blockIdx.x - kParts * a.n_v) * kCommitThreads + tid;
         griddep_wait();
         if (c >= a.conv_dim) return;
         const int len = ws.len[b], ph = a.conv_phase ? a.conv_phase[slot] & 3 : 0;
@@ -771,9 +772,9 @@ __global__ void __launch_bounds__(kCommitThreads, 2) gdn_tree_commit_kernel(GdnT
         *ring = make_float4(out[0], out[1], out[2], out[3]);
         return;
     }
-    const int h = blockIdx.x;
-    float* Sh = a.S_out + (size_t(slot) * a.n_v + h) * (kDk * kDv);
-    const int row0 = (warp >> 2) * 32 + (lane >> 3) * 8, col0 = (warp & 3) * 32 + (lane & 7) * 4;
+    const int h = blockIdx.x / kParts, part0 = blockIdx.x % kParts * kCommitCols;
+    float* Sh = a.S_out + (size_t(slot) * a.n_v + h) * (kDk * kDv) + part0;
+    const int row0 = (warp >> 1) * 32 + (lane >> 3) * 8, col0 = (warp & 1) * 32 + (lane & 7) * 4;
     float4 st[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) st[r] = __ldcs(reinterpret_cast<const float4*>(Sh + (row0 + r) * kDv + col0));
@@ -782,10 +783,11 @@ __global__ void __launch_bounds__(kCommitThreads, 2) gdn_tree_commit_kernel(GdnT
     if (tid < len) s.cb[tid] = ws.cb[(size_t(b) * a.n_v + h) * a.max_nodes + tid];
     for (int t0 = 0; t0 < len; t0 += kChunk) {
         const int m = min(kChunk, len - t0);
-        if (warp < m) {
-            const size_t at = size_t(b) * a.max_nodes + t0 + warp;
-            *reinterpret_cast<float4*>(&s.k[warp][lane * 4]) = *reinterpret_cast<const float4*>(ws.k + (at * a.n_qk + hs) * kDk + lane * 4);
-            *reinterpret_cast<float4*>(&s.v[warp][lane * 4]) = *reinterpret_cast<const float4*>(ws.v + (at * a.n_v + h) * kDv + lane * 4);
+        for (int i = warp; i < m; i += kCommitThreads / 32) {
+            const size_t at = size_t(b) * a.max_nodes + t0 + i;
+            *reinterpret_cast<float4*>(&s.k[i][lane * 4]) = *reinterpret_cast<const float4*>(ws.k + (at * a.n_qk + hs) * kDk + lane * 4);
+            if (lane < kCommitCols / 4)
+                *reinterpret_cast<float4*>(&s.v[i][lane * 4]) = *reinterpret_cast<const float4*>(ws.v + (at * a.n_v + h) * kDv + part0 + lane * 4);
         }
         __syncthreads();
         const float c_in = t0 ? s.cb[t0 - 1].x : 0.f;         // decays are taken from the chunk's start
@@ -813,11 +815,11 @@ __global__ void __launch_bounds__(kCommitThreads, 2) gdn_tree_commit_kernel(GdnT
                 kv.z += __shfl_xor_sync(0xffffffffu, kv.z, off);
                 kv.w += __shfl_xor_sync(0xffffffffu, kv.w, off);
             }
-            if (lane < 8) *reinterpret_cast<float4*>(&s.red[warp >> 2][i][col0]) = kv;
+            if (lane < 8) *reinterpret_cast<float4*>(&s.red[warp >> 1][i][col0]) = kv;
         }
         __syncthreads();
         // the solve, one column per thread
-        if (tid < kDv) {
+        if (tid < kCommitCols) {
             for (int i = 0; i < m; ++i) {
                 const float kv = (s.red[0][i][tid] + s.red[1][i][tid]) + (s.red[2][i][tid] + s.red[3][i][tid]);
                 float r = s.cb[t0 + i].y * (s.v[i][tid] - expf(s.cb[t0 + i].x - c_in) * kv);
@@ -889,7 +891,7 @@ void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st) {
     gdn_tree_path_kernel<<<dim3(unsigned((a.n_qk + a.n_v + kPathWarps - 1) / kPathWarps), unsigned(a.batch)), kPathWarps * 32, 0, st>>>(a);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.n_v + (a.conv_dim + kCommitThreads - 1) / kCommitThreads), unsigned(a.batch));
+    cfg.gridDim = dim3(unsigned(kParts * a.n_v + (a.conv_dim + kCommitThreads - 1) / kCommitThreads), unsigned(a.batch));
     cfg.blockDim = dim3(kCommitThreads);
     cfg.dynamicSmemBytes = sizeof(CommitSmem);
     cfg.stream = st;
