@@ -508,10 +508,15 @@ typedef struct rl_gdn_tree_params {
  *   conv_window fp32 [n_slots][conv_dim][4] and conv_phase as in rl_gdn_decode, or conv_phase == NULL:
  *               shifted windows, oldest tap first (rl_conv1d_update's state)
  *   qkv fp32 [batch][max_nodes] rows of conv_dim channels;  beta, g_log fp32 [batch][max_nodes][n_v]
- *   o   fp32 [batch][max_nodes][n_v][128] */
+ *   o   fp32 [batch][max_nodes][n_v][128]
+ * beta in [0, 2] and g_log <= 0 as the gates give them (the coefficients between nodes are held in a fixed range);
+ * inputs of all nodes finite (what is not reaches the node's siblings).  workspace: rl_gdn_tree_workspace_bytes()
+ * bytes, 16-byte aligned, for the rows after the conv. */
+size_t rl_gdn_tree_workspace_bytes(const rl_gdn_tree_params* p);
 int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
                 const int32_t* parents, const int32_t* n_nodes, const float* qkv, const float* conv_w,
-                const float* beta, const float* g_log, float* o, const rl_gdn_tree_params* p, void* stream);
+                const float* beta, const float* g_log, float* o, void* workspace, size_t workspace_bytes,
+                const rl_gdn_tree_params* p, void* stream);
 
 /* Keep one path: S and the conv window of each sequence's slot advance by the path's tokens, as that many
  * decode steps would (the sums are in another order).  The window's entries move and conv_phase stays, so no

@@ -200,7 +200,8 @@ SYMBOLS = {
     "rl_attn_tree_workspace_bytes": (_sz, [C.POINTER(AttnTreeParams)]),
     "rl_attn_tree": (_i, [_vp] * 10 + [_sz, C.POINTER(AttnTreeParams), _vp]),
     "rl_kv_tree_commit": (_i, [_vp] * 7 + [C.POINTER(KvTreeCommitParams), _vp]),
-    "rl_gdn_tree": (_i, [_vp] * 11 + [C.POINTER(GdnTreeParams), _vp]),
+    "rl_gdn_tree_workspace_bytes": (_sz, [C.POINTER(GdnTreeParams)]),
+    "rl_gdn_tree": (_i, [_vp] * 11 + [_vp, _sz, C.POINTER(GdnTreeParams), _vp]),
     "rl_gdn_tree_commit_workspace_bytes": (_sz, [C.POINTER(GdnTreeParams)]),
     "rl_gdn_tree_commit": (_i, [_vp] * 11 + [_sz, C.POINTER(GdnTreeParams), _vp]),
     "rl_cache_create": (_i, [C.POINTER(CacheConfig), C.POINTER(_vp)]),

@@ -1674,19 +1674,28 @@ static int gdn_tree_args(rl::GdnTreeArgs* a, const float* S, const float* conv_w
     return RL_OK;
 }
 
+size_t rl_gdn_tree_workspace_bytes(const rl_gdn_tree_params* p) {
+    rl::GdnTreeArgs a = {};
+    if (gdn_tree_check(p, &a)) return 0;
+    return std::max<size_t>(256, rl::gdn_tree_workspace_bytes(p->batch, p->max_nodes, p->n_v, p->n_qk));
+}
+
 int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
                 const int32_t* parents, const int32_t* n_nodes, const float* qkv, const float* conv_w, const float* beta,
-                const float* g_log, float* o, const rl_gdn_tree_params* p, void* stream) {
+                const float* g_log, float* o, void* workspace, size_t workspace_bytes, const rl_gdn_tree_params* p, void* stream) {
     rl::GdnTreeArgs a = {};
     if (int st = gdn_tree_args(&a, S, conv_window, conv_phase, slot_ids, parents, qkv, conv_w, beta, g_log, p)) return st;
     if (p->batch == 0 || p->max_nodes == 0) return RL_OK;
-    if (!o) return fail(RL_ERR_RANGE, "NULL pointer argument");
-    if (!aligned16(o)) return fail(RL_ERR_RANGE, "o must be 16-byte aligned");
+    if (!o || !workspace) return fail(RL_ERR_RANGE, "NULL pointer argument");
+    if (!aligned16(o) || !aligned16(workspace)) return fail(RL_ERR_RANGE, "o and workspace must be 16-byte aligned");
+    const size_t need = rl::gdn_tree_workspace_bytes(p->batch, p->max_nodes, p->n_v, p->n_qk);
+    if (workspace_bytes < need) return fail(RL_ERR_RANGE, "workspace %zu bytes < %zu required", workspace_bytes, need);
     a.n_nodes = n_nodes;
     a.o = o;
+    a.workspace = workspace;
     DevInfo* d;
     if (int st = dev_info(&d)) return st;
-    rl::launch_gdn_tree(a, d->sms, as_stream(stream));
+    RL_CUDA(rl::launch_gdn_tree(a, d->sms, as_stream(stream)));
     RL_CUDA(cudaGetLastError());
     return RL_OK;
 }

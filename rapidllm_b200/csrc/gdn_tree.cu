@@ -139,22 +139,16 @@ struct TreeSmem {
     static constexpr int kSub = 2 * NB * 128;                 // 64 dims of the rows [k; q], 128 bytes each
     static constexpr int kPitch = NB + 4;                     // of the fp32 triangle: 16-byte rows on all banks
     alignas(1024) unsigned char kq[4][kSub];                  // hi dims 0-63, 64-127, lo dims 0-63, 64-127
+    alignas(1024) unsigned char inv[2][NB * 128];             // scratch of the inversion; then T as tiles, hi and lo
     union {
-        float v[NB][kDv];                                     // first: v of all nodes
-        struct {
-            alignas(1024) unsigned char inv[2][NB * 128];     // then: scratch of the inversion; T as tiles, hi and lo
-            union {
-                float tri[NB][kPitch];                        // L, inverted in place
-                alignas(1024) unsigned char mix[2][NB * 128]; // then: coefficients of u_j in o_i as tiles
-            };
-        };
+        float tri[NB][kPitch];                                // L, inverted in place
+        alignas(1024) unsigned char mix[2][NB * 128];         // then: coefficients of u_j in o_i as tiles
     };
     float decay[NB], grow[NB], beta[NB], in[NB];              // c_i log2 e, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
     float amax[2][kDv];
     unsigned long long word[kMaxNodes];
     int parents[kMaxNodes];
-    int4 src[NB];
-    uint64_t bar_gram, bar_half, bar_in, bar_u, bar_out;
+    uint64_t bar_rows, bar_gram, bar_half, bar_in, bar_u, bar_out;
     uint32_t tmem_base;
 };
 template <int NB>
@@ -234,10 +228,75 @@ __device__ __forceinline__ void invert_triangle(float (&t)[NB][P], float* x, int
 // byte offset of fp16 element (row, d < 64) in a tile of 128-byte rows under the 128-byte swizzle
 __device__ __forceinline__ int tile_at(int row, int d) { return row * 128 + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2; }
 
+// Workspace of the verify: the rows [k; q] of every (sequence, key head) as the main kernel's shared memory holds
+// them (4 parts of 2 nb rows of 128 bytes), then v [batch][max_nodes][n_v][128].
+struct VerifyWorkspace {
+    unsigned char* kq;
+    float* v;
+    size_t bytes;
+};
+__host__ __device__ __forceinline__ int rounded_nodes(int max_nodes) { return (max_nodes + 15) / 16 * 16; }
+__host__ __device__ __forceinline__ VerifyWorkspace verify_workspace(void* base, int batch, int max_nodes, int n_v, int n_qk) {
+    VerifyWorkspace w;
+    const size_t kq = size_t(batch) * n_qk * rounded_nodes(max_nodes) * 1024;
+    w.kq = static_cast<unsigned char*>(base);
+    w.v = reinterpret_cast<float*>(static_cast<char*>(base) + kq);
+    w.bytes = kq + size_t(batch) * max_nodes * n_v * kDv * 4;
+    return w;
+}
+constexpr int kPrepWarps = 4, kPrepNodes = 16;
+
 }  // namespace
 
-// One CTA per (key head, sequence) with that key head's value heads one after the other (a.heads > 1), or per
-// (value head, sequence).  Node count rounded up to NB.
+// Conv, SiLU, unit length and split of all rows, before the states are touched: a warp per head (k, q or v) and 16
+// nodes, the taps of four nodes in flight.  grid (ceil((2 n_qk + n_v) / 4), batch, nb / 16).  Inside the main kernel,
+// where few warps share an SM with the states, the same work took more than half of its time (32 chains of 64: 187 us).
+__global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeArgs a) {
+    __shared__ int parents[kMaxNodes];
+    griddep_launch();
+    const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i0 = blockIdx.z * kPrepNodes;
+    const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
+    const int slot = a.slot_ids ? a.slot_ids[b] : b;
+    if (slot < 0 || slot >= a.n_slots || n == 0) return;      // recorded by the main kernel
+    const int role = blockIdx.x * kPrepWarps + warp;          // k heads, q heads, value heads
+    const bool is_v = role >= 2 * a.n_qk, is_q = !is_v && role >= a.n_qk;
+    const int h = is_v ? min(role - 2 * a.n_qk, a.n_v - 1) : (is_q ? role - a.n_qk : role);
+    const int ch = (is_v ? 2 * a.n_qk * kDk + h * kDv : (is_q ? h * kDk : (a.n_qk + h) * kDk)) + lane * 4;
+    Conv4 cv;
+    cv.load(a, slot, ch);
+    if (tid < kMaxNodes) parents[tid] = tree::checked_parent(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, tid, n, a.err);
+    __syncthreads();
+    if (role >= 2 * a.n_qk + a.n_v || (is_v && i0 >= n)) return;
+    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + ch;
+    const int nb = rounded_nodes(a.max_nodes);
+    const VerifyWorkspace ws = verify_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
+    for (int i = i0; i < i0 + kPrepNodes; i += 4) {
+        int4 src[4];
+        float4 y[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) src[m] = conv_sources(min(i + m, n - 1), parents, int(a.x_stride));
+        conv_nodes(cv, x, src, y);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (is_v) {
+                if (i + m < n) *reinterpret_cast<float4*>(ws.v + ((size_t(b) * a.max_nodes + i + m) * a.n_v + h) * kDv + lane * 4) = y[m];
+            } else {
+                y[m] = unit(y[m], a.eps_l2, kLift);
+                if (i + m >= n) y[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+                uint2 hi, lo;
+                split2(y[m].x, y[m].y, hi.x, lo.x);
+                split2(y[m].z, y[m].w, hi.y, lo.y);
+                unsigned char* part = ws.kq + (size_t(b) * a.n_qk + h) * nb * 1024 + (lane >> 4) * (nb * 256);
+                const int at = tile_at((is_q ? nb : 0) + i + m, (lane * 4) & 63);
+                *reinterpret_cast<uint2*>(part + at) = hi;
+                *reinterpret_cast<uint2*>(part + nb * 512 + at) = lo;
+            }
+        }
+    }
+}
+
+// The rest, behind gdn_tree_rows_kernel: one CTA per (key head, sequence) with that key head's value heads one after
+// the other (a.heads > 1), or per (value head, sequence).  Node count rounded up to NB.
 //
 // S0^T k and S0^T q of all nodes are one product per value head, D[v][row] = sum_d S0[d][v] [k; q][row][d],
 // with the state as the A operand in tensor memory (a thread reads column v of the state with coalesced loads
@@ -283,31 +342,20 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         for (int d = 0; d < kDk / 2; ++d) st[d] = __ldcs(S + d * kDv);
     };
 
-    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride;
-    // all that this CTA will read starts on its way into L2: the stages below wait for it one after the other
-    {
-        auto line = [](const float* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); };
-        const int rows = 2 + a.heads;                         // segments of 128 channels: q, k, v of the heads
-        auto channel = [&](int r) { return r == 0 ? hs * kDk : (r == 1 ? (a.n_qk + hs) * kDk : 2 * a.n_qk * kDk + (h0 + (r - 2) * h_step) * kDv); };
-        for (int i = tid; i < rows * n * 4; i += kThreads) line(x + (i >> 2) % n * a.x_stride + channel((i >> 2) / n) + (i & 3) * 32);
-        for (int i = tid; i < rows * 16; i += kThreads) {
-            line(a.w + size_t(channel(i >> 4)) * kTaps + (i & 15) * 32);
-            line(a.conv + (size_t(slot) * a.conv_dim + channel(i >> 4)) * kTaps + (i & 15) * 32);
-        }
-        for (int i = tid; i < a.heads * 512; i += kThreads)
-            line(a.S + (size_t(slot) * a.n_v + h0 + (i >> 9) * h_step) * (kDk * kDv) + (i & 511) * 32);
-    }
+    // the other heads' states start on their way into L2
+    for (int i = tid; i < (a.heads - 1) * 512; i += kThreads)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.S + (size_t(slot) * a.n_v + h0 + ((i >> 9) + 1) * h_step) * (kDk * kDv) + (i & 511) * 32));
+    fetch(h0);
     if (warp == 0) {
         const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, n, lane, a.err);
         s.word[lane] = w.lo;
         s.word[lane + 32] = w.hi;
         s.parents[lane] = w.parent_lo;
         s.parents[lane + 32] = w.parent_hi;
-        __syncwarp();
-        for (int i = lane; i < n; i += 32) s.src[i] = conv_sources(i, s.parents, int(a.x_stride));
     } else if (warp == 1) {
         tc::tmem_alloc(&s.tmem_base, kCols);
     } else if (tid == 64) {
+        mbar_init(&s.bar_rows, 1);
         mbar_init(&s.bar_gram, 1);
         mbar_init(&s.bar_half, 1);
         mbar_init(&s.bar_in, 1);
@@ -327,36 +375,14 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         }
     };
 
-    // ---- k and q of all nodes: conv, SiLU, unit length, split; a warp per node, 4 dims per lane ----
-#pragma unroll 1
-    for (int role = 0; role < 2; ++role) {                    // 0: k, 1: q
-        const int c0 = (role == 0 ? (a.n_qk + hs) * kDk : hs * kDk) + lane * 4;
-        Conv4 cv;
-        cv.load(a, slot, c0);
-        for (int i0 = warp; i0 < NB; i0 += kConv * kWarps) {
-            int4 src[kConv];
-            float4 y[kConv];
-#pragma unroll
-            for (int m = 0; m < kConv; ++m) src[m] = s.src[min(i0 + m * kWarps, n - 1)];
-            conv_nodes(cv, x + c0, src, y);
-#pragma unroll
-            for (int m = 0; m < kConv; ++m) {
-                const int i = i0 + m * kWarps;
-                if (i >= NB) break;
-                y[m] = unit(y[m], a.eps_l2, kLift);
-                if (i >= n) y[m] = make_float4(0.f, 0.f, 0.f, 0.f);
-                uint2 hi, lo;
-                split2(y[m].x, y[m].y, hi.x, lo.x);
-                split2(y[m].z, y[m].w, hi.y, lo.y);
-                const int at = tile_at(role * NB + i, (lane * 4) & 63);
-                *reinterpret_cast<uint2*>(s.kq[lane >> 4] + at) = hi;
-                *reinterpret_cast<uint2*>(s.kq[2 + (lane >> 4)] + at) = lo;
-            }
-        }
+    const VerifyWorkspace ws = verify_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
+    griddep_wait();                                           // the rows; all that was read so far was there before
+    if (tid == 0) {
+        mbar_arrive_expect_tx(&s.bar_rows, sizeof(s.kq));
+        bulk_g2s(s.kq, ws.kq + (size_t(b) * a.n_qk + hs) * sizeof(s.kq), sizeof(s.kq), &s.bar_rows);
     }
-    fetch(h0);
-    tc::fence_async_smem();
-    __syncthreads();
+    __syncwarp();
+    wait(&s.bar_rows, 0);
     auto kq_desc = [&](int part) { return tc::smem_desc(smem_u32(s.kq[part]), 16, 1024); };
     if (tid == 0) {
         // [k; q] k^T, lane = row
@@ -444,30 +470,15 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             }
             tc::commit(grp ? &s.bar_in : &s.bar_half);
         }
-        // ---- v of all nodes: conv and SiLU by rows (a warp per node), handed over by columns ----
+        float u[kMine];                                       // column v of W, later of U, at this group's nodes
         {
-            const int c0 = 2 * a.n_qk * kDk + h * kDv + lane * 4;
-            Conv4 cv;
-            cv.load(a, slot, c0);
-            for (int i0 = warp; i0 < n; i0 += kConv * kWarps) {
-                int4 src[kConv];
-                float4 y[kConv];
+            const float* vp = ws.v + (size_t(b) * a.max_nodes * a.n_v + h) * kDv + v;
 #pragma unroll
-                for (int m = 0; m < kConv; ++m) src[m] = s.src[min(i0 + m * kWarps, n - 1)];
-                conv_nodes(cv, x + c0, src, y);
-#pragma unroll
-                for (int m = 0; m < kConv; ++m)
-                    if (i0 + m * kWarps < n) *reinterpret_cast<float4*>(&s.v[i0 + m * kWarps][lane * 4]) = y[m];
+            for (int e = 0; e < kMine; ++e) {
+                const int i = grp * kMine + e;
+                u[e] = i < n ? vp[size_t(i) * a.n_v * kDv] : 0.f;
             }
         }
-        __syncthreads();
-        float u[kMine];                                       // column v of W, later of U, at this group's nodes
-#pragma unroll
-        for (int e = 0; e < kMine; ++e) {
-            const int i = grp * kMine + e;
-            u[e] = i < n ? s.v[i][v] * s.beta[i] : 0.f;
-        }
-        __syncthreads();
         // ---- this head's coefficients, half a row of [k; q] k^T per thread: L to shared memory, those of o kept ----
         float m[kMine];
         {
@@ -523,7 +534,8 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             tc::tmem_ld8(lanes + kColD + grp * kMine + c, d);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[c + e] = fmaf(__uint_as_float(d[e]) * back, s.in[grp * kMine + c + e], u[c + e]);
+            for (int e = 0; e < 8; ++e)
+                u[c + e] = fmaf(__uint_as_float(d[e]) * back, s.in[grp * kMine + c + e], u[c + e] * s.beta[grp * kMine + c + e]);
         }
         // column v of W or U, both halves' largest magnitude scaled into place -> A; returns the scale's inverse
         auto store_column = [&]() {
@@ -857,13 +869,29 @@ size_t gdn_tree_commit_workspace_bytes(int batch, int max_nodes, int n_v, int n_
 }
 
 namespace {
+// a launch that may become resident while the kernel before it runs (both call griddep_*)
+cudaError_t launch_behind(void (*kernel)(GdnTreeArgs), dim3 grid, int threads, size_t smem, cudaStream_t st, const GdnTreeArgs& a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
 template <int NB>
 cudaError_t set_attr() {
     return cudaFuncSetAttribute(gdn_tree_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(tree_smem_bytes<NB>()));
 }
 template <int NB>
-void launch(const GdnTreeArgs& a, cudaStream_t st) {
-    gdn_tree_kernel<NB><<<dim3(unsigned(a.n_v / a.heads), unsigned(a.batch)), kThreads, tree_smem_bytes<NB>(), st>>>(a);
+cudaError_t launch(const GdnTreeArgs& a, cudaStream_t st) {
+    gdn_tree_rows_kernel<<<dim3(unsigned((2 * a.n_qk + a.n_v + kPrepWarps - 1) / kPrepWarps), unsigned(a.batch), NB / kPrepNodes),
+                           kPrepWarps * 32, 0, st>>>(a);
+    return launch_behind(gdn_tree_kernel<NB>, dim3(unsigned(a.n_v / a.heads), unsigned(a.batch)), kThreads, tree_smem_bytes<NB>(), st, a);
 }
 }  // namespace
 
@@ -877,30 +905,26 @@ cudaError_t gdn_tree_setup() {
     return e;
 }
 
-void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
+cudaError_t launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
     // one CTA per value head while that leaves SMs without a second CTA; else a key head's value heads share
-    // the preparation of its k and q rows
-    const int ratio = a.n_v / a.n_qk;
-    a.heads = a.batch * a.n_v <= 2 * sms ? 1 : ratio;
-    if (a.max_nodes <= 16) launch<16>(a, st);
-    else if (a.max_nodes <= 32) launch<32>(a, st);
-    else if (a.max_nodes <= 48) launch<48>(a, st);
-    else launch<64>(a, st);
+    // its rows and their products
+    a.heads = a.batch * a.n_v <= 2 * sms ? 1 : a.n_v / a.n_qk;
+    switch (rounded_nodes(a.max_nodes)) {
+        case 16: return launch<16>(a, st);
+        case 32: return launch<32>(a, st);
+        case 48: return launch<48>(a, st);
+        default: return launch<64>(a, st);
+    }
+}
+
+size_t gdn_tree_workspace_bytes(int batch, int max_nodes, int n_v, int n_qk) {
+    return verify_workspace(nullptr, batch, max_nodes, n_v, n_qk).bytes;
 }
 
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st) {
     gdn_tree_path_kernel<<<dim3(unsigned((a.n_qk + a.n_v + kPathWarps - 1) / kPathWarps), unsigned(a.batch)), kPathWarps * 32, 0, st>>>(a);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(kParts * a.n_v + (a.conv_dim + kCommitThreads - 1) / kCommitThreads), unsigned(a.batch));
-    cfg.blockDim = dim3(kCommitThreads);
-    cfg.dynamicSmemBytes = sizeof(CommitSmem);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, gdn_tree_commit_kernel, a);
+    return launch_behind(gdn_tree_commit_kernel, dim3(unsigned(kParts * a.n_v + (a.conv_dim + kCommitThreads - 1) / kCommitThreads), unsigned(a.batch)),
+                         kCommitThreads, sizeof(CommitSmem), st, a);
 }
 
 }  // namespace rl

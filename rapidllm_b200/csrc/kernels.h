@@ -356,11 +356,12 @@ struct GdnTreeArgs {
     size_t x_stride;
     int batch, max_nodes, n_v, n_qk, n_slots, head_map, conv_dim;
     int heads;                   // verify: value heads of a CTA, 1 or n_v / n_qk (set by the launch)
-    void* workspace;             // commit
+    void* workspace;
     float eps_l2;
 };
 cudaError_t gdn_tree_setup();    // kernel attributes, once per device
-void launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st);
+size_t gdn_tree_workspace_bytes(int batch, int max_nodes, int n_v, int n_qk);
+cudaError_t launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st);
 size_t gdn_tree_commit_workspace_bytes(int batch, int max_nodes, int n_v, int n_qk);
 cudaError_t launch_gdn_tree_commit(const GdnTreeArgs& a, cudaStream_t st);
 

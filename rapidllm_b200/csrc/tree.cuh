@@ -17,25 +17,28 @@ __device__ __forceinline__ T of_node(T lo, T hi, int i) {
     return i & 32 ? b : a;
 }
 
+// parent of node i < n of one sequence's row (null: a chain); one that is not in [-1, i) records DEV_ERR_BAD_TREE and
+// counts as -1
+__device__ __forceinline__ int checked_parent(const int32_t* parents, int i, int n, int* err) {
+    if (i >= n) return -1;
+    if (!parents) return i - 1;
+    const int p = parents[i];
+    if (p >= -1 && p < i) return p;
+    set_err(err, DEV_ERR_BAD_TREE);
+    return -1;
+}
+
 // Called by one full warp.  parents: one sequence's row, or null for a chain; n nodes.  Returns the
 // ancestor words of the nodes lane (lo) and lane + 32 (hi), and their checked parents (-1 for a
-// root).  A parent that is not in [-1, i) records DEV_ERR_BAD_TREE and counts as -1.
+// root).
 struct Words {
     unsigned long long lo, hi;
     int parent_lo, parent_hi;
 };
 __device__ __forceinline__ Words ancestors(const int32_t* parents, int n, int lane, int* err) {
     Words w;
-    auto parent = [&](int i) {
-        if (i >= n) return -1;
-        if (!parents) return i - 1;
-        const int p = parents[i];
-        if (p >= -1 && p < i) return p;
-        set_err(err, DEV_ERR_BAD_TREE);
-        return -1;
-    };
-    w.parent_lo = parent(lane);
-    w.parent_hi = parent(lane + 32);
+    w.parent_lo = checked_parent(parents, lane, n, err);
+    w.parent_hi = checked_parent(parents, lane + 32, n, err);
     w.lo = 1ull << lane;
     w.hi = 1ull << (lane + 32);
     int jl = w.parent_lo, jh = w.parent_hi;

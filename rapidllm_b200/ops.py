@@ -439,6 +439,15 @@ def _row_distance(shape, strides, inner, name):
     return row
 
 
+def _scratch(workspace, need, device):
+    """The caller's workspace where it is large enough, else a new one; and its size."""
+    if workspace is not None:
+        size = workspace.numel() * workspace.element_size()
+        if size >= need:
+            return workspace, size
+    return torch.empty(need, dtype=torch.uint8, device=device), need
+
+
 def _pools(k_pool, v_pool, page_table, batch, dev):
     shape = k_pool.shape
     if len(shape) != 3 or shape[2] != PAGE_TOKENS * HEAD_DIM:
@@ -523,9 +532,7 @@ def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=Non
         gate_p = gate.data_ptr()
     p, need = _attn_tree_plan(dev, n_q, n_kv, hd, batch, nodes, PAGE_TOKENS, n_pages, pages,
                               pages * PAGE_TOKENS if max_seq_len is None else max_seq_len, _TYPES[q.dtype], _TYPES[out.dtype], row, head)
-    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    if size < need:
-        workspace, size = torch.empty(need, dtype=torch.uint8, device=q.device), need
+    workspace, size = _scratch(workspace, need, q.device)
     check(lib().rl_attn_tree(kp, vp, table, _needed(base_len, _I32, (batch,), dev, "base_len"),
                              _arg(parents, _I32, (batch, nodes), dev, "parents"), _arg(n_nodes, _I32, (batch,), dev, "n_nodes"),
                              _arg(q, q.dtype, shape, dev, "q"), gate_p, _arg(out, out.dtype, shape, dev, "out"),
@@ -571,7 +578,7 @@ def _gdn_tree_args(dev, S, conv_window, conv_phase, qkv, conv_w, beta, g_log, pa
 
 
 def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk, n_nodes=None, slot_ids=None,
-             head_map=None, eps_l2=1e-6, out=None):
+             head_map=None, eps_l2=1e-6, out=None, workspace=None):
     """The Gated DeltaNet step of every node of a draft tree, each along its own path; S [n_slots][n_v][128][128]
     and conv_window [n_slots][conv_dim][4] are only read.  conv_phase int32 [n_slots] (rings, see gdn_decode) or
     None (shifted windows, conv1d_update's state).  qkv fp32 [batch][nodes][conv_dim] (rows may be a column range),
@@ -582,7 +589,9 @@ def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk
     shape = (qkv.shape[0], qkv.shape[1], S.shape[1], S.shape[3])
     if out is None:
         out = torch.empty(shape, dtype=_F32, device=S.device)
-    check(lib().rl_gdn_tree(*args, _arg(out, _F32, shape, dev, "out"), p, _stream_of(dev)))
+    workspace, size = _scratch(workspace, lib().rl_gdn_tree_workspace_bytes(p), S.device)
+    check(lib().rl_gdn_tree(*args, _arg(out, _F32, shape, dev, "out"), _arg(workspace, workspace.dtype, workspace.shape, dev, "workspace"),
+                            size, p, _stream_of(dev)))
     return out
 
 
@@ -595,8 +604,5 @@ def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parent
                              head_map, eps_l2)
     if leaf is None:
         raise _lib.RlError(6, "leaf: is None")
-    need = lib().rl_gdn_tree_commit_workspace_bytes(p)
-    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    if size < need:
-        workspace, size = torch.empty(need, dtype=torch.uint8, device=S.device), need
+    workspace, size = _scratch(workspace, lib().rl_gdn_tree_commit_workspace_bytes(p), S.device)
     check(lib().rl_gdn_tree_commit(*args, _arg(workspace, workspace.dtype, workspace.shape, dev, "workspace"), size, p, _stream_of(dev)))

@@ -43,7 +43,7 @@ def _gdn(commit=False, **kw):
         setattr(p, k, v)
     if commit:
         return _lib.lib().rl_gdn_tree_commit(*[None] * 11, 0, C.byref(p), None)
-    return _lib.lib().rl_gdn_tree(*[None] * 11, C.byref(p), None)
+    return _lib.lib().rl_gdn_tree(*[None] * 12, 0, C.byref(p), None)
 
 
 @pytest.mark.parametrize("call,status,kw", [
@@ -73,7 +73,7 @@ def test_null_params_and_empty_calls():
     assert L.rl_attn_tree(*[None] * 10, 0, None, None) == RANGE
     assert L.rl_attn_tree_workspace_bytes(None) == 0
     assert L.rl_kv_tree_commit(*[None] * 9) == RANGE
-    assert L.rl_gdn_tree(*[None] * 13) == RANGE and L.rl_gdn_tree_commit(*[None] * 11, 0, None, None) == RANGE
+    assert L.rl_gdn_tree(*[None] * 12, 0, None, None) == RANGE and L.rl_gdn_tree_workspace_bytes(None) == 0 and L.rl_gdn_tree_commit(*[None] * 11, 0, None, None) == RANGE
     assert L.rl_gdn_tree_commit_workspace_bytes(None) == 0
     assert _append(batch=0) == 0 and _append(n_tok=0) == 0
     assert _attn(batch=0) == 0 and _attn(max_nodes=0) == 0
