@@ -182,16 +182,16 @@ __device__ __forceinline__ void invert_triangle(float (&t)[NB][P], float* x, int
         float y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float r = i == c ? 1.f : 0.f;
+            float r[4] = {i == c ? 1.f : 0.f, 0.f, 0.f, 0.f};       // four sums: no 15-step chain
 #pragma unroll
             for (int j = 0; j < i; j += 4) {
                 const float4 l = *reinterpret_cast<const float4*>(&t[r0 + i][r0 + j]);
-                r = fmaf(-l.x, y[j], r);
-                if (j + 1 < i) r = fmaf(-l.y, y[j + 1], r);
-                if (j + 2 < i) r = fmaf(-l.z, y[j + 2], r);
-                if (j + 3 < i) r = fmaf(-l.w, y[j + 3], r);
+                r[0] = fmaf(-l.x, y[j], r[0]);
+                if (j + 1 < i) r[1] = fmaf(-l.y, y[j + 1], r[1]);
+                if (j + 2 < i) r[2] = fmaf(-l.z, y[j + 2], r[2]);
+                if (j + 3 < i) r[3] = fmaf(-l.w, y[j + 3], r[3]);
             }
-            y[i] = r;
+            y[i] = (r[0] + r[1]) + (r[2] + r[3]);
         }
         __syncwarp();
         if (tid < NB) {
@@ -253,6 +253,7 @@ constexpr int kPrepWarps = 4, kPrepNodes = 16;
 // where few warps share an SM with the states, the same work took more than half of its time (32 chains of 64: 187 us).
 __global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeArgs a) {
     __shared__ int parents[kMaxNodes];
+    __shared__ int4 sources[kPrepNodes];
     griddep_launch();
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i0 = blockIdx.z * kPrepNodes;
     const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
@@ -266,6 +267,8 @@ __global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeA
     cv.load(a, slot, ch);
     if (tid < kMaxNodes) parents[tid] = tree::checked_parent(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, tid, n, a.err);
     __syncthreads();
+    if (tid < kPrepNodes) sources[tid] = conv_sources(min(i0 + tid, n - 1), parents, int(a.x_stride));
+    __syncthreads();
     if (role >= 2 * a.n_qk + a.n_v || (is_v && i0 >= n)) return;
     const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + ch;
     const int nb = rounded_nodes(a.max_nodes);
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeA
         int4 src[4];
         float4 y[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) src[m] = conv_sources(min(i + m, n - 1), parents, int(a.x_stride));
+        for (int m = 0; m < 4; ++m) src[m] = sources[i - i0 + m];
         conv_nodes(cv, x, src, y);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -485,7 +488,9 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             const bool is_q = v >= NB;
             const int i = is_q ? v - NB : v;
             const bool row = v < 2 * NB && i < n;
-            const unsigned long long word = row ? s.word[i] : 0ull;
+            // this half's columns that count: ancestors, and for o the node itself
+            const unsigned long long word = row ? (is_q ? s.word[i] : s.word[i] & ~(1ull << i)) : 0ull;
+            const uint32_t on = uint32_t(word >> (grp * kMine));
             const float ci = row ? s.decay[i] : 0.f;
             const float f_ = is_q ? kBack * 0.08838834764831845f : (row ? s.beta[i] * kBack * kBack : 0.f);      // 1 / sqrt(128)
 #pragma unroll
@@ -495,9 +500,14 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                 tc::tmem_ld8(lanes + kColG + j0, g);
                 tc::tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool on = (word >> (j0 + e) & 1) && (is_q || j0 + e < i);
-                    m[c + e] = on ? fast_exp2(ci - s.decay[j0 + e]) * f_ * __uint_as_float(g[e]) : 0.f;
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 d4 = *reinterpret_cast<const float4*>(&s.decay[j0 + e]);
+                    const float cj[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const float y = fast_exp2(ci - cj[z]) * (f_ * __uint_as_float(g[e + z]));     // no branch: what does not count is dropped
+                        m[c + e + z] = on >> (c + e + z) & 1 ? y : 0.f;
+                    }
                 }
                 if (v < NB) {
                     *reinterpret_cast<float4*>(&s.tri[i][j0]) = make_float4(m[c], m[c + 1], m[c + 2], m[c + 3]);
