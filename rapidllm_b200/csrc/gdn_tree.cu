@@ -448,16 +448,15 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         __syncthreads();
         float back;
         const float f = lift(fmaxf(s.amax[0][v], s.amax[1][v]), back);
-        if (grp == 1) wait(&s.bar_half, par);                 // the first half's products are done with A
+        {
+            uint32_t th[32], tl[32];
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-            uint32_t h8[8], l8[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) split2(st[2 * (c + e)] * f, st[2 * (c + e) + 1] * f, h8[e], l8[e]);
-            tc::tmem_st8(lanes + kColA + c, h8);
-            tc::tmem_st8(lanes + kColA + 32 + c, l8);
+            for (int c = 0; c < 32; ++c) split2(st[2 * c] * f, st[2 * c + 1] * f, th[c], tl[c]);
+            if (grp == 1) wait(&s.bar_half, par);             // the first half's products are done with A
+            tc::tmem_st32(lanes + kColA, th);
+            tc::tmem_st32(lanes + kColA + 32, tl);
+            tc::tmem_wait_st();
         }
-        tc::tmem_wait_st();
         tc::fence_before_sync();
         named_bar_sync(1 + grp, kHalf);
         if ((tid & (kHalf - 1)) == 0) {
