@@ -44,8 +44,13 @@ struct Conv4 {
 };
 __device__ __forceinline__ float comp(const float4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
-// hardware exponential and quotient: within 2^-21 for the magnitudes that matter, 2 instructions instead of 20
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+// v / (1 + e^-v) by the hardware exponential and reciprocal: within 2^-21 for the magnitudes that matter, in five
+// instructions (far below, e^-v = inf makes it -0)
+__device__ __forceinline__ float silu(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(v * -1.4426950408889634f)));
+    return v * r;
+}
 
 // SiLU(conv) of channels c0 .. c0+3 at M nodes, all their taps requested before the first is used: taps are the
 // node, its parent, ... (src.x .. src.w: offsets of their rows in floats; negative: window entry ~src).
@@ -244,14 +249,14 @@ __host__ __device__ __forceinline__ VerifyWorkspace verify_workspace(void* base,
     w.bytes = kq + size_t(batch) * max_nodes * n_v * kDv * 4;
     return w;
 }
-constexpr int kPrepWarps = 4, kPrepNodes = 16;
+constexpr int kPrepWarps = 4, kPrepNodes = 16, kPrepAhead = 2;
 
 }  // namespace
 
 // Conv, SiLU, unit length and split of all rows, before the states are touched: a warp per head (k, q or v) and 16
-// nodes, the taps of four nodes in flight.  grid (ceil((2 n_qk + n_v) / 4), batch, nb / 16).  Inside the main kernel,
+// nodes, the taps of two nodes in flight.  grid (ceil((2 n_qk + n_v) / 4), batch, nb / 16).  Inside the main kernel,
 // where few warps share an SM with the states, the same work took more than half of its time (32 chains of 64: 187 us).
-__global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeArgs a) {
+__global__ void __launch_bounds__(kPrepWarps * 32, 6) gdn_tree_rows_kernel(GdnTreeArgs a) {
     __shared__ int parents[kMaxNodes];
     __shared__ int4 sources[kPrepNodes];
     griddep_launch();
@@ -263,6 +268,11 @@ __global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeA
     const bool is_v = role >= 2 * a.n_qk, is_q = !is_v && role >= a.n_qk;
     const int h = is_v ? min(role - 2 * a.n_qk, a.n_v - 1) : (is_q ? role - a.n_qk : role);
     const int ch = (is_v ? 2 * a.n_qk * kDk + h * kDv : (is_q ? h * kDk : (a.n_qk + h) * kDk)) + lane * 4;
+    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + ch;
+    // the warp's own rows, 4 lines each, are requested before the tree and the weights are known
+#pragma unroll
+    for (int z = 0; z < kPrepNodes / 8; ++z)
+        if (i0 + z * 8 + (lane >> 2) < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(x - lane * 4 + (i0 + z * 8 + (lane >> 2)) * a.x_stride + (lane & 3) * 32));
     Conv4 cv;
     cv.load(a, slot, ch);
     if (tid < kMaxNodes) parents[tid] = tree::checked_parent(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, tid, n, a.err);
@@ -270,17 +280,16 @@ __global__ void __launch_bounds__(kPrepWarps * 32) gdn_tree_rows_kernel(GdnTreeA
     if (tid < kPrepNodes) sources[tid] = conv_sources(min(i0 + tid, n - 1), parents, int(a.x_stride));
     __syncthreads();
     if (role >= 2 * a.n_qk + a.n_v || (is_v && i0 >= n)) return;
-    const float* x = a.x + size_t(b) * a.max_nodes * a.x_stride + ch;
     const int nb = rounded_nodes(a.max_nodes);
     const VerifyWorkspace ws = verify_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
-    for (int i = i0; i < i0 + kPrepNodes; i += 4) {
-        int4 src[4];
-        float4 y[4];
+    for (int i = i0; i < i0 + kPrepNodes; i += kPrepAhead) {
+        int4 src[kPrepAhead];
+        float4 y[kPrepAhead];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) src[m] = sources[i - i0 + m];
+        for (int m = 0; m < kPrepAhead; ++m) src[m] = sources[i - i0 + m];
         conv_nodes(cv, x, src, y);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < kPrepAhead; ++m) {
             if (is_v) {
                 if (i + m < n) *reinterpret_cast<float4*>(ws.v + ((size_t(b) * a.max_nodes + i + m) * a.n_v + h) * kDv + lane * 4) = y[m];
             } else {
