@@ -388,16 +388,14 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     };
 
     const VerifyWorkspace ws = verify_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
-    griddep_wait();                                           // the rows; all that was read so far was there before
-    if (tid == 0) {
+    auto kq_desc = [&](int part) { return tc::smem_desc(smem_u32(s.kq[part]), 16, 1024); };
+    // one thread: the rows into shared memory, then [k; q] k^T (lane = row).  Everything in front of it reads inputs that
+    // were there before the rows kernel started, and runs beside it.
+    auto gram = [&]() {
+        griddep_wait();
         mbar_arrive_expect_tx(&s.bar_rows, sizeof(s.kq));
         bulk_g2s(s.kq, ws.kq + (size_t(b) * a.n_qk + hs) * sizeof(s.kq), sizeof(s.kq), &s.bar_rows);
-    }
-    __syncwarp();
-    wait(&s.bar_rows, 0);
-    auto kq_desc = [&](int part) { return tc::smem_desc(smem_u32(s.kq[part]), 16, 1024); };
-    if (tid == 0) {
-        // [k; q] k^T, lane = row
+        if (!mbar_wait(&s.bar_rows, 0)) set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
         constexpr uint32_t idesc = tc::idesc_f16(128, NB, false, false);
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
@@ -408,9 +406,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                            pass > 0 || kk > 0);
         }
         tc::commit(&s.bar_gram);
-    }
-    wait(&s.bar_gram, 0);
-    tc::fence_after_sync();
+    };
 
 #pragma unroll 1
     for (int hi = 0; hi < a.heads; ++hi) {
@@ -470,6 +466,8 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         named_bar_sync(1 + grp, kHalf);
         if ((tid & (kHalf - 1)) == 0) {
             tc::fence_after_sync();
+            if (hi == 0 && grp == 0) gram();
+            if (hi == 0 && grp == 1 && !mbar_wait(&s.bar_rows, 0)) set_err(a.err, DEV_ERR_WAIT_TIMEOUT);
             constexpr uint32_t idesc = tc::idesc_f16(128, 2 * NB, false, false);
 #pragma unroll 1
             for (int pass = 0; pass < 3; ++pass) {
@@ -483,6 +481,8 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         }
         float u[kMine];                                       // column v of W, later of U, at this group's nodes
         {
+            __syncwarp();
+            if (hi == 0) griddep_wait();
             const float* vp = ws.v + (size_t(b) * a.max_nodes * a.n_v + h) * kDv + v;
 #pragma unroll
             for (int e = 0; e < kMine; ++e) {
@@ -492,6 +492,10 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         }
         // ---- this head's coefficients, half a row of [k; q] k^T per thread: L to shared memory, those of o kept ----
         float m[kMine];
+        if (hi == 0) {
+            wait(&s.bar_gram, 0);
+            tc::fence_after_sync();
+        }
         {
             const bool is_q = v >= NB;
             const int i = is_q ? v - NB : v;
@@ -924,8 +928,8 @@ cudaError_t gdn_tree_setup() {
 }
 
 cudaError_t launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
-    // one CTA per value head while that leaves SMs without a second CTA; else a key head's value heads share
-    // its rows and their products
+    // one CTA per value head while that leaves SMs without a second CTA; else a key head's value heads share its rows
+    // and their products (16 trees of 21: 47.5 us shared, 48.9 not; 32 chains of 64: 156 and 159)
     a.heads = a.batch * a.n_v <= 2 * sms ? 1 : a.n_v / a.n_qk;
     switch (rounded_nodes(a.max_nodes)) {
         case 16: return launch<16>(a, st);
