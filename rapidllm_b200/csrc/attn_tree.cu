@@ -580,10 +580,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
 }
 
 // Rows whose pages were divided: log-sum-exp over the row's slots (log2 domain), gate, rounding.  A block takes 16
-// rows of a row tile, a thread 16 dims of one row (lane = row: 32 bytes of 16 rows are contiguous in a slot); four
+// rows of a row tile, a thread 8 dims of one row (lane = row: 32 bytes of 16 rows are contiguous in a slot); four
 // slots are in flight.  grid (n_kv * row tiles * 8, batch).
-constexpr int kMergeRows = 16, kAhead = 4;
-__global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
+constexpr int kMergeRows = 16, kAhead = 4, kMergeThreads = kMergeRows * kHeadDim / 8;
+__global__ void __launch_bounds__(kMergeThreads, 2) attn_tree_merge_kernel(AttnTreeArgs a) {
     __shared__ Prefix prefix;
     const int tid = threadIdx.x, b = blockIdx.y;
     const int G = a.n_q / a.n_kv;
@@ -591,37 +591,33 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
     __syncthreads();
     const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
     const int hr = blockIdx.x / (kRows / kMergeRows), r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + (tid & (kMergeRows - 1));
-    const int d0 = (tid / kMergeRows) * 16;
+    const int d0 = (tid / kMergeRows) * 8;
     if (hr >= a.n_kv * q.row_tiles) return;
     const int h = hr / q.row_tiles, tr = (hr - h * q.row_tiles) * kRows + r, node = tr / G, hq = h * G + tr - node * G;
     const int share = share_of(prefix.unit[a.batch], a);
     const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
     const int first = u0 / share, parts = (u0 + q.tiles - 1) / share - first + 1;
     if (node >= q.nodes || parts == 1) return;                // whole: written by the CTA that held all of it
-    uint32_t gate[2][8];
+    float4 g0, g1;
     if (a.gate) {
         const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 g = __ldcs(reinterpret_cast<const float4*>(gp + 4 * i));
-            gate[i / 2][4 * (i & 1)] = __float_as_uint(g.x);
-            gate[i / 2][4 * (i & 1) + 1] = __float_as_uint(g.y);
-            gate[i / 2][4 * (i & 1) + 2] = __float_as_uint(g.z);
-            gate[i / 2][4 * (i & 1) + 3] = __float_as_uint(g.w);
-        }
+        g0 = __ldcs(reinterpret_cast<const float4*>(gp));
+        g1 = __ldcs(reinterpret_cast<const float4*>(gp + 4));
     }
     griddep_wait();
     const size_t slot0 = size_t(first) + prefix.seg[b] + hr;
-    float m = kNoMax, l = 0.f, x[16] = {};
+    float m = kNoMax, l = 0.f, x[8] = {};
     for (int p0 = 0; p0 < parts; p0 += kAhead) {
         float2 ml[kAhead];
-        uint32_t o[kAhead][2][8];
+        uint32_t o[kAhead][8];
 #pragma unroll
         for (int z = 0; z < kAhead; ++z) {
-            const size_t slot = slot0 + min(p0 + z, parts - 1);
-            ml[z] = *reinterpret_cast<const float2*>(a.part_ml + (slot * kRows + r) * 2);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) ld_sector(a.part_o + (slot * (kHeadDim / 8) + d0 / 8 + i) * (kRows * 8) + r * 8, o[z][i]);
+            ml[z] = make_float2(kNoMax, 0.f);
+            if (p0 + z < parts) {
+                const size_t slot = slot0 + p0 + z;
+                ml[z] = *reinterpret_cast<const float2*>(a.part_ml + (slot * kRows + r) * 2);
+                ld_sector(a.part_o + (slot * (kHeadDim / 8) + d0 / 8) * (kRows * 8) + r * 8, o[z]);
+            }
         }
         float mx = m;
 #pragma unroll
@@ -630,23 +626,25 @@ __global__ void __launch_bounds__(256) attn_tree_merge_kernel(AttnTreeArgs a) {
         m = mx;
         l *= back;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] *= back;
+        for (int e = 0; e < 8; ++e) x[e] *= back;
 #pragma unroll
         for (int z = 0; z < kAhead; ++z) {
             if (p0 + z >= parts) break;
             const float w = fast_exp2(ml[z].x - m);
             l = fmaf(ml[z].y, w, l);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = fmaf(__uint_as_float(o[z][e / 8][e & 7]), w, x[e]);
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(__uint_as_float(o[z][e]), w, x[e]);
         }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] *= a.gate ? inv * sigmoid(__uint_as_float(gate[e / 8][e & 7])) : inv;
-    uint32_t w[8];
+    for (int e = 0; e < 8; ++e) x[e] *= a.gate ? inv * sigmoid(g[e]) : inv;
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = a.o_type == 1 ? pack_h2(x[2 * e], x[2 * e + 1]) : pack_b2(x[2 * e], x[2 * e + 1]);
-    st_sector(static_cast<uint16_t*>(a.o) + ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + d0, w);
+    for (int e = 0; e < 4; ++e) w[e] = a.o_type == 1 ? pack_h2(x[2 * e], x[2 * e + 1]) : pack_b2(x[2 * e], x[2 * e + 1]);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + d0) =
+        make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 size_t attn_tree_smem_bytes() { return sizeof(Smem) + 1024; }
@@ -658,7 +656,7 @@ cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
     cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * (kRows / kMergeRows)), unsigned(a.batch));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kMergeThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
