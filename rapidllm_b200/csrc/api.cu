@@ -117,8 +117,7 @@ int dev_info(DevInfo** out) {
                                      int(rl::attn_prefill_smem_bytes())));
         RL_CUDA(cudaFuncSetAttribute(rl::attn_decode_tq_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      int(rl::attn_decode_tq_smem_bytes())));
-        RL_CUDA(cudaFuncSetAttribute(rl::attn_tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     int(rl::attn_tree_smem_bytes())));
+        RL_CUDA(rl::attn_tree_setup());
         RL_CUDA(rl::gdn_tree_setup());
         d.ready = true;
     }

@@ -21,7 +21,10 @@
 // 16 softmax warps in two groups take alternate pages, so that one page's exponentials run under the
 // other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
 // to fp16, as the cache's V is; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
-// its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.
+// its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
+// query for an fp16 output is two such terms, the second from shared memory in the place of a third page of the
+// ring: with one, the scores' rounding would show (4.3e-4 relative instead of 2.9e-4).  A bf16 output's own
+// rounding (1.7e-3) hides it, and one term is faster (16 trees of 21 over 16K: 155 us against 180).
 // Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
 // not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
 // rows past the last node are cleared for the same reason.
@@ -37,7 +40,7 @@ namespace {
 
 constexpr int kRows = 128;                        // MMA rows: (node, query head of the group)
 constexpr int kTile = kPageTokens;
-constexpr int kKStages = 3, kVStages = 3;
+constexpr int kMaxStages = 3;                     // K and V pages in shared memory; 2 where the queries' second term takes the third's place
 constexpr int kSliceBytes = kPageTokens * kHeadDim * 2;
 constexpr int kGroupThreads = 256, kSoftmaxThreads = 512, kThreads = 608;
 constexpr int kWarpLoader = 16, kWarpQK = 17, kWarpPV = 18;
@@ -136,10 +139,12 @@ __device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArg
 }
 
 struct Smem {
-    alignas(1024) unsigned char k[kKStages][kSliceBytes];
-    alignas(1024) unsigned char v[kVStages][kSliceBytes];
+    alignas(1024) unsigned char k[kMaxStages][kSliceBytes];
+    alignas(1024) unsigned char v[kMaxStages][kSliceBytes];
     Prefix prefix;
-    uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+    uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+    // rows of Q's second term, 64 dims per tile of 128 rows x 128 bytes (128-byte swizzle), in the last stage's place
+    __device__ __forceinline__ unsigned char* q_lo(int sub) { return (sub < 2 ? k : v)[kMaxStages - 1] + (sub & 1) * (kRows * 128); }
     uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_m[2], bar_q;
     float xch[2][2][kRows][2];                    // [group][use parity] row maxima of the two column halves
     float mrow[2][kRows];                         // [page parity] running row maximum, in units of S
@@ -213,7 +218,9 @@ __device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const 
 
 }  // namespace
 
+template <bool kTwoTerms>
 __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) {
+    constexpr int kStages = kTwoTerms ? kMaxStages - 1 : kMaxStages;
     extern __shared__ unsigned char smem_raw[];
     // (aligned by an offset, not by integer arithmetic on the pointer: the compiler keeps the loads shared-space ones)
     Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -222,11 +229,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
     griddep_launch();
     if (warp == 0) build_prefix(s.prefix, a, lane, a.err);
     if (tid == 32) {
-        for (int i = 0; i < kKStages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&s.k_full[i], 1);
             mbar_init(&s.k_empty[i], 1);
         }
-        for (int i = 0; i < kVStages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&s.v_full[i], 1);
             mbar_init(&s.v_empty[i], 1);
         }
@@ -284,12 +291,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 for (int j = 0; j < count; ++j, ++it) {
                     const int page = __shfl_sync(0xffffffffu, mine, j);
                     if (lane != 0 || !ok) continue;
-                    const int ks = it % kKStages, vs = it % kVStages;
+                    const int ks = it % kStages, vs = it % kStages;
                     const size_t slice = (size_t(page) * a.n_kv + g.h) * kv_slice_elems();
-                    if (!mbar_wait(&s.k_empty[ks], ((it / kKStages) & 1) ^ 1)) { ok = false; continue; }
+                    if (!mbar_wait(&s.k_empty[ks], ((it / kStages) & 1) ^ 1)) { ok = false; continue; }
                     mbar_arrive_expect_tx(&s.k_full[ks], kSliceBytes);
                     bulk_g2s(s.k[ks], a.k_pool + slice, kSliceBytes, &s.k_full[ks]);
-                    if (!mbar_wait(&s.v_empty[vs], ((it / kVStages) & 1) ^ 1)) { ok = false; continue; }
+                    if (!mbar_wait(&s.v_empty[vs], ((it / kStages) & 1) ^ 1)) { ok = false; continue; }
                     mbar_arrive_expect_tx(&s.v_full[vs], kSliceBytes);
                     bulk_g2s(s.v[vs], a.v_pool + slice, kSliceBytes, &s.v_full[vs]);
                 }
@@ -304,10 +311,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         // ------------------------------ S = Q K^T issuer ------------------------------
         if (lane == 0) {
             constexpr uint32_t idesc_qk = tc::idesc_f16(kRows, kTile, false, false);
-            uint64_t k_desc[kKStages];
+            uint64_t k_desc[kStages];
 #pragma unroll
-            for (int i = 0; i < kKStages; ++i) k_desc[i] = tc::smem_desc(smem_u32(s.k[i]), 16, 1024);
+            for (int i = 0; i < kStages; ++i) k_desc[i] = tc::smem_desc(smem_u32(s.k[i]), 16, 1024);
             const uint32_t q_tmem = tmem + kColQ;
+            uint64_t lo_desc[4] = {};
+            if (kTwoTerms) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lo_desc[i] = tc::smem_desc(smem_u32(s.q_lo(i)), 16, 1024);
+            }
             int b = 0, it = 0, sg = 0;
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok;) {
@@ -317,17 +329,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 ok = mbar_wait(&s.bar_q, sg & 1);
                 ++sg;
                 for (int j = 0; j < g.n_tiles && ok; ++j, ++it) {
-                    const int st = it % kKStages;
-                    if (!mbar_wait(&s.k_full[st], (it / kKStages) & 1)) { ok = false; break; }
+                    const int st = it % kStages;
+                    if (!mbar_wait(&s.k_full[st], (it / kStages) & 1)) { ok = false; break; }
                     // this S buffer held the P of two pages before
                     if (it >= 2 && !mbar_wait(&s.bar_pv[it & 1], ((it - 2) >> 1) & 1)) { ok = false; break; }
                     tc::fence_after_sync();
                     const uint32_t s_tmem = tmem + kColS + (it & 1) * 64;
-                    const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[2]);
+                    const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[kStages - 1]);
 #pragma unroll
-                    for (int kk = 0; kk < 16; ++kk)
-                        tc::mma_ts(s_tmem, q_tmem + kk * 8, kd + uint64_t(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4),
-                                   idesc_qk, kk > 0);
+                    for (int kk = 0; kk < 16; ++kk) {
+                        const uint64_t kd16 = kd + uint64_t(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4);
+                        if (kTwoTerms) tc::mma_ss(s_tmem, lo_desc[kk >> 2] + (kk & 3) * 2, kd16, idesc_qk, kk > 0);
+                        tc::mma_ts(s_tmem, q_tmem + kk * 8, kd16, idesc_qk, kTwoTerms || kk > 0);
+                    }
                     tc::commit(&s.k_empty[st]);
                     tc::commit(&s.bar_s[it & 1]);
                 }
@@ -341,9 +355,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         // ------------------------------ O += P V issuer ------------------------------
         if (lane == 0) {
             constexpr uint32_t idesc_pv = tc::idesc_f16(kRows, kHeadDim, false, true);
-            uint64_t v_desc[kVStages];
+            uint64_t v_desc[kStages];
 #pragma unroll
-            for (int i = 0; i < kVStages; ++i) v_desc[i] = tc::smem_desc(smem_u32(s.v[i]), kTile * 128, 1024);
+            for (int i = 0; i < kStages; ++i) v_desc[i] = tc::smem_desc(smem_u32(s.v[i]), kTile * 128, 1024);
             int b = 0, it = 0;
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok;) {
@@ -351,12 +365,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 pos = g.next;
                 if (!g.n_tiles) continue;
                 for (int j = 0; j < g.n_tiles; ++j, ++it) {
-                    const int st = it % kVStages;
-                    if (!mbar_wait(&s.v_full[st], (it / kVStages) & 1)) { ok = false; break; }
+                    const int st = it % kStages;
+                    if (!mbar_wait(&s.v_full[st], (it / kStages) & 1)) { ok = false; break; }
                     // P of a segment's first page is published after every thread has read the segment before's O
                     if (!mbar_wait(&s.bar_p[it & 1], (it >> 1) & 1)) { ok = false; break; }
                     tc::fence_after_sync();
-                    const uint64_t vd = st == 0 ? v_desc[0] : (st == 1 ? v_desc[1] : v_desc[2]);
+                    const uint64_t vd = st == 0 ? v_desc[0] : (st == 1 ? v_desc[1] : v_desc[kStages - 1]);
                     const uint32_t p_tmem = tmem + kColS + (it & 1) * 64;
                     tc::mma_ts(tmem + kColO, p_tmem, vd, idesc_pv, j > 0);
 #pragma unroll
@@ -415,6 +429,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 uint32_t regs[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) regs[i] = pack_h2(x[2 * i] * f, x[2 * i + 1] * f);
+                if (kTwoTerms) {
+                    unsigned char* row_lo = s.q_lo(quarter) + r * 128;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&regs[i + z]));
+                            w[z] = pack_h2(fmaf(x[2 * (i + z)], f, -hi.x), fmaf(x[2 * (i + z) + 1], f, -hi.y));
+                        }
+                        *reinterpret_cast<uint4*>(row_lo + (((i / 4) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    tc::fence_async_smem();
+                }
                 tc::tmem_st32(lane_addr + kColQ + quarter * 32, regs);
                 tc::tmem_wait_st();
                 tc::fence_before_sync();
@@ -441,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 const int tok0 = (g.j0 + j) * kTile;
                 if (last_pos + 1 - tok0 < kTile) {
                     // V rows past the last node may hold anything (0 * NaN would poison O): clear them
-                    wait(&s.v_full[it % kVStages], (it / kVStages) & 1);
+                    wait(&s.v_full[it % kStages], (it / kStages) & 1);
                     const int first = last_pos + 1 - tok0;
-                    unsigned char* vt = s.v[it % kVStages];
+                    unsigned char* vt = s.v[it % kStages];
                     for (int idx = tid - grp * kGroupThreads; idx < (kTile - first) * 32; idx += kGroupThreads) {
                         const int vr = first + (idx >> 5), c16 = idx & 31;
                         *reinterpret_cast<uint4*>(vt + (c16 >> 3) * (kTile * 128) + vr * 128 + (c16 & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -647,12 +675,22 @@ __global__ void __launch_bounds__(kMergeThreads, 2) attn_tree_merge_kernel(AttnT
         make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-size_t attn_tree_smem_bytes() { return sizeof(Smem) + 1024; }
+namespace {
+constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+}
+
+cudaError_t attn_tree_setup() {
+    cudaError_t e = cudaFuncSetAttribute(attn_tree_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_tree_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes));
+    return e;
+}
 int attn_tree_rows() { return kRows; }
 int attn_tree_max_batch() { return kMaxBatch; }
 
 cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
-    attn_tree_kernel<<<a.grid, kThreads, attn_tree_smem_bytes(), st>>>(a);
+    // fp16 and bf16 queries are exact in one fp16 term
+    if (a.q_type == 0 && a.o_type == 1) attn_tree_kernel<true><<<a.grid, kThreads, kSmemBytes, st>>>(a);
+    else attn_tree_kernel<false><<<a.grid, kThreads, kSmemBytes, st>>>(a);
     cudaLaunchConfig_t cfg = {};
     const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
     cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * (kRows / kMergeRows)), unsigned(a.batch));

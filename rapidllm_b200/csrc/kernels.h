@@ -331,10 +331,9 @@ struct AttnTreeArgs {
     int boundary;                // charge of a (sequence, head, row tile), in pages
     float scale;
 };
-size_t attn_tree_smem_bytes();
+cudaError_t attn_tree_setup();   // kernel attributes, once per device
 int attn_tree_rows();
 int attn_tree_max_batch();
-__global__ void attn_tree_kernel(AttnTreeArgs a);
 cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st);
 
 struct GdnTreeArgs {
