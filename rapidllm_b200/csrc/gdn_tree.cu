@@ -107,6 +107,10 @@ __device__ __forceinline__ int4 conv_sources(int i, const int* parents, int row_
     return make_int4(s[0], s[1], s[2], s[3]);
 }
 
+// Decays along a path are sums of up to 64 logs whose differences are exponentiated: summed in 64 bits, so that one
+// strongly closed gate does not cost the nodes behind it their digits; e^-10000 is 0 as e^-inf is, and has differences.
+__device__ __forceinline__ float log_decay(float g) { return fmaxf(g, -1e4f); }
+
 __device__ __forceinline__ float sum_warp(float v) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
@@ -149,7 +153,8 @@ struct TreeSmem {
         float tri[NB][kPitch];                                // L, inverted in place
         alignas(1024) unsigned char mix[2][NB * 128];         // then: coefficients of u_j in o_i as tiles
     };
-    float decay[NB], grow[NB], beta[NB], in[NB];              // c_i log2 e, e^{c_i}, beta_i, -beta_i e^{c_i} / lift
+    float decay[NB], decay_lo[NB];                            // c_i log2 e in two terms
+    float grow[NB], beta[NB], in[NB];                         // e^{c_i}, beta_i, -beta_i e^{c_i} / lift
     float amax[2][kDv];
     unsigned long long word[kMaxNodes];
     int parents[kMaxNodes];
@@ -415,13 +420,13 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         // ---- decays along the paths ----
         if (warp == 4) {
             const size_t at = size_t(b) * a.max_nodes * a.n_v + h;
-            float c0 = lane < n ? a.g_log[at + size_t(lane) * a.n_v] : 0.f;
-            float c1 = NB > 32 && lane + 32 < n ? a.g_log[at + size_t(lane + 32) * a.n_v] : 0.f;
+            double c0 = lane < n ? log_decay(a.g_log[at + size_t(lane) * a.n_v]) : 0.f;
+            double c1 = NB > 32 && lane + 32 < n ? log_decay(a.g_log[at + size_t(lane + 32) * a.n_v]) : 0.f;
             const float b0 = lane < n ? a.beta[at + size_t(lane) * a.n_v] : 0.f;
             const float b1 = NB > 32 && lane + 32 < n ? a.beta[at + size_t(lane + 32) * a.n_v] : 0.f;
             int j0 = s.parents[lane], j1 = s.parents[lane + 32];
             while (__any_sync(0xffffffffu, j0 >= 0 || j1 >= 0)) {
-                const float x0 = tree::of_node(c0, c1, j0 & 63), x1 = tree::of_node(c0, c1, j1 & 63);
+                const double x0 = tree::of_node(c0, c1, j0 & 63), x1 = tree::of_node(c0, c1, j1 & 63);
                 const int y0 = tree::of_node(j0, j1, j0 & 63), y1 = tree::of_node(j0, j1, j1 & 63);
                 if (j0 >= 0) {
                     c0 += x0;
@@ -436,8 +441,10 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             for (int z = 0; z < 2; ++z) {
                 const int i = lane + 32 * z;
                 if (i >= NB) break;
-                const float c = (z ? c1 : c0) * 1.4426950408889634f, bt = z ? b1 : b0, e = fast_exp2(c);
-                s.decay[i] = c;
+                const double c = (z ? c1 : c0) * 1.4426950408889634;
+                const float bt = z ? b1 : b0, e = fast_exp2(float(c));
+                s.decay[i] = float(c);
+                s.decay_lo[i] = float(c - double(float(c)));
                 s.grow[i] = e;
                 s.beta[i] = bt;
                 s.in[i] = -bt * e * kBack;
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             // this half's columns that count: ancestors, and for o the node itself
             const unsigned long long word = row ? (is_q ? s.word[i] : s.word[i] & ~(1ull << i)) : 0ull;
             const uint32_t on = uint32_t(word >> (grp * kMine));
-            const float ci = row ? s.decay[i] : 0.f;
+            const float ci = row ? s.decay[i] : 0.f, ci_lo = row ? s.decay_lo[i] : 0.f;
             const float f_ = is_q ? kBack * 0.08838834764831845f : (row ? s.beta[i] * kBack * kBack : 0.f);      // 1 / sqrt(128)
 #pragma unroll
             for (int c = 0; c < kMine; c += 8) {
@@ -513,11 +520,11 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                 tc::tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
-                    const float4 d4 = *reinterpret_cast<const float4*>(&s.decay[j0 + e]);
-                    const float cj[4] = {d4.x, d4.y, d4.z, d4.w};
+                    const float4 d4 = *reinterpret_cast<const float4*>(&s.decay[j0 + e]), l4 = *reinterpret_cast<const float4*>(&s.decay_lo[j0 + e]);
+                    const float cj[4] = {d4.x, d4.y, d4.z, d4.w}, cj_lo[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
-                        const float y = fast_exp2(ci - cj[z]) * (f_ * __uint_as_float(g[e + z]));     // no branch: what does not count is dropped
+                        const float y = fast_exp2((ci - cj[z]) + (ci_lo - cj_lo[z])) * (f_ * __uint_as_float(g[e + z]));     // no branch: what does not count is dropped
                         m[c + e + z] = on >> (c + e + z) & 1 ? y : 0.f;
                     }
                 }
@@ -663,14 +670,16 @@ struct CommitSmem {
     float k[kChunk][kDk], v[kChunk][kCommitCols];             // v, then u
     float low[kChunk][kChunk];                                // coefficient of u_j in u_i
     float red[4][kChunk][kCommitCols];                        // S0^T k by row blocks
-    float2 cb[kMaxNodes];                                     // log decay from the state to the path's token; beta
+    double c[kMaxNodes];                                      // log decay from the state to the path's token
+    float beta[kMaxNodes];
 };
-// workspace: path lengths, then the path's nodes [batch][max_nodes], (c, beta) [batch][n_v][max_nodes], k
+// workspace: path lengths, then the path's nodes [batch][max_nodes], c and beta [batch][n_v][max_nodes], k
 // [batch][max_nodes][n_qk][128], v [batch][max_nodes][n_v][128]
 struct CommitWorkspace {
     int* len;
     int* path;
-    float2* cb;
+    double* c;
+    float* beta;
     float *k, *v;
     size_t bytes;
 };
@@ -686,7 +695,8 @@ __host__ __device__ __forceinline__ CommitWorkspace commit_workspace(void* base,
     const size_t rows = size_t(batch) * max_nodes;
     w.len = reinterpret_cast<int*>(take(size_t(batch) * 4));
     w.path = reinterpret_cast<int*>(take(rows * 4));
-    w.cb = reinterpret_cast<float2*>(take(rows * n_v * 8));
+    w.c = reinterpret_cast<double*>(take(rows * n_v * 8));
+    w.beta = reinterpret_cast<float*>(take(rows * n_v * 4));
     w.k = reinterpret_cast<float*>(take(rows * n_qk * kDk * 4));
     w.v = reinterpret_cast<float*>(take(rows * n_v * kDv * 4));
     w.bytes = at;
@@ -754,18 +764,21 @@ __global__ void __launch_bounds__(kPathWarps * 32) gdn_tree_path_kernel(GdnTreeA
         }
     }
     if (is_v) {
-        float carry = 0.f;
+        double carry = 0.0;
         for (int t0 = 0; t0 < len; t0 += 32) {
             const int t = t0 + lane;
             const size_t at = t < len ? (size_t(b) * a.max_nodes + path[t]) * a.n_v + h : 0;
-            float g = t < len ? a.g_log[at] : 0.f;
+            double g = t < len ? log_decay(a.g_log[at]) : 0.f;
             const float bt = t < len ? a.beta[at] : 0.f;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
-                const float up = __shfl_up_sync(0xffffffffu, g, off);
+                const double up = __shfl_up_sync(0xffffffffu, g, off);
                 if (lane >= off) g += up;
             }
-            if (t < len) ws.cb[(size_t(b) * a.n_v + h) * a.max_nodes + t] = make_float2(carry + g, bt);
+            if (t < len) {
+                ws.c[(size_t(b) * a.n_v + h) * a.max_nodes + t] = carry + g;
+                ws.beta[(size_t(b) * a.n_v + h) * a.max_nodes + t] = bt;
+            }
             carry += __shfl_sync(0xffffffffu, g, 31);
         }
     }
@@ -814,7 +827,10 @@ __global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnT
     for (int r = 0; r < 8; ++r) st[r] = __ldcs(reinterpret_cast<const float4*>(Sh + (row0 + r) * kDv + col0));
     griddep_wait();
     const int len = ws.len[b], hs = key_head_of(h, a.n_v, a.n_qk, a.head_map);
-    if (tid < len) s.cb[tid] = ws.cb[(size_t(b) * a.n_v + h) * a.max_nodes + tid];
+    if (tid < len) {
+        s.c[tid] = ws.c[(size_t(b) * a.n_v + h) * a.max_nodes + tid];
+        s.beta[tid] = ws.beta[(size_t(b) * a.n_v + h) * a.max_nodes + tid];
+    }
     for (int t0 = 0; t0 < len; t0 += kChunk) {
         const int m = min(kChunk, len - t0);
         for (int i = warp; i < m; i += kCommitThreads / 32) {
@@ -824,13 +840,13 @@ __global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnT
                 *reinterpret_cast<float4*>(&s.v[i][lane * 4]) = *reinterpret_cast<const float4*>(ws.v + (at * a.n_v + h) * kDv + part0 + lane * 4);
         }
         __syncthreads();
-        const float c_in = t0 ? s.cb[t0 - 1].x : 0.f;         // decays are taken from the chunk's start
+        const double c_in = t0 ? s.c[t0 - 1] : 0.0;           // decays are taken from the chunk's start
         // coefficients: pair (i, j < i) per warp; S0^T k: 8 rows x 4 columns per thread
         for (int p = warp; p < m * (m - 1) / 2; p += kCommitThreads / 32) {
             int i = 1, j = p;
             while (j >= i) j -= i++;
             const float d = sum_warp(dot4(*reinterpret_cast<const float4*>(&s.k[i][lane * 4]), *reinterpret_cast<const float4*>(&s.k[j][lane * 4]), 0.f));
-            if (lane == 0) s.low[i][j] = s.cb[t0 + i].y * expf(s.cb[t0 + i].x - s.cb[t0 + j].x) * d;
+            if (lane == 0) s.low[i][j] = s.beta[t0 + i] * expf(float(s.c[t0 + i] - s.c[t0 + j])) * d;
         }
 #pragma unroll 2
         for (int i = 0; i < m; ++i) {
@@ -856,20 +872,20 @@ __global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnT
         if (tid < kCommitCols) {
             for (int i = 0; i < m; ++i) {
                 const float kv = (s.red[0][i][tid] + s.red[1][i][tid]) + (s.red[2][i][tid] + s.red[3][i][tid]);
-                float r = s.cb[t0 + i].y * (s.v[i][tid] - expf(s.cb[t0 + i].x - c_in) * kv);
+                float r = s.beta[t0 + i] * (s.v[i][tid] - expf(float(s.c[t0 + i] - c_in)) * kv);
                 for (int j = 0; j < i; ++j) r = fmaf(-s.low[i][j], s.v[j][tid], r);
                 s.v[i][tid] = r;
             }
         }
         __syncthreads();
-        const float c_out = s.cb[t0 + m - 1].x;
-        const float e = expf(c_out - c_in);
+        const double c_out = s.c[t0 + m - 1];
+        const float e = expf(float(c_out - c_in));
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             st[r].x *= e; st[r].y *= e; st[r].z *= e; st[r].w *= e;
         }
         for (int i = 0; i < m; ++i) {
-            const float f = expf(c_out - s.cb[t0 + i].x);
+            const float f = expf(float(c_out - s.c[t0 + i]));
             const float4 ka = *reinterpret_cast<const float4*>(&s.k[i][row0]), kb = *reinterpret_cast<const float4*>(&s.k[i][row0 + 4]);
             const float kr[8] = {ka.x, ka.y, ka.z, ka.w, kb.x, kb.y, kb.z, kb.w};
             float4 u4 = *reinterpret_cast<const float4*>(&s.v[i][col0]);

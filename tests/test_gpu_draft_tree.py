@@ -380,6 +380,80 @@ def test_gdn_commit(n_v, n_qk, tiled, nodes, counts, width, ring):
         assert torch.equal(pc.cpu(), phase)
 
 
+def test_gdn_closed_gates_do_not_cost_digits():
+    """Gates that forget everything in between (log decays of -60, -5000 and -inf): the nodes behind them keep the
+    tolerance, in the verify and in the commit."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(77)
+    n_v, n_qk, nodes = 4, 2, 40
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, 2, nodes, n_v, n_qk, 2)
+    g[:, 3::7, 0] = -60.0
+    g[:, 2::9, 1] = -5000.0
+    g[:, 4::11, 2] = -math.inf
+    parents = torch.stack([torch.arange(nodes) - 1, _tree(gen, 1, nodes, 3)[0]]).int()
+    dev = [t.cuda() for t in (S, win)]
+    rest = [t.cuda() for t in (qkv, w, beta, g, parents)]
+    o = ops.gdn_tree(*dev, None, *rest, n_qk).cpu()
+    leaf = torch.tensor([nodes - 1, nodes - 1], dtype=torch.int32)
+    ops.gdn_tree_commit(*dev, None, *rest, leaf.cuda(), n_qk)
+    _lib.check_device()
+    for b in range(2):
+        par = parents[b].tolist()
+        want = torch.stack([_gdn_exact(S[b], win[b], qkv[b], w, beta[b], g[b], _path(par, i), n_v, n_qk, False)[0] for i in range(nodes)])
+        for h in range(n_v):
+            assert rel_l2(o[b, :, h], want[:, h]) <= STATE_REL_L2, (b, h)
+            for i in range(nodes):
+                assert rel_l2(o[b, i, h], want[i, h]) <= 1e-4, (b, h, i)
+        state = _gdn_exact(S[b], win[b], qkv[b], w, beta[b], g[b], _path(par, nodes - 1), n_v, n_qk, False)[1]
+        for h in range(n_v):
+            assert rel_l2(dev[0][b, h].cpu(), state[h]) <= STATE_REL_L2, (b, h)
+
+
+def test_refusals_of_the_wrappers():
+    """Wrong device, type, shape or stride of a tensor is an RlError with the argument's name; nothing is launched."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(4)
+    B, n = 2, 5
+    kp, vp, table, _ = _pages(gen, [10, 70], [n, n], 4, 0.0)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    base, parents, leaf = i32(10, 70), _tree(gen, B, n, 2).cuda(), i32(1, 2)
+    q = torch.zeros(B, n, 24, HD, device="cuda")
+    qg, k = torch.zeros(B, n, 24, 512, device="cuda"), torch.zeros(B, n, 4, HD, device="cuda")
+    S, win, qkv, w, beta, g = (t.cuda() for t in _gdn_inputs(gen, B, n, 6, 2, B))
+    attn = dict(q=q, k_pool=kp, v_pool=vp, page_table=table, base_len=base, parents=parents)
+    app = dict(qg=qg, k=k, v=k, k_pool=kp, v_pool=vp, page_table=table, pos=base, parents=parents)
+    kv = dict(k_pool=kp, v_pool=vp, page_table=table, base_len=base, parents=parents, leaf=leaf)
+    gdn = dict(S=S, conv_window=win, conv_phase=None, qkv=qkv, conv_w=w, beta=beta, g_log=g, parents=parents, n_qk=2)
+    before = kp.clone(), S.clone(), win.clone()
+    for call, good, bad in (
+        (ops.attn_tree, attn, dict(q=q.cpu())), (ops.attn_tree, attn, dict(q=q.double())), (ops.attn_tree, attn, dict(parents=parents.long())),
+        (ops.attn_tree, attn, dict(base_len=None)), (ops.attn_tree, attn, dict(base_len=base[:1])), (ops.attn_tree, attn, dict(page_table=table[:1])),
+        (ops.attn_tree, attn, dict(out=torch.zeros_like(q))), (ops.attn_tree, attn, dict(gate=q.half())), (ops.attn_tree, attn, dict(v_pool=vp[:1])),
+        (ops.attn_tree, attn, dict(gate=torch.zeros(B, n, 24, 2 * HD, device="cuda")[..., ::2])),
+        (ops.attn_tree, attn, dict(q=torch.zeros(B, 65, 24, HD, device="cuda"), parents=None)),
+        (ops.attn_tree, attn, dict(q=torch.zeros(B, n, HD, 24, device="cuda").transpose(2, 3))),
+        (ops.attn_tree, attn, dict(max_seq_len=10 ** 6)), (ops.attn_tree, attn, dict(q=torch.zeros(B, n, 6, HD, device="cuda"))),
+        (ops.attn_qk_append, app, dict(qg=qg[..., :256])), (ops.attn_qk_append, app, dict(k=k[:, :, ::2])), (ops.attn_qk_append, app, dict(v=k.half())),
+        (ops.attn_qk_append, app, dict(qg=torch.zeros(n, B, 24, 512, device="cuda").transpose(0, 1))), (ops.attn_qk_append, app, dict(q_norm=base)),
+        (ops.attn_qk_append, app, dict(q_dtype=torch.float64)), (ops.attn_qk_append, app, dict(rotary_dim=40)),
+        (ops.kv_tree_commit, kv, dict(leaf=leaf.long())), (ops.kv_tree_commit, kv, dict(parents=parents[:1])), (ops.kv_tree_commit, kv, dict(parents=65)),
+        (ops.gdn_tree, gdn, dict(n_qk=3)), (ops.gdn_tree, gdn, dict(S=S.half())), (ops.gdn_tree, gdn, dict(conv_window=win[:1])),
+        (ops.gdn_tree, gdn, dict(S=S[:1], conv_window=win[:1])), (ops.gdn_tree, gdn, dict(beta=beta[:, :, :2])), (ops.gdn_tree, gdn, dict(g_log=None)),
+        (ops.gdn_tree_commit, dict(gdn, leaf=leaf), dict(leaf=None)), (ops.gdn_tree_commit, dict(gdn, leaf=leaf), dict(parents=parents.cpu())),
+        (ops.gdn_tree_commit, dict(gdn, leaf=leaf), dict(slot_ids=i32(0, 1, 1))),
+    ):
+        with pytest.raises(_lib.RlError):
+            call(**{**good, **bad})
+    torch.cuda.synchronize()
+    assert _lib.device_error() == 0
+    for t, was in zip((kp, S, win), before):
+        assert torch.equal(t, was)
+    # a workspace that is large enough is used, one that is not is replaced
+    want = ops.gdn_tree(**gdn)
+    for size in (16, 1 << 24):
+        assert torch.equal(ops.gdn_tree(**gdn, workspace=torch.empty(size, dtype=torch.uint8, device="cuda")), want)
+
+
 def test_bad_trees_are_recorded_and_skipped():
     """A parent that is not in [-1, i) counts as a root, a bad count as an empty draft, a bad leaf as none."""
     from rapidllm_b200 import _lib, ops
