@@ -10,7 +10,6 @@
 // so no node needs a state of its own: 64 KiB per value head are read once, whatever the tree.
 #include "common.cuh"
 #include "kernels.h"
-#include "launch.cuh"
 #include "tcgen05.cuh"
 #include "tree.cuh"
 
