@@ -620,12 +620,18 @@ __global__ void __launch_bounds__(kMergeThreads, 2) attn_tree_merge_kernel(AttnT
     const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
     const int hr = blockIdx.x / (kRows / kMergeRows), r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + (tid & (kMergeRows - 1));
     const int d0 = (tid / kMergeRows) * 8;
-    if (hr >= a.n_kv * q.row_tiles) return;
+    if (hr >= a.n_kv * q.row_tiles) {
+        griddep_wait();                                       // on every path: what follows this kernel follows the one in front too
+        return;
+    }
     const int h = hr / q.row_tiles, tr = (hr - h * q.row_tiles) * kRows + r, node = tr / G, hq = h * G + tr - node * G;
     const int share = share_of(prefix.unit[a.batch], a);
     const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
     const int first = u0 / share, parts = (u0 + q.tiles - 1) / share - first + 1;
-    if (node >= q.nodes || parts == 1) return;                // whole: written by the CTA that held all of it
+    if (node >= q.nodes || parts == 1) {                      // whole: written by the CTA that held all of it
+        griddep_wait();
+        return;
+    }
     float4 g0, g1;
     if (a.gate) {
         const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0;

@@ -340,11 +340,11 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     const int v = tid & (kDv - 1);                            // column of the state = TMEM lane
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
     const int n = tree::node_count(a.n_nodes, b, a.max_nodes, a.err);
-    if (slot < 0 || slot >= a.n_slots) {
-        if (tid == 0) set_err(a.err, DEV_ERR_BAD_SLOT);
+    if (slot < 0 || slot >= a.n_slots || n == 0) {
+        if (tid == 0 && n) set_err(a.err, DEV_ERR_BAD_SLOT);
+        griddep_wait();                                       // on every path: what follows this kernel follows the one in front too
         return;
     }
-    if (n == 0) return;
     const int ratio = a.n_v / a.n_qk;
     const int h0 = a.heads == 1 ? int(blockIdx.x) : (a.head_map == 1 ? int(blockIdx.x) * ratio : int(blockIdx.x));
     const int h_step = a.head_map == 1 ? 1 : a.n_qk;
@@ -797,7 +797,10 @@ __global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnT
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
-    if (slot < 0 || slot >= a.n_slots || a.leaf[b] < 0 || a.leaf[b] >= a.max_nodes) return;
+    if (slot < 0 || slot >= a.n_slots || a.leaf[b] < 0 || a.leaf[b] >= a.max_nodes) {
+        griddep_wait();                                       // on every path: what follows this kernel follows the one in front too
+        return;
+    }
     if (int(blockIdx.x) >= kParts * a.n_v) {
         const int c = (blockIdx.x - kParts * a.n_v) * kCommitThreads + tid;
         griddep_wait();
