@@ -652,3 +652,58 @@ def test_a_tree_through_the_mixers_equals_decode_along_each_path():
         want = decode(nxt.cuda(), [base[0] + ends[0][1], base[1] + ends[1][1]], None)[b].cpu()
         assert (got[b] - want).abs().max() <= ATTN_MAX_ABS and rel_l2(got[b], want) <= ATTN_REL_L2
     del committed
+
+
+def test_chains_without_parents():
+    """parents None (a number of nodes for the KV commit) is the tree whose every node continues the one before."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(31)
+    B, n = 2, 9
+    chain = (torch.arange(n) - 1).int().expand(B, n).contiguous().cuda()
+    base = torch.tensor([61, 200], dtype=torch.int32, device="cuda")
+    counts, leaf = torch.tensor([9, 4], dtype=torch.int32, device="cuda"), torch.tensor([8, 2], dtype=torch.int32, device="cuda")
+    results = []
+    for parents in (chain, None):
+        gen.manual_seed(31)
+        kp, vp, table, _ = _pages(gen, [61, 200], [n, n], 4, 0.0)
+        S, win, qkv, w, beta, g = (t.cuda() for t in _gdn_inputs(gen, B, n, 6, 2, B))
+        qg, k, v = (torch.randn(B, n, h, d, generator=gen).cuda() for h, d in ((24, 512), (4, HD), (4, HD)))
+        out = torch.zeros(B, n, 24, HD, dtype=torch.float16, device="cuda")
+        o = torch.zeros(B, n, 6, DK, device="cuda")
+        q, gate = ops.attn_qk_append(qg, k, v, kp, vp, table, base, parents=parents, q_dtype=torch.float16)
+        ops.attn_tree(q, kp, vp, table, base, parents, n_nodes=counts, gate=gate, out=out)
+        ops.gdn_tree(S, win, None, qkv, w, beta, g, parents, 2, n_nodes=counts, out=o)
+        ops.gdn_tree_commit(S, win, None, qkv, w, beta, g, parents, leaf, 2)
+        taken = ops.kv_tree_commit(kp, vp, table, base, n if parents is None else parents, leaf)
+        _lib.check_device()
+        assert taken.tolist() == [9, 3]
+        results.append((q, gate, kp, vp, out, o, S, win))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_pages_far_into_a_large_pool():
+    """Pages whose offset in the pool passes 2^32 bytes and 2^31 values."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(32)
+    n, base, n_pages = 12, 130, 33000
+    kp, vp = ops.new_pool(n_pages, 4), ops.new_pool(n_pages, 4)
+    table = torch.tensor([[n_pages - 1, 5, n_pages - 7]], dtype=torch.int32, device="cuda")
+    rows = [torch.randn(base + n, 4, HD, generator=gen).half() for _ in range(2)]
+    ops.kv_append(kp, vp, table[0], rows[0][:base].cuda(), rows[1][:base].cuda(), pos0=0)
+    parents = _tree(gen, 1, n, 3)
+    at = torch.tensor([base], dtype=torch.int32, device="cuda")
+    qg = torch.randn(1, n, 24, 512, generator=gen)
+    k, v = (r[base:].float().unsqueeze(0).cuda() for r in rows)
+    q, _ = ops.attn_qk_append(qg.cuda(), k, v, kp, vp, table, at, parents=parents.cuda(), rotary_dim=0, q_dtype=torch.float16, want_gate=False)
+    rows[0][base:] = torch.stack([_pool_row(kp, table, 0, base + i) for i in range(n)]).cpu()
+    assert torch.equal(torch.stack([_pool_row(vp, table, 0, base + i) for i in range(n)]).cpu(), rows[1][base:])
+    got = ops.attn_tree(q, kp, vp, table, at, parents.cuda())
+    o, _, _ = _attn_exact(q[0].cpu(), None, rows, base, parents[0].tolist(), n, 24, 4)
+    assert rel_l2(got[0].float().cpu(), o) <= 1e-3
+    path = _path(parents[0].tolist(), n - 1)
+    ops.kv_tree_commit(kp, vp, table, at, parents.cuda(), torch.tensor([n - 1], dtype=torch.int32, device="cuda"))
+    _lib.check_device()
+    for j, i in enumerate(path):
+        assert torch.equal(_pool_row(kp, table, 0, base + j).cpu(), rows[0][base + i])
+        assert torch.equal(_pool_row(vp, table, 0, base + j).cpu(), rows[1][base + i])
