@@ -459,7 +459,7 @@ typedef struct rl_attn_tree_params {
     int n_q, n_kv, head_dim;     /* 24, 4, 256; n_q / n_kv <= 8 */
     int batch, max_nodes;        /* sequences, rows per sequence in q and o (<= 64) */
     int page_tokens, n_pages, max_pages_per_seq;
-    int max_seq_len;             /* host-side upper bound of every base_len[b] + n_nodes[b] (sizing only) */
+    int max_seq_len;             /* host-side upper bound of every base_len[b] + n_nodes[b] */
     int q_type;                  /* RL_TYPE_* of q */
     int o_type;                  /* RL_TYPE_F16 or RL_TYPE_BF16 */
     long long gate_row, gate_head;   /* floats between the gate's rows and heads (0 = dense), multiples of 4 */
@@ -475,8 +475,10 @@ size_t rl_attn_tree_workspace_bytes(const rl_attn_tree_params* p);
  *     q, o and workspace 32-byte aligned
  *   o [batch][max_nodes][n_q][256] in 16 bits: a mean of fp16 values times a gate in (0, 1), it fits fp16,
  *     and the probabilities meet V as fp16, so 32 bits would carry no more
- * The V rows of all nodes of a sequence must be finite (one that is not reaches its siblings too); K rows
- * may hold anything where they are not visible.  Reads only the F16 cache (RL_KV_F16). */
+ * What a row does not see has no part in it, whatever it holds; a drafted V row that is not finite makes the
+ * whole output row of the nodes and heads that see it NaN.  A sequence longer than max_seq_len is recorded
+ * (rl_device_error) and left out.  Calls that may overlap need workspaces of their own.  Reads only the F16
+ * cache (RL_KV_F16). */
 int rl_attn_tree(const void* k_pool, const void* v_pool, const int32_t* page_table, const int32_t* base_len,
                  const int32_t* parents, const int32_t* n_nodes, const void* q, const float* gate, void* o,
                  void* workspace, size_t workspace_bytes, const rl_attn_tree_params* p, void* stream);

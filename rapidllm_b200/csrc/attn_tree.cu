@@ -27,7 +27,8 @@
 // rounding (1.7e-3) hides it, and one term is faster (16 trees of 21 over 16K: 155 us against 180).
 // Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
 // not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
-// rows past the last node are cleared for the same reason.
+// rows past the last node are cleared for the same reason.  A drafted V row that is not finite would reach the
+// node's siblings as 0 * inf: it is cleared too, and the rows that see it get NaN through their sum.
 #include "common.cuh"
 #include "kernels.h"
 #include "launch.cuh"
@@ -148,6 +149,7 @@ struct Smem {
     uint64_t bar_s[2], bar_p[2], bar_pv[2], bar_m[2], bar_q;
     float xch[2][2][kRows][2];                    // [group][use parity] row maxima of the two column halves
     float mrow[2][kRows];                         // [page parity] running row maximum, in units of S
+    alignas(8) unsigned char v_bad[2][8];         // [group][warp] drafted V rows of its page that are not finite
     alignas(16) float part[kRows][4];             // per row: the four threads' query maxima, later their sums
     uint32_t tmem_base;
     int failed;
@@ -196,6 +198,8 @@ __device__ __forceinline__ void load_q(float (&x)[64], const void* q, int q_type
         }
     }
 }
+// an infinity or a NaN in a pair of fp16
+__device__ __forceinline__ bool has_special(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
 // 32 outputs, gated, rounded to o_type
 __device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const float* gate, float (&o)[32]) {
     if (gate) {
@@ -467,19 +471,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     tc::tmem_wait_ld();
                 }
                 const int tok0 = (g.j0 + j) * kTile;
-                if (last_pos + 1 - tok0 < kTile) {
-                    // V rows past the last node may hold anything (0 * NaN would poison O): clear them
+                const bool drafted = tok0 + kTile > g.base;   // rows behind the committed ones
+                const int first = max(g.base - tok0, 0);
+                if (drafted) {
+                    // each warp clears its share of the V rows past the last node, and of the drafted ones that are not finite
                     wait(&s.v_full[it % kStages], (it / kStages) & 1);
-                    const int first = last_pos + 1 - tok0;
-                    unsigned char* vt = s.v[it % kStages];
-                    for (int idx = tid - grp * kGroupThreads; idx < (kTile - first) * 32; idx += kGroupThreads) {
-                        const int vr = first + (idx >> 5), c16 = idx & 31;
-                        *reinterpret_cast<uint4*>(vt + (c16 >> 3) * (kTile * 128) + vr * 128 + (c16 & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    const int end = last_pos + 1 - tok0;
+                    uint32_t found = 0;
+                    for (int vr = first + (warp & 7), bit = 1; vr < kTile; vr += 8, bit <<= 1) {
+                        uint4* at = reinterpret_cast<uint4*>(s.v[it % kStages] + (lane >> 3) * (kTile * 128) + vr * 128 + (lane & 7) * 16);
+                        bool clear = vr >= end;
+                        if (!clear) {
+                            const uint4 x = *at;
+                            clear = __any_sync(0xffffffffu, has_special(x.x) || has_special(x.y) || has_special(x.z) || has_special(x.w));
+                            if (clear) found |= bit;
+                        }
+                        if (clear) *at = make_uint4(0, 0, 0, 0);
                     }
+                    if (lane == 0) s.v_bad[grp][warp & 7] = static_cast<unsigned char>(found);
                     tc::fence_async_smem();
                 }
                 float mx = kNoMax;
-                if (tok0 + kTile > g.base) {
+                if (drafted) {
                     // bit i of `vis`: token tok0 + 32 half + i is committed, or a node that this row sees
                     const int rel = tok0 + half * 32 - g.base;
                     uint32_t vis;
@@ -548,6 +561,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     ph[i] = pack_h2(p0, p1);
                 }
                 l_part += lsum0 + lsum1;
+                if (drafted) {
+                    named_bar_sync(10 + grp, kGroupThreads);
+                    if (unsigned long long bad = *reinterpret_cast<const unsigned long long*>(s.v_bad[grp])) {
+                        for (; bad; bad &= bad - 1) {         // bit 8 w + z: row first + w + 8 z
+                            const int bit = __ffsll(bad) - 1, rel = tok0 + first + (bit >> 3) + 8 * (bit & 7) - g.base;
+                            if (seen >> rel & 1) l_part = __uint_as_float(0x7fc00000u);
+                        }
+                    }
+                }
                 if (ok) {                                     // both halves' scores left the buffer before the maxima met
                     tc::tmem_st16(lane_addr + kColS + grp * 64 + half * 16, ph);
                     tc::tmem_wait_st();

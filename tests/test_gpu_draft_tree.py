@@ -707,3 +707,31 @@ def test_pages_far_into_a_large_pool():
     for j, i in enumerate(path):
         assert torch.equal(_pool_row(kp, table, 0, base + j).cpu(), rows[0][base + i])
         assert torch.equal(_pool_row(vp, table, 0, base + j).cpu(), rows[1][base + i])
+
+
+@pytest.mark.parametrize("base,q_type", [([40, 3], torch.float16), ([6000, 64], torch.float32)])
+def test_attn_tree_bad_rows_stay_with_their_descendants(base, q_type):
+    """K, V or a query that is not finite: NaN in the rows that see it, nothing else changes by a bit (what a row does not
+    see has weight 0 and is replaced by 0 before the product)."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(33)
+    B, n = 2, 40
+    kp, vp, table, _ = _pages(gen, base, [n, n], 4, float("nan"))
+    parents = _tree(gen, B, n, 6)
+    q = torch.randn(B, n, 24, HD, generator=gen).to(q_type)
+    at = torch.tensor(base, dtype=torch.int32, device="cuda")
+    clean = ops.attn_tree(q.cuda(), kp, vp, table, at, parents.cuda())
+    hit = torch.zeros(B, n, 4, dtype=torch.bool)
+    for b, pool, node, head, value in ((0, vp, 4, 1, math.inf), (0, vp, 25, 3, math.nan), (0, kp, 11, 0, math.nan), (1, vp, 30, 2, -math.inf)):
+        page, row = int(table[b, (base[b] + node) // 64]), (base[b] + node) % 64
+        pool[page, head, int(ops.kv_slice_index(torch.tensor(row), torch.tensor(77)))] = value
+        for i in range(n):
+            hit[b, i, head] |= node in _path(parents[b].tolist(), i)
+    q[1, 7, 20, 200] = math.nan
+    got = ops.attn_tree(q.cuda(), kp, vp, table, at, parents.cuda())
+    _lib.check_device()
+    rows = hit.repeat_interleave(6, 2)
+    rows[1, 7, 20] = True
+    assert rows.any() and not rows.all()
+    assert torch.isnan(got.cpu()[rows]).all()
+    assert torch.equal(got.cpu()[~rows], clean.cpu()[~rows])
