@@ -511,9 +511,11 @@ typedef struct rl_gdn_tree_params {
  *               shifted windows, oldest tap first (rl_conv1d_update's state)
  *   qkv fp32 [batch][max_nodes] rows of conv_dim channels;  beta, g_log fp32 [batch][max_nodes][n_v]
  *   o   fp32 [batch][max_nodes][n_v][128]
- * beta in [0, 2] and g_log <= 0 as the gates give them (the coefficients between nodes are held in a fixed range);
- * inputs of all nodes finite (what is not reaches the node's siblings).  workspace: rl_gdn_tree_workspace_bytes()
- * bytes, 16-byte aligned, for the rows after the conv. */
+ * beta in [0, 2] and g_log <= 0 as the gates give them (the coefficients between nodes are held in a fixed range).
+ * Inputs of a node that are not finite (g_log = -inf is a closed gate) reach its descendants alone.  The nodes'
+ * values share a scale per column: one 2^k above its siblings' leaves those k fewer than 22 bits.
+ * workspace: rl_gdn_tree_workspace_bytes() bytes, 16-byte aligned, for the rows after the conv; calls that may
+ * overlap need workspaces of their own. */
 size_t rl_gdn_tree_workspace_bytes(const rl_gdn_tree_params* p);
 int rl_gdn_tree(const float* S, const float* conv_window, const int32_t* conv_phase, const int32_t* slot_ids,
                 const int32_t* parents, const int32_t* n_nodes, const float* qkv, const float* conv_w,

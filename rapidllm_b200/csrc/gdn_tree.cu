@@ -82,12 +82,6 @@ __device__ __forceinline__ void conv_nodes(const Conv4& cv, const float* x, cons
         y[m] = make_float4(silu(a[0]), silu(a[1]), silu(a[2]), silu(a[3]));
     }
 }
-__device__ __forceinline__ float4 conv_node(const Conv4& cv, const float* x, int4 src) {
-    const int4 s[1] = {src};
-    float4 y[1];
-    conv_nodes(cv, x, s, y);
-    return y[0];
-}
 
 // taps of a node: itself and its next three ancestors, then the window from its newest entry (3) down
 __device__ __forceinline__ int4 conv_sources(int i, const int* parents, int row_stride) {
@@ -107,8 +101,8 @@ __device__ __forceinline__ int4 conv_sources(int i, const int* parents, int row_
 }
 
 // Decays along a path are sums of up to 64 logs whose differences are exponentiated: summed in 64 bits, so that one
-// strongly closed gate does not cost the nodes behind it their digits; e^-10000 is 0 as e^-inf is, and has differences.
-__device__ __forceinline__ float log_decay(float g) { return fmaxf(g, -1e4f); }
+// strongly closed gate does not cost the nodes behind it their digits; e^-10000 is 0 as e^-inf is, and has differences.  NaN stays NaN.
+__device__ __forceinline__ float log_decay(float g) { return g < -1e4f ? -1e4f : g; }
 
 __device__ __forceinline__ float sum_warp(float v) {
 #pragma unroll
@@ -129,6 +123,12 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
     const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = pack_h2(x0 - f.x, x1 - f.y);
+}
+// the larger one, NaN if either is
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+    return m;
 }
 // the power of two that brings a largest magnitude mx into [2^14, 2^15), and its inverse
 __device__ __forceinline__ float lift(float mx, float& back) {
@@ -156,6 +156,8 @@ struct TreeSmem {
     float grow[NB], beta[NB], in[NB];                         // e^{c_i}, beta_i, -beta_i e^{c_i} / lift
     float amax[2][kDv];
     unsigned long long word[kMaxNodes];
+    uint32_t bad[2][kDv];                                     // [half of the nodes][column]: W, U that are not finite, a bit each
+    uint32_t hole[2][kDv];                                    // [half of the columns][row]: [k; q] k^T that are not finite
     int parents[kMaxNodes];
     uint64_t bar_rows, bar_gram, bar_half, bar_in, bar_u, bar_out;
     uint32_t tmem_base;
@@ -323,6 +325,10 @@ __global__ void __launch_bounds__(kPrepWarps * 32, 6) gdn_tree_rows_kernel(GdnTr
 // T is formed in fp32 (16 x 16 blocks by substitution, then joined): n^3 / 6 products once instead of n^2 / 2
 // for each of the 128 columns, and no thread walks 64 dependent steps.  Its entries are k_i^T (a product of
 // contractions) k_j beta, at most max beta in magnitude, so a fixed scale serves them.
+//
+// A node whose inputs are not finite would reach its siblings as 0 * inf through T and U.  Its row of W shows it,
+// whichever input it was (k by S0^T k, gates by e^c): that entry of W is replaced by 0, the coefficients that are NaN
+// too, and the outputs of the column at the node and its descendants become NaN at the end.  A bad q stays in its row.
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     using Smem = TreeSmem<NB>;
@@ -333,8 +339,6 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
     constexpr uint32_t kColA = 0, kColD = 64, kColG = 64 + 2 * NB;
     constexpr uint32_t kCols = 64 + 3 * NB <= 128 ? 128 : 256;
     constexpr int kMine = NB / 2;                             // nodes of a thread's group
-    constexpr int kConv = NB <= 16 ? 2 : 4;                   // nodes a warp has in flight
-    constexpr int kWarps = kThreads / 32;
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int grp = warp >> 2;                                // which half of the state's dims, of the nodes
     const int v = tid & (kDv - 1);                            // column of the state = TMEM lane
@@ -419,10 +423,12 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
         // ---- decays along the paths ----
         if (warp == 4) {
             const size_t at = size_t(b) * a.max_nodes * a.n_v + h;
-            double c0 = lane < n ? log_decay(a.g_log[at + size_t(lane) * a.n_v]) : 0.f;
-            double c1 = NB > 32 && lane + 32 < n ? log_decay(a.g_log[at + size_t(lane + 32) * a.n_v]) : 0.f;
+            const float g0 = lane < n ? a.g_log[at + size_t(lane) * a.n_v] : 0.f;
+            const float g1 = NB > 32 && lane + 32 < n ? a.g_log[at + size_t(lane + 32) * a.n_v] : 0.f;
             const float b0 = lane < n ? a.beta[at + size_t(lane) * a.n_v] : 0.f;
             const float b1 = NB > 32 && lane + 32 < n ? a.beta[at + size_t(lane + 32) * a.n_v] : 0.f;
+            const bool bad0 = !(g0 < INFINITY) || !(fabsf(b0) < INFINITY), bad1 = !(g1 < INFINITY) || !(fabsf(b1) < INFINITY);
+            double c0 = bad0 ? 0.f : log_decay(g0), c1 = bad1 ? 0.f : log_decay(g1);
             int j0 = s.parents[lane], j1 = s.parents[lane + 32];
             while (__any_sync(0xffffffffu, j0 >= 0 || j1 >= 0)) {
                 const double x0 = tree::of_node(c0, c1, j0 & 63), x1 = tree::of_node(c0, c1, j1 & 63);
@@ -441,12 +447,13 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                 const int i = lane + 32 * z;
                 if (i >= NB) break;
                 const double c = (z ? c1 : c0) * 1.4426950408889634;
-                const float bt = z ? b1 : b0, e = fast_exp2(float(c));
+                const bool bad = z ? bad1 : bad0;             // NaN in W alone
+                const float bt = bad ? 0.f : (z ? b1 : b0), e = fast_exp2(float(c));
                 s.decay[i] = float(c);
                 s.decay_lo[i] = float(c - double(float(c)));
                 s.grow[i] = e;
                 s.beta[i] = bt;
-                s.in[i] = -bt * e * kBack;
+                s.in[i] = bad ? __uint_as_float(0x7fc00000u) : -bt * e * kBack;
             }
         }
         // ---- the state's column -> A, 64 dims at a time ----
@@ -508,7 +515,22 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
             const bool row = v < 2 * NB && i < n;
             // this half's columns that count: ancestors, and for o the node itself
             const unsigned long long word = row ? (is_q ? s.word[i] : s.word[i] & ~(1ull << i)) : 0ull;
-            const uint32_t on = uint32_t(word >> (grp * kMine));
+            uint32_t on = uint32_t(word >> (grp * kMine));
+            if (hi == 0) {
+                uint32_t hole = 0;
+#pragma unroll
+                for (int c = 0; c < kMine; c += 8) {
+                    uint32_t g[8];
+                    tc::tmem_ld8(lanes + kColG + grp * kMine + c, g);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hole |= uint32_t(!(fabsf(__uint_as_float(g[e])) < INFINITY)) << (c + e);
+                }
+                s.hole[grp][v] = hole;                        // read by this thread alone
+                on &= ~hole;
+            } else {
+                on &= ~s.hole[grp][v];
+            }
             const float ci = row ? s.decay[i] : 0.f, ci_lo = row ? s.decay_lo[i] : 0.f;
             const float f_ = is_q ? kBack * 0.08838834764831845f : (row ? s.beta[i] * kBack * kBack : 0.f);      // 1 / sqrt(128)
 #pragma unroll
@@ -566,10 +588,23 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                 u[c + e] = fmaf(__uint_as_float(d[e]) * back, s.in[grp * kMine + c + e], u[c + e] * s.beta[grp * kMine + c + e]);
         }
         // column v of W or U, both halves' largest magnitude scaled into place -> A; returns the scale's inverse
+        uint32_t bad = 0;
         auto store_column = [&]() {
             float mx = 0.f;
 #pragma unroll
-            for (int e = 0; e < kMine; ++e) mx = fmaxf(mx, fabsf(u[e]));
+            for (int e = 0; e < kMine; ++e) mx = max_or_nan(mx, fabsf(u[e]));
+            if (!(mx < INFINITY)) {
+                mx = 0.f;
+#pragma unroll
+                for (int e = 0; e < kMine; ++e) {
+                    if (!(fabsf(u[e]) < INFINITY)) {
+                        bad |= 1u << e;
+                        u[e] = 0.f;
+                    }
+                    mx = fmaxf(mx, fabsf(u[e]));
+                }
+            }
+            s.bad[grp][v] = bad;
             s.amax[grp][v] = mx;
             __syncthreads();
             float bk;
@@ -647,6 +682,11 @@ __global__ void __launch_bounds__(kThreads, 2) gdn_tree_kernel(GdnTreeArgs a) {
                 if (ok && i0 + e < n)
                     __stcs(o + size_t(i0 + e) * a.n_v * kDv,
                            fmaf(__uint_as_float(dq[e]) * qs, s.grow[i0 + e], __uint_as_float(du[e]) * uback));
+        }
+        if (const unsigned long long hit = s.bad[0][v] | (unsigned long long)s.bad[1][v] << kMine; hit && ok) {
+#pragma unroll 1
+            for (int i = grp * kMine; i < min(n, (grp + 1) * kMine); ++i)
+                if (s.word[i] & hit) o[size_t(i) * a.n_v * kDv] = __uint_as_float(0x7fc00000u);
         }
         tc::fence_before_sync();
         __syncthreads();                                      // D, A and the head's tables may be rewritten
@@ -787,7 +827,7 @@ __global__ void __launch_bounds__(kPathWarps * 32) gdn_tree_path_kernel(GdnTreeA
 // x < 2 n_v: 64 columns of one value head's state, in registers: warp w holds rows 32 (w / 2) .. and columns 32 (w % 2)
 // .., a lane 8 rows x 4 columns, requested before the wait for the path kernel (only this kernel writes states).  Four
 // such CTAs fit an SM, so that one's exchanges run under the others' loads and stores (two CTAs of 128 columns: 75
-// against 64 us).  Up to 16 tokens at a time in the closed form above.
+// against 68 us).  Up to 16 tokens at a time in the closed form above.
 // The other blocks, a thread per channel: entry w (oldest first) of the new conv window is input len + w of the old
 // window followed by the path's rows.  The ring keeps its phase: rewriting the four taps of a channel is one 16-byte
 // store either way, and a phase that every block reads could only be advanced by another launch.

@@ -735,3 +735,69 @@ def test_attn_tree_bad_rows_stay_with_their_descendants(base, q_type):
     assert rows.any() and not rows.all()
     assert torch.isnan(got.cpu()[rows]).all()
     assert torch.equal(got.cpu()[~rows], clean.cpu()[~rows])
+
+
+@pytest.mark.parametrize("n_v,n_qk,nodes", [(4, 2, 14), (6, 2, 30), (3, 3, 64)])
+def test_gdn_tree_bad_nodes_stay_with_their_descendants(n_v, n_qk, nodes):
+    """Projections and gates that are not finite: the outputs that the formula makes so are not finite, all others keep
+    their tolerance."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(34)
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, 2, nodes, n_v, n_qk, 2)
+    parents = _tree(gen, 2, nodes, 6)
+    qkv[0, 5, 3] = math.inf                                   # q of head 0
+    qkv[0, 7, n_qk * DK + DK + 9] = math.nan                  # k of head 1
+    qkv[1, 6, 2 * n_qk * DK + 2 * DK + 50] = math.nan         # v of head 2, one column
+    qkv[1, nodes - 2, 2 * n_qk * DK + 100] = -math.inf
+    beta[1, 9, 0] = math.nan
+    g[1, 8, 1] = math.inf
+    g[1, 4, 1] = -math.inf                                    # a closed gate
+    o = ops.gdn_tree(S.cuda(), win.cuda(), None, *(t.cuda() for t in (qkv, w, beta, g, parents)), n_qk).cpu()
+    _lib.check_device()
+    for b in range(2):
+        par = parents[b].tolist()
+        want = torch.stack([_gdn_exact(S[b], win[b], qkv[b], w, beta[b], g[b], _path(par, i), n_v, n_qk, False)[0] for i in range(nodes)])
+        fine = torch.isfinite(want)
+        assert not fine.all() and fine.double().mean() > 0.3
+        assert torch.equal(torch.isfinite(o[b]), fine)
+        for h in range(n_v):
+            assert rel_l2(o[b, :, h][fine[:, h]], want[:, h][fine[:, h]]) <= STATE_REL_L2, (b, h)
+
+
+def test_gdn_commit_of_paths_with_bad_nodes():
+    """Nodes off the path leave no trace, whatever they hold; on the path they spoil what the formula says and no more."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(35)
+    B, n_v, n_qk, nodes = 2, 6, 2, 20
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, B, nodes, n_v, n_qk, B)
+    parents = torch.full((B, nodes), -1, dtype=torch.int32)
+    parents[:, 2::2] = torch.arange(0, nodes - 2, 2)           # two chains: even and odd nodes
+    parents[:, 3::2] = torch.arange(1, nodes - 2, 2)
+    leaf = torch.tensor([nodes - 2, nodes - 1], dtype=torch.int32)
+
+    def run(qkv, beta, g):
+        dev = [t.cuda() for t in (S, win)]
+        ops.gdn_tree_commit(*dev, None, *(t.cuda() for t in (qkv, w, beta, g, parents, leaf)), n_qk)
+        _lib.check_device()
+        return [t.cpu() for t in dev]
+
+    clean = run(qkv, beta, g)
+    bad = [t.clone() for t in (qkv, beta, g)]
+    bad[0][:, 5], bad[1][:, 7], bad[2][:, 9] = math.nan, math.inf, math.nan         # on the second sequence's path
+    got = run(*bad)
+    assert torch.equal(got[0][0], clean[0][0]) and torch.equal(got[1][0], clean[1][0])
+    assert not torch.isfinite(got[0][1]).any()
+    one = [t.clone() for t in (qkv, beta, g)]
+    one[0][1, 15, n_qk * DK + DK + 4] = math.inf              # k of head 1: value heads 3, 4, 5
+    one[0][1, 11, 2 * n_qk * DK + 7] = math.nan               # a column of value head 0
+    one[1][1, 13, 1] = math.nan
+    one[2][0, 8, 2] = math.nan
+    got = run(*one)
+    for b in range(B):
+        path = _path(parents[b].tolist(), int(leaf[b]))
+        _, state, window = _gdn_exact(S[b], win[b], one[0][b], w, one[1][b], one[2][b], path, n_v, n_qk, False)
+        fine = torch.isfinite(state)
+        assert fine.any() and not fine.all()
+        assert torch.equal(torch.isfinite(got[0][b]), fine)
+        assert rel_l2(got[0][b][fine], state[fine]) <= STATE_REL_L2
+        assert torch.equal(got[1][b].isnan(), window.isnan())
