@@ -987,7 +987,7 @@ cudaError_t gdn_tree_setup() {
 
 cudaError_t launch_gdn_tree(GdnTreeArgs a, int sms, cudaStream_t st) {
     // one CTA per value head while that leaves SMs without a second CTA; else a key head's value heads share its rows
-    // and their products (16 trees of 21: 47.5 us shared, 48.9 not; 32 chains of 64: 156 and 159)
+    // and their products (16 trees of 21: 49.8 us shared, 51.3 not; 32 chains of 64: 161.6 and 169.8; one of 8: 26.0 and 15.1)
     a.heads = a.batch * a.n_v <= 2 * sms ? 1 : a.n_v / a.n_qk;
     switch (rounded_nodes(a.max_nodes)) {
         case 16: return launch<16>(a, st);
