@@ -630,49 +630,55 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
 }
 
 // Rows whose pages were divided: log-sum-exp over the row's slots (log2 domain), gate, rounding.  A block takes 16
-// rows of a row tile, a thread 8 dims of one row (lane = row: 32 bytes of 16 rows are contiguous in a slot); four
-// slots are in flight.  grid (n_kv * row tiles * 8, batch).
-constexpr int kMergeRows = 16, kAhead = 4, kMergeThreads = kMergeRows * kHeadDim / 8;
-__global__ void __launch_bounds__(kMergeThreads, 2) attn_tree_merge_kernel(AttnTreeArgs a) {
+// rows and 32 dims of a row tile, a thread 4 dims of one row (32 bytes of 16 rows are contiguous in a slot); four
+// slots are in flight.  Blocks this small fit beside a CTA of the main kernel (56 registers a thread are left there),
+// so that they stand ready when its last CTA ends.  grid (n_kv * row tiles * 8 * 8, batch).
+constexpr int kMergeRows = 16, kMergeDims = 32, kAhead = 4, kMergeThreads = kMergeRows * kMergeDims / 4;
+constexpr int kMergeBlocks = kRows / kMergeRows * (kHeadDim / kMergeDims);             // of a row tile
+__global__ void __launch_bounds__(kMergeThreads, 9) attn_tree_merge_kernel(AttnTreeArgs a) {
     __shared__ Prefix prefix;
     const int tid = threadIdx.x, b = blockIdx.y;
     const int G = a.n_q / a.n_kv;
     if (tid < 32) build_prefix(prefix, a, tid, nullptr);
     __syncthreads();
     const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
-    const int hr = blockIdx.x / (kRows / kMergeRows), r = blockIdx.x % (kRows / kMergeRows) * kMergeRows + (tid & (kMergeRows - 1));
-    const int d0 = (tid / kMergeRows) * 8;
-    if (hr >= a.n_kv * q.row_tiles) {
-        griddep_wait();                                       // on every path: what follows this kernel follows the one in front too
+    const int hr = blockIdx.x / kMergeBlocks, part = blockIdx.x % kMergeBlocks;
+    const int r = part / (kHeadDim / kMergeDims) * kMergeRows + (tid >> 1 & (kMergeRows - 1));
+    const int d0 = part % (kHeadDim / kMergeDims) * kMergeDims + (tid >> 5) * 8 + (tid & 1) * 4;
+    int h = 0, node = 0, hq = 0, first = 0, parts = 0;
+    if (hr < a.n_kv * q.row_tiles) {
+        h = hr / q.row_tiles;
+        const int tr = (hr - h * q.row_tiles) * kRows + r, share = share_of(prefix.unit[a.batch], a);
+        node = tr / G;
+        hq = h * G + tr - node * G;
+        const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
+        first = u0 / share;
+        parts = node < q.nodes ? (u0 + q.tiles - 1) / share - first + 1 : 0;
+    }
+    // one part: written by the CTA that held all of it.  The grid's first block waits all the same: what follows this
+    // kernel then follows the one in front too.
+    if (parts <= 1) {
+        if (blockIdx.x == 0 && b == 0) griddep_wait();
         return;
     }
-    const int h = hr / q.row_tiles, tr = (hr - h * q.row_tiles) * kRows + r, node = tr / G, hq = h * G + tr - node * G;
-    const int share = share_of(prefix.unit[a.batch], a);
-    const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
-    const int first = u0 / share, parts = (u0 + q.tiles - 1) / share - first + 1;
-    if (node >= q.nodes || parts == 1) {                      // whole: written by the CTA that held all of it
-        griddep_wait();
-        return;
-    }
-    float4 g0, g1;
-    if (a.gate) {
-        const float* gp = a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0;
-        g0 = __ldcs(reinterpret_cast<const float4*>(gp));
-        g1 = __ldcs(reinterpret_cast<const float4*>(gp + 4));
-    }
+    const size_t row = (size_t(b) * a.max_nodes + node) * a.n_q + hq;
+    float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.gate) gate = __ldcs(reinterpret_cast<const float4*>(a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0));
     griddep_wait();
     const size_t slot0 = size_t(first) + prefix.seg[b] + hr;
-    float m = kNoMax, l = 0.f, x[8] = {};
+    const float* ml_at = a.part_ml + (slot0 * kRows + r) * 2;
+    const float* o_at = a.part_o + (slot0 * (kHeadDim / 8) + d0 / 8) * (kRows * 8) + r * 8 + (d0 & 7);
+    float m = kNoMax, l = 0.f, x[4] = {};
     for (int p0 = 0; p0 < parts; p0 += kAhead) {
         float2 ml[kAhead];
-        uint32_t o[kAhead][8];
+        float4 o[kAhead];
 #pragma unroll
         for (int z = 0; z < kAhead; ++z) {
             ml[z] = make_float2(kNoMax, 0.f);
+            o[z] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (p0 + z < parts) {
-                const size_t slot = slot0 + p0 + z;
-                ml[z] = *reinterpret_cast<const float2*>(a.part_ml + (slot * kRows + r) * 2);
-                ld_sector(a.part_o + (slot * (kHeadDim / 8) + d0 / 8) * (kRows * 8) + r * 8, o[z]);
+                ml[z] = *reinterpret_cast<const float2*>(ml_at + size_t(p0 + z) * (kRows * 2));
+                o[z] = *reinterpret_cast<const float4*>(o_at + size_t(p0 + z) * (kRows * kHeadDim));
             }
         }
         float mx = m;
@@ -682,25 +688,25 @@ __global__ void __launch_bounds__(kMergeThreads, 2) attn_tree_merge_kernel(AttnT
         m = mx;
         l *= back;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= back;
+        for (int e = 0; e < 4; ++e) x[e] *= back;
 #pragma unroll
         for (int z = 0; z < kAhead; ++z) {
-            if (p0 + z >= parts) break;
             const float w = fast_exp2(ml[z].x - m);
             l = fmaf(ml[z].y, w, l);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = fmaf(__uint_as_float(o[z][e]), w, x[e]);
+            x[0] = fmaf(o[z].x, w, x[0]);
+            x[1] = fmaf(o[z].y, w, x[1]);
+            x[2] = fmaf(o[z].z, w, x[2]);
+            x[3] = fmaf(o[z].w, w, x[3]);
         }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+    const float g[4] = {gate.x, gate.y, gate.z, gate.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= a.gate ? inv * sigmoid(g[e]) : inv;
-    uint32_t w[4];
+    for (int e = 0; e < 4; ++e) x[e] *= a.gate ? inv * sigmoid(g[e]) : inv;
+    uint32_t w[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = a.o_type == 1 ? pack_h2(x[2 * e], x[2 * e + 1]) : pack_b2(x[2 * e], x[2 * e + 1]);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + ((size_t(b) * a.max_nodes + node) * a.n_q + hq) * kHeadDim + d0) =
-        make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < 2; ++e) w[e] = a.o_type == 1 ? pack_h2(x[2 * e], x[2 * e + 1]) : pack_b2(x[2 * e], x[2 * e + 1]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + row * kHeadDim + d0) = make_uint2(w[0], w[1]);
 }
 
 namespace {
@@ -721,7 +727,7 @@ cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
     else attn_tree_kernel<false><<<a.grid, kThreads, kSmemBytes, st>>>(a);
     cudaLaunchConfig_t cfg = {};
     const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
-    cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * (kRows / kMergeRows)), unsigned(a.batch));
+    cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * kMergeBlocks), unsigned(a.batch));
     cfg.blockDim = dim3(kMergeThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
