@@ -1518,11 +1518,11 @@ static int attn_tree_check(const rl_attn_tree_params* p) {
 }
 
 // One persistent CTA per SM, fewer when the batch has less than kTreeMinShare pages for each: 8 nodes over 2 000
-// tokens take 20.7 us with 2 pages, 19.3 with 4, 21.4 with 6 (more CTAs leave more partials to merge).
-static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 4);
+// tokens take 15.3 us with 1 page, 14.8 with 2, 16.2 with 3, 16.5 with 4 (more CTAs leave more partials to merge).
+static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 2);
 // What a CTA pays to close one (sequence, head, row tile) and open the next (partial out, queries in, behind the pages
-// already requested), in pages.  16 trees of 21 over 16K: 161.5 us with 0, 157.0 with 6, 154.1 with 12, 149.6 with 18,
-// 150.4 with 26; 4 trees of 64 over 32K: 215.9, 210.3, 198.9, 201.1, 201.4.
+// already requested), in pages.  16 trees of 21 over 16K: 161.0 us with 4, 159.1 with 8, 156.3 with 12, 152.0 with 16,
+// 150.8 with 20; 4 trees of 64 over 32K: 208.5, 202.7, 197.7, 197.9, 202.6.
 static const int kTreeBoundary = knob("RL_B200_TREE_BOUNDARY", 16);
 struct AttnTreePlan {
     int grid;

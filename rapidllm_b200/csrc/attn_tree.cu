@@ -11,10 +11,11 @@
 // Work division: the (sequence, KV head, row tile, page) units of the whole batch form one list, computed on
 // the device from base_len and n_nodes (a captured step may advance them), and every CTA of a persistent
 // grid takes a contiguous share of equal cost, cut into segments at (sequence, head, row tile) boundaries; a
-// boundary is charged as kBoundary pages.  The page ring runs on across segments.  A segment that holds all
-// pages of its rows writes the output, the others write (unnormalised o, max, sum) to slot `CTA + segment
-// index`, distinct because a CTA's last segment is the next one's first at most; attn_tree_merge_kernel joins
-// them.
+// boundary is charged as some pages.  The page ring runs on across segments.  A segment's (unnormalised o, max,
+// sum) go to slot `CTA + segment index`, distinct because a CTA's last segment is the next one's first at most;
+// attn_tree_merge_kernel joins them, applies the gate and rounds.  Segments that hold all pages of their rows go
+// the same way: here a lane has a row, whose gate it would read 16 bytes from a line at a time (all outputs written
+// by the merge: 1 x 8 nodes over 120 tokens 14.1 us against 20.2, 16 x 64 over 2000 123 against 146).
 //
 // Inside a segment: S = Q K^T (M 128, N 64) and O += P V (M 128, N 256) with Q, P, S and O in tensor memory
 // and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
@@ -24,7 +25,7 @@
 // its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
 // query for an fp16 output is two such terms, the second from shared memory in the place of a third page of the
 // ring: with one, the scores' rounding would show (4.3e-4 relative instead of 2.9e-4).  A bf16 output's own
-// rounding (1.7e-3) hides it, and one term is faster (16 trees of 21 over 16K: 155 us against 180).
+// rounding (1.7e-3) hides it, and one term is faster (16 trees of 21 over 16K: 152 us against 177).
 // Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
 // not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
 // rows past the last node are cleared for the same reason.  A drafted V row that is not finite would reach the
@@ -55,7 +56,7 @@ constexpr int kMaxBatch = 512;
 
 struct Segment {
     int b, h, rt, index;                          // index: running number of (b, h, rt)
-    int j0, n_tiles, n_all;                       // pages [j0, j0 + n_tiles) of n_all; n_tiles 0: only the charge
+    int j0, n_tiles;                              // pages [j0, j0 + n_tiles); n_tiles 0: only the charge
     int base, nodes;
     int next;                                     // position of the next segment
 };
@@ -131,7 +132,6 @@ __device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArg
     s.rt = hr - s.h * q.row_tiles;
     s.index = p.seg[b] + hr;
     s.j0 = max(at, 0);
-    s.n_all = q.tiles;
     s.next = min(end, pos + q.tiles - at);
     s.n_tiles = max(at + s.next - pos - s.j0, 0);
     s.base = q.base;
@@ -200,25 +200,6 @@ __device__ __forceinline__ void load_q(float (&x)[64], const void* q, int q_type
 }
 // an infinity or a NaN in a pair of fp16
 __device__ __forceinline__ bool has_special(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
-// 32 outputs, gated, rounded to o_type
-__device__ __forceinline__ void store_o(const AttnTreeArgs& a, size_t at, const float* gate, float (&o)[32]) {
-    if (gate) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            const float4 g = __ldcs(reinterpret_cast<const float4*>(gate + i));
-            o[i] *= sigmoid(g.x); o[i + 1] *= sigmoid(g.y); o[i + 2] *= sigmoid(g.z); o[i + 3] *= sigmoid(g.w);
-        }
-    }
-    uint16_t* dst = static_cast<uint16_t*>(a.o) + at;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            w[e] = a.o_type == 1 ? pack_h2(o[16 * i + 2 * e], o[16 * i + 2 * e + 1]) : pack_b2(o[16 * i + 2 * e], o[16 * i + 2 * e + 1]);
-        st_sector(dst + 16 * i, w);
-    }
-}
 
 }  // namespace
 
@@ -588,9 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             const float l_run = (lp.x + lp.y) + (lp.z + lp.w);
             wait(&s.bar_pv[it_last & 1], (it_last >> 1) & 1);              // every P.V of the segment is done
             tc::fence_after_sync();
-            const bool whole = g.n_tiles == g.n_all;
             const size_t slot = size_t(blockIdx.x) + g.index;
-            const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
             const int col0 = quarter * 64;
             if (ok && __all_sync(0xffffffffu, !*const_cast<volatile int*>(&s.failed))) {
 #pragma unroll 1
@@ -600,26 +579,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     tc::tmem_ld32(lane_addr + kColO + col0 + c0, raw);
                     tc::tmem_wait_ld();
                     if (!live) continue;
-                    float o[32];
+                    // [slot][dims / 8][row][8]: a warp's 32 rows of 32 bytes are contiguous
+                    float* dst = a.part_o + (slot * (kHeadDim / 8) + (col0 + c0) / 8) * (kRows * 8) + r * 8;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(raw[i]) * inv;
-                    if (whole) {
-                        const float* gate = a.gate ? a.gate + (size_t(g.b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + col0 + c0
-                                                   : nullptr;
-                        store_o(a, flat * kHeadDim + col0 + c0, gate, o);
-                    } else {
-                        // [slot][dims / 8][row][8]: a warp's 32 rows of 32 bytes are contiguous
-                        float* dst = a.part_o + (slot * (kHeadDim / 8) + (col0 + c0) / 8) * (kRows * 8) + r * 8;
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t w[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) w[e] = raw[8 * i + e];
-                            st_sector(dst + i * (kRows * 8), w);
-                        }
+                        for (int e = 0; e < 8; ++e) w[e] = raw[8 * i + e];
+                        st_sector(dst + i * (kRows * 8), w);
                     }
                 }
-                if (!whole && live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
+                if (live && quarter == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(m_fin == kNoMax ? kNoMax : m_fin * scale_log2, l_run);
             }
             tc::fence_before_sync();
             named_bar_sync(9, kSoftmaxThreads);               // O, Q and `part` may be rewritten
@@ -629,38 +599,43 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
     if (warp == kWarpQK) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
-// Rows whose pages were divided: log-sum-exp over the row's slots (log2 domain), gate, rounding.  A block takes 16
-// rows and 32 dims of a row tile, a thread 4 dims of one row (32 bytes of 16 rows are contiguous in a slot); four
-// slots are in flight.  Blocks this small fit beside a CTA of the main kernel (56 registers a thread are left there),
-// so that they stand ready when its last CTA ends.  grid (n_kv * row tiles * 8 * 8, batch).
-constexpr int kMergeRows = 16, kMergeDims = 32, kAhead = 4, kMergeThreads = kMergeRows * kMergeDims / 4;
-constexpr int kMergeBlocks = kRows / kMergeRows * (kHeadDim / kMergeDims);             // of a row tile
-__global__ void __launch_bounds__(kMergeThreads, 9) attn_tree_merge_kernel(AttnTreeArgs a) {
+// Log-sum-exp over a row's slots (log2 domain), gate, rounding.  A thread takes 4 dims
+// of one row (32 bytes of 16 rows are contiguous in a slot) with four slots in flight, a block 16 rows; its 4 warps take
+// 4 x 8 dims, or with kSplit a quarter of the slots each of the same 8.  Blocks this small fit beside a CTA of the main
+// kernel (56 registers a thread are left there), so that they stand ready when its last CTA ends.
+// grid (n_kv * row tiles * merge_blocks(kSplit), batch).
+constexpr int kMergeRows = 16, kAhead = 4, kMergeWarps = 4;
+constexpr int merge_chunks(bool split) { return kHeadDim / 8 / (split ? 1 : kMergeWarps); }
+constexpr int merge_blocks(bool split) { return kRows / kMergeRows * merge_chunks(split); }     // of a row tile
+template <bool kSplit>
+__global__ void __launch_bounds__(kMergeWarps * 32, 9) attn_tree_merge_kernel(AttnTreeArgs a) {
     __shared__ Prefix prefix;
-    const int tid = threadIdx.x, b = blockIdx.y;
+    __shared__ float quarter[kMergeWarps - 1][6][32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;
     const int G = a.n_q / a.n_kv;
     if (tid < 32) build_prefix(prefix, a, tid, nullptr);
     __syncthreads();
     const Seq q = sequence(a, prefix.base[b], prefix.nodes[b], nullptr);
-    const int hr = blockIdx.x / kMergeBlocks, part = blockIdx.x % kMergeBlocks;
-    const int r = part / (kHeadDim / kMergeDims) * kMergeRows + (tid >> 1 & (kMergeRows - 1));
-    const int d0 = part % (kHeadDim / kMergeDims) * kMergeDims + (tid >> 5) * 8 + (tid & 1) * 4;
+    const int hr = blockIdx.x / merge_blocks(kSplit), part = blockIdx.x % merge_blocks(kSplit);
+    const int group = part / merge_chunks(kSplit) * kMergeRows, r = group + (lane >> 1);
+    const int d0 = (kSplit ? part % merge_chunks(kSplit) : part % merge_chunks(kSplit) * kMergeWarps + warp) * 8 + (lane & 1) * 4;
     int h = 0, node = 0, hq = 0, first = 0, parts = 0;
     if (hr < a.n_kv * q.row_tiles) {
         h = hr / q.row_tiles;
-        const int tr = (hr - h * q.row_tiles) * kRows + r, share = share_of(prefix.unit[a.batch], a);
-        node = tr / G;
-        hq = h * G + tr - node * G;
+        const int tr0 = (hr - h * q.row_tiles) * kRows, share = share_of(prefix.unit[a.batch], a);
+        node = (tr0 + r) / G;
+        hq = h * G + tr0 + r - node * G;
         const int u0 = prefix.unit[b] + hr * (q.tiles + a.boundary) + a.boundary;
         first = u0 / share;
-        parts = node < q.nodes ? (u0 + q.tiles - 1) / share - first + 1 : 0;
+        parts = (tr0 + group) / G < q.nodes ? (u0 + q.tiles - 1) / share - first + 1 : 0;
     }
-    // one part: written by the CTA that held all of it.  The grid's first block waits all the same: what follows this
-    // kernel then follows the one in front too.
-    if (parts <= 1) {
+    // nothing to do.  The grid's first block waits all the same: what follows this kernel then follows the one in front.
+    if (parts == 0) {
         if (blockIdx.x == 0 && b == 0) griddep_wait();
         return;
     }
+    const bool live = node < q.nodes;
+    if (!live) parts = node = hq = 0;
     const size_t row = (size_t(b) * a.max_nodes + node) * a.n_q + hq;
     float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.gate) gate = __ldcs(reinterpret_cast<const float4*>(a.gate + (size_t(b) * a.max_nodes + node) * a.gate_row + size_t(hq) * a.gate_head + d0));
@@ -669,7 +644,7 @@ __global__ void __launch_bounds__(kMergeThreads, 9) attn_tree_merge_kernel(AttnT
     const float* ml_at = a.part_ml + (slot0 * kRows + r) * 2;
     const float* o_at = a.part_o + (slot0 * (kHeadDim / 8) + d0 / 8) * (kRows * 8) + r * 8 + (d0 & 7);
     float m = kNoMax, l = 0.f, x[4] = {};
-    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+    for (int p0 = kSplit ? warp * kAhead : 0; p0 < parts; p0 += kSplit ? kMergeWarps * kAhead : kAhead) {
         float2 ml[kAhead];
         float4 o[kAhead];
 #pragma unroll
@@ -699,6 +674,32 @@ __global__ void __launch_bounds__(kMergeThreads, 9) attn_tree_merge_kernel(AttnT
             x[3] = fmaf(o[z].w, w, x[3]);
         }
     }
+    if constexpr (kSplit) {
+        if (warp) {
+            float* to = &quarter[warp - 1][0][lane];
+            to[0] = m;
+            to[32] = l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[64 + 32 * e] = x[e];
+        }
+        __syncthreads();
+        if (warp) return;
+        float mx = m;
+#pragma unroll
+        for (int z = 0; z < kMergeWarps - 1; ++z) mx = fmaxf(mx, quarter[z][0][lane]);
+        const float back = fast_exp2(m - mx);
+        l *= back;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= back;
+#pragma unroll
+        for (int z = 0; z < kMergeWarps - 1; ++z) {
+            const float w = fast_exp2(quarter[z][0][lane] - mx);
+            l = fmaf(quarter[z][1][lane], w, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(quarter[z][2 + e][lane], w, x[e]);
+        }
+    }
+    if (!live) return;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const float g[4] = {gate.x, gate.y, gate.z, gate.w};
 #pragma unroll
@@ -727,15 +728,18 @@ cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
     else attn_tree_kernel<false><<<a.grid, kThreads, kSmemBytes, st>>>(a);
     cudaLaunchConfig_t cfg = {};
     const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;
-    cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * kMergeBlocks), unsigned(a.batch));
-    cfg.blockDim = dim3(kMergeThreads);
+    // Many slots per row: their loads, four at a time, are the merge's time (1 x 8 nodes over 5 000 tokens, 37 slots:
+    // 17.9 us split, 23.2 not).  Few: blocks are, and a split has four times as many (4 x 8 over 1 000, 9: 21.1 and 17.5).
+    const bool split = a.grid >= 16 * a.batch * a.n_kv * row_tiles;
+    cfg.gridDim = dim3(unsigned(a.n_kv * row_tiles * merge_blocks(split)), unsigned(a.batch));
+    cfg.blockDim = dim3(kMergeWarps * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_tree_merge_kernel, a);
+    return split ? cudaLaunchKernelEx(&cfg, attn_tree_merge_kernel<true>, a) : cudaLaunchKernelEx(&cfg, attn_tree_merge_kernel<false>, a);
 }
 
 }  // namespace rl
