@@ -56,9 +56,10 @@ constexpr int kMaxBatch = 512;
 
 struct Segment {
     int b, h, rt, index;                          // index: running number of (b, h, rt)
-    int j0, n_tiles;                              // pages [j0, j0 + n_tiles); n_tiles 0: only the charge
+    int j0, n_tiles, tiles;                       // page(0) .. page(n_tiles - 1) of the sequence's `tiles`; n_tiles 0: only the charge
     int base, nodes;
     int next;                                     // position of the next segment
+    __device__ __forceinline__ int page(int j) const { return j0 + j < tiles ? j0 + j : j0 + j - tiles; }
 };
 
 // cost and segments of the sequences before b; entry `batch` holds the totals
@@ -121,8 +122,10 @@ __device__ __forceinline__ int share_of(int units, const AttnTreeArgs& a) {
     return max((units + a.grid - 1) / a.grid, a.min_share);
 }
 // the segment at position `pos` of a share that ends at `end`; b: a sequence at or before it.  A (sequence, head, row
-// tile) spans `boundary` positions of charge, then its pages.
-__device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArgs& a, int pos, int end, int& b) {
+// tile) spans `boundary` positions of charge, then its pages.  Row tiles of a head take the pages in an order rotated so
+// that those at the same place of two shares, which run at the same time, are the same ones: read from HBM once, not
+// once per row tile.
+__device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArgs& a, int share, int pos, int end, int& b) {
     while (p.unit[b + 1] <= pos) ++b;
     Segment s;
     const Seq q = sequence(a, p.base[b], p.nodes[b], nullptr);
@@ -134,6 +137,8 @@ __device__ __forceinline__ Segment segment_at(const Prefix& p, const AttnTreeArg
     s.j0 = max(at, 0);
     s.next = min(end, pos + q.tiles - at);
     s.n_tiles = max(at + s.next - pos - s.j0, 0);
+    s.tiles = q.tiles;
+    if (s.rt) s.j0 = (s.j0 + s.rt * span % share) % q.tiles;
     s.base = q.base;
     s.nodes = q.nodes;
     return s;
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         int b = 0, it = 0;
         bool ok = true;
         for (int pos = u_begin; pos < u_end && ok;) {
-            const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+            const Segment g = segment_at(s.prefix, a, share, pos, u_end, b);
             const bool first = pos == u_begin;
             pos = g.next;
             if (!g.n_tiles) continue;
@@ -261,12 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                 }
                 if (a.parents && lane < 2) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.parents + size_t(g.b) * a.max_nodes + min(lane * 32, a.max_nodes - 1)));
             }
-            const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq + g.j0;
+            const int32_t* table = a.page_table + size_t(g.b) * a.max_pages_per_seq;
             for (int j0 = 0; j0 < g.n_tiles && ok; j0 += 32) {
                 // 32 page ids at a time: the table's latency is paid once per 32 pages
                 int mine = 0;
                 if (j0 + lane < g.n_tiles) {
-                    mine = table[j0 + lane];
+                    mine = table[g.page(j0 + lane)];
                     if (mine < 0 || mine >= a.n_pages) {
                         set_err(a.err, DEV_ERR_BAD_PAGE);
                         mine = 0;
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             int b = 0, it = 0, sg = 0;
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok;) {
-                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+                const Segment g = segment_at(s.prefix, a, share, pos, u_end, b);
                 pos = g.next;
                 if (!g.n_tiles) continue;
                 ok = mbar_wait(&s.bar_q, sg & 1);
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             int b = 0, it = 0;
             bool ok = true;
             for (int pos = u_begin; pos < u_end && ok;) {
-                const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+                const Segment g = segment_at(s.prefix, a, share, pos, u_end, b);
                 pos = g.next;
                 if (!g.n_tiles) continue;
                 for (int j = 0; j < g.n_tiles; ++j, ++it) {
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
         };
         int b = 0, it0 = 0;                                   // it0: pages of the segments before
         for (int pos = u_begin; pos < u_end;) {
-            const Segment g = segment_at(s.prefix, a, pos, u_end, b);
+            const Segment g = segment_at(s.prefix, a, share, pos, u_end, b);
             pos = g.next;
             if (!g.n_tiles) continue;
             const int row = g.rt * kRows + r, node = row / G, hq = g.h * G + row - node * G;
@@ -435,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
             }
             // ---- this row's visible nodes ----
             unsigned long long seen = 0;
-            if ((g.j0 + g.n_tiles) * kTile > g.base) {        // the segment reaches the drafted rows
+            if (min(g.j0 + g.n_tiles, g.tiles) * kTile > g.base) {        // the segment reaches the drafted rows
                 const tree::Words w = tree::ancestors(a.parents ? a.parents + size_t(g.b) * a.max_nodes : nullptr, g.nodes, lane, a.err);
                 seen = tree::of_node(w.lo, w.hi, node & 63);
             }
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     tc::tmem_ld32(lane_addr + kColS + grp * 64 + half * 32, raw);
                     tc::tmem_wait_ld();
                 }
-                const int tok0 = (g.j0 + j) * kTile;
+                const int tok0 = g.page(j) * kTile;
                 const bool drafted = tok0 + kTile > g.base;   // rows behind the committed ones
                 const int first = max(g.base - tok0, 0);
                 if (drafted) {
