@@ -801,3 +801,13 @@ def test_gdn_commit_of_paths_with_bad_nodes():
         assert torch.equal(torch.isfinite(got[0][b]), fine)
         assert rel_l2(got[0][b][fine], state[fine]) <= STATE_REL_L2
         assert torch.equal(got[1][b].isnan(), window.isnan())
+
+
+@pytest.mark.parametrize("n_q,n_kv,nodes,base,counts,q_type,o_type", [
+    (24, 4, 64, [3000, 1500, 900], [64, 50, 30], torch.float16, torch.float16),    # 3, 3 and 2 row tiles in 11 pages a CTA
+    (16, 2, 64, [5000, 0, 2111], [64, 64, 17], torch.float32, torch.float16),      # 4, 4 and 2
+    (24, 4, 43, [9000], [43], torch.bfloat16, torch.bfloat16),                     # 3, the last one of one node
+])
+def test_attn_tree_row_tiles_over_long_caches(n_q, n_kv, nodes, base, counts, q_type, o_type):
+    """Row tiles start at different pages of a sequence and wrap around its end."""
+    test_attn_tree(n_q, n_kv, nodes, base, counts, 5, q_type, o_type, True)
