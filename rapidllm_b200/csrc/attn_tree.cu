@@ -604,10 +604,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
     if (warp == kWarpQK) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
-// Log-sum-exp over a row's slots (log2 domain), gate, rounding.  A thread takes 4 dims
-// of one row (32 bytes of 16 rows are contiguous in a slot) with four slots in flight, a block 16 rows; its 4 warps take
-// 4 x 8 dims, or with kSplit a quarter of the slots each of the same 8.  Blocks this small fit beside a CTA of the main
-// kernel (56 registers a thread are left there), so that they stand ready when its last CTA ends.
+// Log-sum-exp over a row's slots (log2 domain), gate, rounding.  A thread takes 4 dims of one row (32 bytes of 16 rows
+// are contiguous in a slot) with four slots in flight, a block 16 rows; its 4 warps take 4 x 8 dims, or with kSplit a
+// quarter of the slots each of the same 8.  Blocks this small fit beside a CTA of the main kernel (56 registers a thread
+// are left there), so that they stand ready when its last CTA ends (512 threads: 1 x 8 nodes over 9 000 tokens 30.8 us
+// against 26.2, before kSplit).
 // grid (n_kv * row tiles * merge_blocks(kSplit), batch).
 constexpr int kMergeRows = 16, kAhead = 4, kMergeWarps = 4;
 constexpr int merge_chunks(bool split) { return kHeadDim / 8 / (split ? 1 : kMergeWarps); }
