@@ -5,8 +5,9 @@
 //
 // All query rows of a KV head -- (node, query head of the group) pairs, up to 64 x 8 -- share its K and V,
 // so the 128 rows of an MMA tile are such pairs and a sequence's pages are read once per 128 rows (at 24 / 4
-// heads: once for up to 21 nodes).  Up to there the cache's bandwidth is the bound, beyond it the tensor
-// cores are.
+// heads: once for up to 21 nodes).  Up to there the cache's bandwidth is the bound (16 trees of 21 over 16K: 779 MB
+// in 151 us, boundaries included), beyond it the pages' way into each SM (4 trees of 64 over 32K: 187 us, tensor pipe
+// 41 % busy).
 //
 // Work division: the (sequence, KV head, row tile, page) units of the whole batch form one list, computed on
 // the device from base_len and n_nodes (a captured step may advance them), and every CTA of a persistent
