@@ -433,10 +433,25 @@ def _rows(t, shape, dev, name):
 
 
 def _row_distance(shape, strides, inner, name):
+    """Floats between the rows of [batch][rows]...  Rows that share memory (an expanded tensor has them 0 apart, which
+    the C ABI takes as "dense") are refused here: the kernels would read behind the one row that exists."""
     row = strides[1] if shape[1] > 1 else (strides[0] if shape[0] > 1 else inner)
+    if row < inner:
+        raise _lib.RlError(6, f"{name}: rows {row} floats apart share memory, a row has {inner}")
     if shape[0] > 1 and shape[1] > 1 and strides[0] != shape[1] * row:
         raise _lib.RlError(6, f"{name}: the rows of all sequences must be at one distance")
     return row
+
+
+def _gate(gate, shape, dev):
+    """Address of fp32 [batch][nodes][heads][256], contiguous inside a head; floats between its rows and its heads."""
+    if gate.get_device() != dev or gate.dtype is not _F32 or gate.shape != shape or gate.stride(3) != 1:
+        raise _lib.RlError(6, f"gate: need a {_F32} tensor of shape {tuple(shape)} on the current device cuda:{dev}, contiguous inside a head")
+    strides = gate.stride()
+    head = strides[2] if shape[2] > 1 else shape[3]
+    if head < shape[3]:
+        raise _lib.RlError(6, f"gate: heads {head} floats apart share memory, a head has {shape[3]}")
+    return gate.data_ptr(), _row_distance(shape, strides, head * shape[2], "gate"), head
 
 
 def _scratch(workspace, need, device):
@@ -524,12 +539,7 @@ def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=Non
     row = head = 0
     gate_p = None
     if gate is not None:
-        strides = gate.stride()
-        if gate.get_device() != dev or gate.dtype is not _F32 or gate.shape != shape or strides[3] != 1:
-            raise _lib.RlError(6, f"gate: need a {_F32} tensor of shape {tuple(shape)} on the current device cuda:{dev}, contiguous inside a head")
-        head = strides[2] if n_q > 1 else hd
-        row = _row_distance(shape, strides, head * n_q, "gate")
-        gate_p = gate.data_ptr()
+        gate_p, row, head = _gate(gate, shape, dev)
     p, need = _attn_tree_plan(dev, n_q, n_kv, hd, batch, nodes, PAGE_TOKENS, n_pages, pages,
                               pages * PAGE_TOKENS if max_seq_len is None else max_seq_len, _TYPES[q.dtype], _TYPES[out.dtype], row, head)
     workspace, size = _scratch(workspace, need, q.device)
