@@ -491,7 +491,8 @@ typedef struct rl_kv_tree_commit_params {
 
 /* Keep one path of each sequence: the K and V rows of its nodes move to positions base_len[b],
  * base_len[b] + 1, ...  n_accept int32 [batch] or NULL receives the length of each path (0 for leaf -1);
- * the sequence then has base_len[b] + n_accept[b] tokens. */
+ * the sequence then has base_len[b] + n_accept[b] tokens.  A sequence whose base_len is outside its table or whose rows
+ * from base_len[b] to the leaf's have a bad page is recorded and left as it is: it accepts 0. */
 int rl_kv_tree_commit(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* base_len,
                       const int32_t* parents, const int32_t* leaf, int32_t* n_accept,
                       const rl_kv_tree_commit_params* p, void* stream);

@@ -171,20 +171,30 @@ __global__ void __launch_bounds__(kCommitWarps * 32) kv_tree_commit_kernel(KvTre
             tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, leaf + 1, lane, a.err);
         path = tree::of_node(w.lo, w.hi, leaf);
     }
-    if (a.n_accept && threadIdx.x == 0 && h == 0 && blockIdx.z == 0) a.n_accept[b] = __popcll(path);
+    // A sequence with a row that has no place is left as it is, in both pools and every head, and accepts nothing.  64 rows
+    // lie in two pages at most, the first's and the leaf's.
     const int base = a.base_len[b];
-    if (path && (base < 0 || (long long)base + leaf >= (long long)a.max_pages_per_seq * kPageTokens)) {
-        if (threadIdx.x == 0) set_err(a.err, DEV_ERR_BAD_LEN);
-        return;
-    }
-    __half* pool = blockIdx.z ? a.v_pool : a.k_pool;
     const int32_t* table = a.page_table + size_t(b) * a.max_pages_per_seq;
-    auto row_at = [&](int at) -> __half* {
-        const int page = table[at / kPageTokens];
-        if (page < 0 || page >= a.n_pages) {
-            if (lane == 0) set_err(a.err, DEV_ERR_BAD_PAGE);
-            return nullptr;
+    int page0 = 0, page1 = 0;
+    if (path) {
+        int bad = DEV_OK;
+        if (base < 0 || (long long)base + leaf >= (long long)a.max_pages_per_seq * kPageTokens) {
+            bad = DEV_ERR_BAD_LEN;
+        } else {
+            page0 = table[base / kPageTokens];
+            page1 = table[(base + leaf) / kPageTokens];
+            if (page0 < 0 || page0 >= a.n_pages || page1 < 0 || page1 >= a.n_pages) bad = DEV_ERR_BAD_PAGE;
         }
+        if (bad) {
+            if (threadIdx.x == 0) set_err(a.err, bad);
+            path = 0;
+        }
+    }
+    if (a.n_accept && threadIdx.x == 0 && h == 0 && blockIdx.z == 0) a.n_accept[b] = __popcll(path);
+    if (!path) return;
+    __half* pool = blockIdx.z ? a.v_pool : a.k_pool;
+    auto row_at = [&](int at) -> __half* {
+        const int page = at / kPageTokens == base / kPageTokens ? page0 : page1;
         return pool + (size_t(page) * a.n_kv + h) * kv_slice_elems() + kv_slice_offset(at % kPageTokens, lane * 8);
     };
     uint4 rows[kCommitRows];
@@ -195,9 +205,8 @@ __global__ void __launch_bounds__(kCommitWarps * 32) kv_tree_commit_kernel(KvTre
         got[j] = false;
         // a node whose depth is its index stays where it is
         if ((path >> i & 1) && __popcll(path & ((1ull << i) - 1)) != i) {
-            const __half* src = row_at(base + i);
-            got[j] = src != nullptr;
-            if (src) rows[j] = *reinterpret_cast<const uint4*>(src);
+            got[j] = true;
+            rows[j] = *reinterpret_cast<const uint4*>(row_at(base + i));
         }
     }
     __syncthreads();
@@ -205,8 +214,7 @@ __global__ void __launch_bounds__(kCommitWarps * 32) kv_tree_commit_kernel(KvTre
     for (int j = 0; j < kCommitRows; ++j) {
         const int i = warp + j * kCommitWarps;
         if (!got[j]) continue;
-        __half* dst = row_at(base + __popcll(path & ((1ull << i) - 1)));
-        if (dst) *reinterpret_cast<uint4*>(dst) = rows[j];
+        *reinterpret_cast<uint4*>(row_at(base + __popcll(path & ((1ull << i) - 1)))) = rows[j];
     }
 }
 

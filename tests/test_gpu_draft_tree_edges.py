@@ -43,3 +43,29 @@ def test_expanded_inputs_are_refused():
     _lib.check_device()
     for t, was in zip((kp, S, win), kept):
         assert torch.equal(t, was)
+
+
+def test_kv_commit_accepts_nothing_where_it_moves_nothing():
+    """A base outside the table and a bad page under the rows up to the leaf: the sequence's rows stay, its accepted length
+    is 0 (the caller adds it to base_len); the other sequences are served."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(42)
+    base, n = [60, 60, 62, 130, 70, 10, 40], 8
+    kp, vp, table, _ = _pages(gen, base, [n] * 7, 4, 0.0)
+    parents = torch.tensor([[-1, -1, 1, 0, 2, 4, 3, 5]] * 7, dtype=torch.int32)
+    parents[5] = torch.arange(n) - 1                          # a chain, whose rows stay where they are
+    leaf = [7] * 7
+    table[1, 1] = -1                                          # the page of the leaf
+    table[2, 0] = kp.shape[0]                                 # the page of the first row
+    table[5, 0] = -7
+    bases = [60, 60, 62, table.shape[1] * 64 - 7, -1, 10, 40]
+    want = [pool.clone() for pool in (kp, vp)]
+    for b in (0, 6):
+        for w, src in zip(want, (kp, vp)):
+            for j, i in enumerate(_path(parents[b].tolist(), 7)):
+                page, at = int(table[b, (base[b] + j) // 64]), (base[b] + j) % 64
+                w[page][:, ops.kv_slice_index(torch.full((HD,), at), torch.arange(HD)).cuda()] = _pool_row(src, table, b, base[b] + i)
+    taken = ops.kv_tree_commit(kp, vp, table, _i32(bases), parents.cuda(), _i32(leaf))
+    assert _lib.device_error() in (1, 5)
+    assert taken.tolist() == [5, 0, 0, 0, 0, 0, 5]
+    assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
