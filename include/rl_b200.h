@@ -419,7 +419,7 @@ int rl_delta_gates(const float* a, const float* b, const float* A_log, const flo
  *             -1 = it continues the committed history.  NULL = a chain (parents[i] = i - 1)
  *   n_nodes   int32 [batch], nodes of each sequence in [0, max_nodes]; NULL = max_nodes.  Rows behind
  *             a sequence's last node are neither read nor written
- *   leaf      int32 [batch], the last node of the path to keep, or -1 to keep none
+ *   leaf      int32 [batch], the last node of the path to keep (in [0, n_nodes[b])), or -1 to keep none
  * all on the device.  A parent, count or leaf out of its range is recorded like bad pages and slots
  * (rl_device_error): the parent counts as -1, the count as 0, the leaf as -1.  The K and V rows of node i
  * lie at cache position base_len + i until the commit; its rotary position is base_len + its depth.
@@ -487,6 +487,7 @@ typedef struct rl_kv_tree_commit_params {
     int n_kv, head_dim;          /* 4, 256 */
     int batch, max_nodes;
     int page_tokens, n_pages, max_pages_per_seq;
+    const int32_t* n_nodes;      /* device, as the verify had them: no leaf lies behind them.  NULL = max_nodes */
 } rl_kv_tree_commit_params;
 
 /* Keep one path of each sequence: the K and V rows of its nodes move to positions base_len[b],
@@ -504,6 +505,8 @@ typedef struct rl_gdn_tree_params {
     int head_map;                /* RL_HEADS_* */
     float eps_l2;                /* 1e-6 */
     long long qkv_stride;        /* floats between rows of qkv (0 = dense), a multiple of 4 */
+    const int32_t* commit_nodes; /* rl_gdn_tree_commit: device, rl_gdn_tree's n_nodes; no leaf lies behind them.
+                                  * NULL = max_nodes */
 } rl_gdn_tree_params;
 
 /* rl_gdn_decode for every node of a tree, each along its own path: conv over the node, its ancestors and

@@ -87,12 +87,12 @@ class AttnTreeParams(C.Structure):
 
 class KvTreeCommitParams(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_kv", "head_dim", "batch", "max_nodes", "page_tokens", "n_pages",
-                                       "max_pages_per_seq")]
+                                       "max_pages_per_seq")] + [("n_nodes", C.c_void_p)]
 
 
 class GdnTreeParams(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_v", "n_qk", "dk", "dv", "conv_k", "batch", "max_nodes", "n_slots",
-                                       "head_map")] + [("eps_l2", C.c_float), ("qkv_stride", C.c_longlong)]
+                                       "head_map")] + [("eps_l2", C.c_float), ("qkv_stride", C.c_longlong), ("commit_nodes", C.c_void_p)]
 
 
 class PlanInput(C.Structure):

@@ -1614,6 +1614,7 @@ int rl_kv_tree_commit(void* k_pool, void* v_pool, const int32_t* page_table, con
     a.page_table = page_table;
     a.base_len = base_len;
     a.parents = parents;
+    a.n_nodes = p->n_nodes;
     a.leaf = leaf;
     a.n_accept = n_accept;
     a.err = d->err_ptr;
@@ -1716,6 +1717,7 @@ int rl_gdn_tree_commit(float* S, float* conv_window, const int32_t* conv_phase, 
     if (!aligned16(workspace)) return fail(RL_ERR_RANGE, "workspace must be 16-byte aligned");
     const size_t need = rl::gdn_tree_commit_workspace_bytes(p->batch, p->max_nodes, p->n_v, p->n_qk);
     if (workspace_bytes < need) return fail(RL_ERR_RANGE, "workspace %zu bytes < %zu required", workspace_bytes, need);
+    a.n_nodes = p->commit_nodes;
     a.leaf = leaf;
     a.S_out = S;
     a.conv_out = conv_window;

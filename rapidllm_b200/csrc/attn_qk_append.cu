@@ -161,12 +161,9 @@ void launch_attn_qk_append(const AttnQkAppendArgs& a, int batch, cudaStream_t st
 constexpr int kCommitWarps = 16, kCommitRows = tree::kMaxNodes / kCommitWarps;
 __global__ void __launch_bounds__(kCommitWarps * 32) kv_tree_commit_kernel(KvTreeCommitArgs a) {
     const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int leaf = a.leaf[b];
-    if (leaf < -1 || leaf >= a.max_nodes) {
-        if (threadIdx.x == 0) set_err(a.err, DEV_ERR_BAD_TREE);
-    }
+    const int leaf = tree::checked_leaf(a.leaf, a.n_nodes, b, a.max_nodes, threadIdx.x == 0 ? a.err : nullptr);
     unsigned long long path = 0;
-    if (leaf >= 0 && leaf < a.max_nodes) {
+    if (leaf >= 0) {
         const tree::Words w =
             tree::ancestors(a.parents ? a.parents + size_t(b) * a.max_nodes : nullptr, leaf + 1, lane, a.err);
         path = tree::of_node(w.lo, w.hi, leaf);

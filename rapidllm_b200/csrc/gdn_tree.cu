@@ -750,13 +750,13 @@ __global__ void __launch_bounds__(kPathWarps * 32) gdn_tree_path_kernel(GdnTreeA
     __shared__ int path_len;
     griddep_launch();
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int slot = a.slot_ids ? a.slot_ids[b] : b, leaf = a.leaf[b];
+    const int slot = a.slot_ids ? a.slot_ids[b] : b;
+    const int leaf = tree::checked_leaf(a.leaf, a.n_nodes, b, a.max_nodes, tid == 0 ? a.err : nullptr);
     const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
-    const bool bad_slot = slot < 0 || slot >= a.n_slots, none = leaf < 0 || leaf >= a.max_nodes;
-    if (bad_slot || none) {
+    const bool bad_slot = slot < 0 || slot >= a.n_slots;
+    if (bad_slot || leaf < 0) {
         if (tid == 0) {
             if (bad_slot) set_err(a.err, DEV_ERR_BAD_SLOT);
-            if (none && leaf != -1) set_err(a.err, DEV_ERR_BAD_TREE);
             if (blockIdx.x == 0) ws.len[b] = 0;
         }
         return;
@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(kCommitThreads, 4) gdn_tree_commit_kernel(GdnT
     const int b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const CommitWorkspace ws = commit_workspace(a.workspace, a.batch, a.max_nodes, a.n_v, a.n_qk);
     const int slot = a.slot_ids ? a.slot_ids[b] : b;
-    if (slot < 0 || slot >= a.n_slots || a.leaf[b] < 0 || a.leaf[b] >= a.max_nodes) {
+    if (slot < 0 || slot >= a.n_slots || tree::checked_leaf(a.leaf, a.n_nodes, b, a.max_nodes, nullptr) < 0) {
         griddep_wait();                                       // on every path: what follows this kernel follows the one in front too
         return;
     }

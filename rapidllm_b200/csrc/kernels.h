@@ -304,6 +304,7 @@ struct KvTreeCommitArgs {
     const int32_t* page_table;
     const int32_t* base_len;     // [batch] committed tokens
     const int32_t* parents;
+    const int32_t* n_nodes;      // [batch] or null: max_nodes
     const int32_t* leaf;         // [batch] last node of the path, -1: none
     int32_t* n_accept;           // [batch] length of the path, or null
     int* err;

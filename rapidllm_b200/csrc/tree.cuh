@@ -66,5 +66,13 @@ __device__ __forceinline__ int node_count(const int32_t* n_nodes, int b, int max
     return 0;
 }
 
+// last node of the path to keep, -1: none; one that is not in [-1, nodes) records DEV_ERR_BAD_TREE and counts as -1
+__device__ __forceinline__ int checked_leaf(const int32_t* leaf, const int32_t* n_nodes, int b, int max_nodes, int* err) {
+    const int i = leaf[b], n = node_count(n_nodes, b, max_nodes, err);
+    if (i >= -1 && i < n) return i;
+    set_err(err, DEV_ERR_BAD_TREE);
+    return -1;
+}
+
 }  // namespace tree
 }  // namespace rl

@@ -113,16 +113,17 @@ class DeltaNetMixer:
         z = proj[:, cd:cd + zd].contiguous()
         beta, g = ops.delta_gates(proj[:, cd + zd:cd + zd + nv].contiguous(), proj[:, cd + zd + nv:].contiguous(),
                                   self.A_log, self.dt_bias)
-        pending = (qkv, beta.view(B, n, nv), g.view(B, n, nv))
+        pending = (qkv, beta.view(B, n, nv), g.view(B, n, nv), n_nodes)
         o = ops.gdn_tree(self.S, self.conv_state, None, pending[0], self.conv_w, pending[1], pending[2], parents, self.n_k,
                          n_nodes=n_nodes, slot_ids=slot_ids, head_map=self.head_map)
         og = ops.gated_rmsnorm(o.view(B * n, nv, self.dv), z.view(B * n, nv, self.dv), self.gnorm, 1e-6)
         return (rows + _matmul(og.view(B * n, zd), self.W_out)).view(B, n, hidden), pending
 
     def commit_tree(self, pending, parents, leaf, slot_ids=None):
-        """Advance the slots by the path to node leaf[b] (-1: nothing) of the tree that verify_tree ran."""
+        """Advance the slots by the path to node leaf[b] (-1: nothing) of the tree that verify_tree ran; a leaf behind
+        the n_nodes it was given is recorded and counts as -1."""
         ops.gdn_tree_commit(self.S, self.conv_state, None, pending[0], self.conv_w, pending[1], pending[2], parents, leaf,
-                            self.n_k, slot_ids=slot_ids, head_map=self.head_map)
+                            self.n_k, slot_ids=slot_ids, head_map=self.head_map, n_nodes=pending[3])
 
 
 class GatedAttentionMixer:
@@ -172,9 +173,10 @@ class GatedAttentionMixer:
         o = ops.attn_tree(q, self.k_pool, self.v_pool, page_table, base_len, parents, n_nodes=n_nodes, gate=qg[..., self.hd:])
         return (rows + _matmul(o.view(B * n, qn), self.W_out)).view(B, n, hidden)
 
-    def commit_tree(self, page_table, base_len, parents, leaf):
-        """Keep the path to node leaf[b] (-1: nothing); returns the paths' lengths, by which base_len grows."""
-        return ops.kv_tree_commit(self.k_pool, self.v_pool, page_table, base_len, parents, leaf)
+    def commit_tree(self, page_table, base_len, parents, leaf, n_nodes=None):
+        """Keep the path to node leaf[b] (-1: nothing); returns the paths' lengths, by which base_len grows.  n_nodes as
+        verify_tree had them."""
+        return ops.kv_tree_commit(self.k_pool, self.v_pool, page_table, base_len, parents, leaf, n_nodes=n_nodes)
 
 
 class MixerStack:
@@ -216,7 +218,7 @@ class MixerStack:
         for layer in self.layers:
             if isinstance(layer, GatedAttentionMixer):
                 x = layer.verify_tree(x, page_table, base_len, parents, n_nodes)
-                pending.append(None)
+                pending.append(n_nodes)
             else:
                 x, kept = layer.verify_tree(x, parents, n_nodes, slot_ids)
                 pending.append(kept)
@@ -228,7 +230,7 @@ class MixerStack:
         taken = None
         for layer, kept in zip(self.layers, pending):
             if isinstance(layer, GatedAttentionMixer):
-                taken = layer.commit_tree(page_table, base_len, parents, leaf)
+                taken = layer.commit_tree(page_table, base_len, parents, leaf, kept)
             else:
                 layer.commit_tree(kept, parents, leaf, slot_ids)
         return taken

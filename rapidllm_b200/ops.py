@@ -550,17 +550,18 @@ def attn_tree(q, k_pool, v_pool, page_table, base_len, parents=None, n_nodes=Non
     return out
 
 
-def kv_tree_commit(k_pool, v_pool, page_table, base_len, parents, leaf):
+def kv_tree_commit(k_pool, v_pool, page_table, base_len, parents, leaf, n_nodes=None):
     """Keep the path to node leaf[b] (int32 [batch], -1 = nothing) of each sequence's tree: its K and V rows move
     to positions base_len[b], base_len[b] + 1, ...  Returns the paths' lengths, int32 [batch].  parents int32
-    [batch][nodes], or the number of nodes for chains."""
+    [batch][nodes], or the number of nodes for chains; n_nodes int32 [batch] as the verify had them: a leaf behind
+    them counts as -1."""
     dev = torch.cuda.current_device()
     batch = leaf.shape[0]
     chain = isinstance(parents, int)
     nodes = parents if chain else parents.shape[1]
     n_pages, n_kv, pages, kp, vp, table = _pools(k_pool, v_pool, page_table, batch, dev)
     n_accept = torch.empty_like(leaf)
-    p = _lib.KvTreeCommitParams(n_kv, HEAD_DIM, batch, nodes, PAGE_TOKENS, n_pages, pages)
+    p = _lib.KvTreeCommitParams(n_kv, HEAD_DIM, batch, nodes, PAGE_TOKENS, n_pages, pages, _arg(n_nodes, _I32, (batch,), dev, "n_nodes"))
     check(lib().rl_kv_tree_commit(kp, vp, table, _needed(base_len, _I32, (batch,), dev, "base_len"),
                                   None if chain else _needed(parents, _I32, (batch, nodes), dev, "parents"),
                                   _needed(leaf, _I32, (batch,), dev, "leaf"), n_accept.data_ptr(), p, _stream_of(dev)))
@@ -606,13 +607,14 @@ def gdn_tree(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, n_qk
 
 
 def gdn_tree_commit(S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, n_qk, slot_ids=None,
-                    head_map=None, eps_l2=1e-6, workspace=None):
+                    head_map=None, eps_l2=1e-6, workspace=None, n_nodes=None):
     """Advance S and conv_window of each sequence's slot by the path to node leaf[b] (-1 = nothing), in place, with
-    gdn_tree's inputs; conv_phase stays.  slot_ids must be distinct."""
+    gdn_tree's inputs; conv_phase stays.  slot_ids must be distinct; a leaf behind n_nodes[b] counts as -1."""
     dev = torch.cuda.current_device()
     p, args = _gdn_tree_args(dev, S, conv_window, conv_phase, qkv, conv_w, beta, g_log, parents, leaf, "leaf", n_qk, slot_ids,
                              head_map, eps_l2)
     if leaf is None:
         raise _lib.RlError(6, "leaf: is None")
+    p.commit_nodes = _arg(n_nodes, _I32, (qkv.shape[0],), dev, "n_nodes")
     workspace, size = _scratch(workspace, lib().rl_gdn_tree_commit_workspace_bytes(p), S.device)
     check(lib().rl_gdn_tree_commit(*args, _arg(workspace, workspace.dtype, workspace.shape, dev, "workspace"), size, p, _stream_of(dev)))

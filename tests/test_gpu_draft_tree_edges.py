@@ -69,3 +69,54 @@ def test_kv_commit_accepts_nothing_where_it_moves_nothing():
     assert _lib.device_error() in (1, 5)
     assert taken.tolist() == [5, 0, 0, 0, 0, 0, 5]
     assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+def test_a_leaf_behind_the_last_node_keeps_nothing():
+    """Of a ragged draft: rows behind n_nodes[b] are neither read nor written, so a leaf there is recorded and counts as
+    -1, in both commits and through the mixers; the last node itself is a leaf."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(43)
+    B, n, n_v, n_qk = 5, 12, 6, 2
+    counts, leaf = [5, 5, 0, 12, 13], [5, 4, 0, 11, 3]        # the last count is itself out of range: an empty draft
+    parents = _tree(gen, B, n, 3)
+    parents[0, 5:] = 77                                       # not validated by a verify, and not followed here
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, B, n, n_v, n_qk, B)
+    qkv[0, 5:] = float("nan")
+    dev = [t.cuda() for t in (S, win)]
+    ops.gdn_tree_commit(*dev, None, *(t.cuda() for t in (qkv, w, beta, g, parents)), _i32(leaf), n_qk, n_nodes=_i32(counts))
+    assert _lib.device_error() == 6
+    for b in range(B):
+        if b in (1, 3):
+            path = _path(parents[b].tolist(), leaf[b])
+            _, state, window = _gdn_exact(S[b], win[b], qkv[b], w, beta[b], g[b], path, n_v, n_qk, False)
+            assert rel_l2(dev[0][b].cpu(), state) <= STATE_REL_L2 and torch.equal(dev[1][b].cpu(), window.float())
+        else:
+            assert torch.equal(dev[0][b].cpu(), S[b]) and torch.equal(dev[1][b].cpu(), win[b])
+    base = [60, 61, 62, 63, 10]
+    kp, vp, table, _ = _pages(gen, base, [n] * B, 4, 0.0)
+    before = [[_pool_row(kp, table, b, base[b] + i).clone() for i in range(n)] for b in range(B)]
+    taken = ops.kv_tree_commit(kp, vp, table, _i32(base), parents.cuda(), _i32(leaf), n_nodes=_i32(counts))
+    assert _lib.device_error() == 6
+    paths = [_path(parents[b].tolist(), leaf[b]) if b in (1, 3) else [] for b in range(B)]
+    assert taken.tolist() == [len(p) for p in paths]
+    for b in range(B):
+        for i in range(n):
+            src = paths[b][i] if i < len(paths[b]) else i
+            assert torch.equal(_pool_row(kp, table, b, base[b] + i), before[b][src])
+
+
+def test_the_stack_remembers_the_nodes_of_a_draft():
+    """A commit through the mixers refuses the leaves that its verify did not run."""
+    from rapidllm_b200 import _lib
+    from rapidllm_b200.mixer import MixerStack
+    gen = torch.Generator().manual_seed(44)
+    attn, delta = _weights(gen, 128)
+    stack = MixerStack([_lib.RL_LAYER_LINEAR_ATTENTION, _lib.RL_LAYER_FULL_ATTENTION], [delta, attn], n_pages=2, n_slots=2, n_q=6,
+                       n_kv=1, n_k=2, n_v=6)
+    table, base, parents = _i32([[0], [1]]), _i32([0, 0]), _tree(gen, 2, 6, 2).cuda()
+    _, pending = stack.verify_tree(torch.randn(2, 6, 128, generator=gen).cuda(), table, base, parents, _i32([3, 6]))
+    _lib.check_device()
+    taken = stack.commit_tree(pending, table, base, parents, _i32([3, 5]))
+    assert _lib.device_error() == 6
+    assert taken.tolist() == [0, len(_path(parents[1].tolist(), 5))]
+    assert not stack.layers[0].S[0].any() and not stack.layers[0].conv_state[0].any() and stack.layers[0].S[1].any()
