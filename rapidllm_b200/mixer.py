@@ -174,8 +174,8 @@ class GatedAttentionMixer:
         return (rows + _matmul(o.view(B * n, qn), self.W_out)).view(B, n, hidden)
 
     def commit_tree(self, page_table, base_len, parents, leaf, n_nodes=None):
-        """Keep the path to node leaf[b] (-1: nothing); returns the paths' lengths, by which base_len grows.  n_nodes as
-        verify_tree had them."""
+        """Keep the path to node leaf[b] (-1: nothing); returns the paths' lengths, by which base_len grows.  parents,
+        or the number of nodes for chains, and n_nodes as verify_tree had them."""
         return ops.kv_tree_commit(self.k_pool, self.v_pool, page_table, base_len, parents, leaf, n_nodes=n_nodes)
 
 
@@ -212,13 +212,13 @@ class MixerStack:
 
     def verify_tree(self, x, page_table, base_len, parents, n_nodes=None, slot_ids=None):
         """One verify pass over a draft tree: x fp32 [batch][nodes][hidden] -> hidden states after the last mixer, and
-        what commit_tree needs.  parents int32 [batch][nodes] (< own index, -1 = continues the committed tokens),
-        n_nodes int32 [batch] or None, base_len int32 [batch] committed tokens, all on the device."""
+        what commit_tree needs.  parents int32 [batch][nodes] (< own index, -1 = continues the committed tokens) or
+        None for chains, n_nodes int32 [batch] or None, base_len int32 [batch] committed tokens, all on the device."""
         pending = []
         for layer in self.layers:
             if isinstance(layer, GatedAttentionMixer):
                 x = layer.verify_tree(x, page_table, base_len, parents, n_nodes)
-                pending.append(n_nodes)
+                pending.append((x.shape[1], n_nodes))
             else:
                 x, kept = layer.verify_tree(x, parents, n_nodes, slot_ids)
                 pending.append(kept)
@@ -226,11 +226,17 @@ class MixerStack:
 
     def commit_tree(self, pending, page_table, base_len, parents, leaf, slot_ids=None):
         """Keep the path to node leaf[b] (int32 [batch], -1: nothing) in every layer; returns the paths' lengths,
-        int32 [batch] (the caller adds them to base_len), or None without an attention layer."""
+        int32 [batch] (the caller adds them to base_len), or None without an attention layer.  pending and parents (None
+        for chains) as the verify had them."""
+        if len(pending) != len(self.layers):
+            raise _lib.RlError(6, f"pending of {len(pending)} layers, the stack has {len(self.layers)}")
+        if parents is not None and not torch.is_tensor(parents):
+            raise _lib.RlError(6, "parents: need the verify's tensor, or None for chains")
         taken = None
         for layer, kept in zip(self.layers, pending):
             if isinstance(layer, GatedAttentionMixer):
-                taken = layer.commit_tree(page_table, base_len, parents, leaf, kept)
+                nodes, n_nodes = kept
+                taken = layer.commit_tree(page_table, base_len, nodes if parents is None else parents, leaf, n_nodes)
             else:
                 layer.commit_tree(kept, parents, leaf, slot_ids)
         return taken

@@ -558,6 +558,8 @@ def kv_tree_commit(k_pool, v_pool, page_table, base_len, parents, leaf, n_nodes=
     dev = torch.cuda.current_device()
     batch = leaf.shape[0]
     chain = isinstance(parents, int)
+    if parents is None:
+        raise _lib.RlError(6, "parents: is None (chains: the number of nodes)")
     nodes = parents if chain else parents.shape[1]
     n_pages, n_kv, pages, kp, vp, table = _pools(k_pool, v_pool, page_table, batch, dev)
     n_accept = torch.empty_like(leaf)

@@ -120,3 +120,36 @@ def test_the_stack_remembers_the_nodes_of_a_draft():
     assert _lib.device_error() == 6
     assert taken.tolist() == [0, len(_path(parents[1].tolist(), 5))]
     assert not stack.layers[0].S[0].any() and not stack.layers[0].conv_state[0].any() and stack.layers[0].S[1].any()
+
+
+@pytest.mark.parametrize("attn_first", [False, True])
+def test_chains_through_a_stack(attn_first):
+    """parents None in verify and commit of a stack with both kinds of layer is the chain written out."""
+    from rapidllm_b200 import _lib, ops
+    from rapidllm_b200.mixer import MixerStack
+    gen = torch.Generator().manual_seed(45)
+    attn, delta = _weights(gen, 128)
+    B, n = 2, 7
+    kinds = [(_lib.RL_LAYER_FULL_ATTENTION, attn), (_lib.RL_LAYER_LINEAR_ATTENTION, delta)]
+    if not attn_first:
+        kinds.reverse()
+    x = torch.randn(B, n, 128, generator=gen).cuda()
+    chain = (torch.arange(n) - 1).int().expand(B, n).contiguous().cuda()
+    table, base, counts, leaf = _i32([[1, 2], [3, 0]]), _i32([61, 5]), _i32([7, 4]), _i32([5, 3])
+    results = []
+    for parents in (chain, None):
+        stack = MixerStack([k for k, _ in kinds], [w for _, w in kinds], n_pages=4, n_slots=B, n_q=6, n_kv=1, n_k=2, n_v=6)
+        y, pending = stack.verify_tree(x, table, base, parents, counts)
+        taken = stack.commit_tree(pending, table, base, parents, leaf)
+        _lib.check_device()
+        assert taken.tolist() == [6, 4]
+        d, a = stack.layers[attn_first], stack.layers[not attn_first]
+        results.append([y[0], y[1, :4], d.S, d.conv_state, a.k_pool, a.v_pool])
+        with pytest.raises(_lib.RlError):
+            stack.commit_tree(pending[:1], table, base, parents, leaf)
+        with pytest.raises(_lib.RlError):                     # before the first layer has moved
+            stack.commit_tree(pending, table, base, n, leaf)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    with pytest.raises(_lib.RlError):
+        ops.kv_tree_commit(results[0][4], results[0][5], table, base, None, leaf)
