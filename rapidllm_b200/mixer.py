@@ -110,6 +110,8 @@ class DeltaNetMixer:
         rows = x.reshape(B * n, hidden)
         proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in)
         qkv = proj.view(B, n, -1)[..., :cd]                  # read where the projection left it
+        if proj.shape[1] % 4:                                # (odd n_v: rows that 16-byte loads cannot start at)
+            qkv = qkv.contiguous()
         z = proj[:, cd:cd + zd].contiguous()
         beta, g = ops.delta_gates(proj[:, cd + zd:cd + zd + nv].contiguous(), proj[:, cd + zd + nv:].contiguous(),
                                   self.A_log, self.dt_bias)

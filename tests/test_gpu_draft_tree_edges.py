@@ -153,3 +153,23 @@ def test_chains_through_a_stack(attn_first):
         assert torch.equal(a, b)
     with pytest.raises(_lib.RlError):
         ops.kv_tree_commit(results[0][4], results[0][5], table, base, None, leaf)
+
+
+@pytest.mark.parametrize("n_v,n_k", [(3, 1), (5, 5), (2, 1)])
+def test_delta_mixer_with_odd_head_counts(n_v, n_k):
+    """A chain through verify_tree and commit_tree equals decode steps, whatever the row of the projection (a multiple of 4
+    floats or not)."""
+    from rapidllm_b200 import _lib
+    from rapidllm_b200.mixer import DeltaNetMixer
+    torch.backends.cuda.matmul.allow_tf32 = False
+    gen = torch.Generator().manual_seed(46)
+    _, delta = _weights(gen, 128, nk=n_k, nv=n_v)
+    B, n = 2, 5
+    x = torch.randn(B, n, 128, generator=gen).cuda()
+    a, b = (DeltaNetMixer(delta, n_k=n_k, n_v=n_v, n_slots=B) for _ in range(2))
+    y, pending = a.verify_tree(x, None)
+    a.commit_tree(pending, None, _i32([n - 1, n - 1]))
+    want = torch.stack([b.decode(x[:, i].contiguous()) for i in range(n)], 1)
+    _lib.check_device()
+    assert rel_l2(y.cpu(), want.cpu()) <= STATE_REL_L2
+    assert rel_l2(a.S.cpu(), b.S.cpu()) <= STATE_REL_L2 and rel_l2(a.conv_state.cpu(), b.conv_state.cpu()) <= STATE_REL_L2
