@@ -109,7 +109,7 @@ class DeltaNetMixer:
         cd, zd, nv = self.conv_dim, self.zdim, self.n_v
         rows = x.reshape(B * n, hidden)
         proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in)
-        qkv = proj.view(B, n, -1)[..., :cd]                  # read where the projection left it
+        qkv = proj.view(B, n, proj.shape[1])[..., :cd]       # read where the projection left it
         if proj.shape[1] % 4:                                # (odd n_v: rows that 16-byte loads cannot start at)
             qkv = qkv.contiguous()
         z = proj[:, cd:cd + zd].contiguous()
@@ -165,7 +165,7 @@ class GatedAttentionMixer:
         B, n, hidden = x.shape
         qn, kn = self.n_q * self.hd, self.n_kv * self.hd
         rows = x.reshape(B * n, hidden)
-        proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in).view(B, n, -1)
+        proj = _matmul(ops.rmsnorm(rows, self.rms_w, self.eps), self.W_in).view(B, n, self.W_in.shape[0])
         qg = proj[..., :2 * qn].view(B, n, self.n_q, 2 * self.hd)
         k = proj[..., 2 * qn:2 * qn + kn].view(B, n, self.n_kv, self.hd)
         v = proj[..., 2 * qn + kn:].view(B, n, self.n_kv, self.hd)

@@ -173,3 +173,22 @@ def test_delta_mixer_with_odd_head_counts(n_v, n_k):
     _lib.check_device()
     assert rel_l2(y.cpu(), want.cpu()) <= STATE_REL_L2
     assert rel_l2(a.S.cpu(), b.S.cpu()) <= STATE_REL_L2 and rel_l2(a.conv_state.cpu(), b.conv_state.cpu()) <= STATE_REL_L2
+
+
+def test_drafts_of_no_nodes():
+    """A round in which nothing was drafted goes through verify and commit and changes nothing."""
+    from rapidllm_b200 import _lib
+    from rapidllm_b200.mixer import MixerStack
+    gen = torch.Generator().manual_seed(47)
+    attn, delta = _weights(gen, 128)
+    stack = MixerStack([_lib.RL_LAYER_LINEAR_ATTENTION, _lib.RL_LAYER_FULL_ATTENTION], [delta, attn], n_pages=2, n_slots=2, n_q=6,
+                       n_kv=1, n_k=2, n_v=6)
+    table, base = _i32([[0], [1]]), _i32([3, 9])
+    for B, n in ((2, 0), (0, 3)):
+        parents = torch.zeros(B, n, dtype=torch.int32, device="cuda")
+        y, pending = stack.verify_tree(torch.zeros(B, n, 128, device="cuda"), table[:B], base[:B], parents)
+        assert y.shape == (B, n, 128)
+        taken = stack.commit_tree(pending, table[:B], base[:B], parents, _i32([-1] * B))
+        assert taken.tolist() == [0] * B
+    _lib.check_device()
+    assert not stack.layers[0].S.any() and not stack.layers[1].k_pool.any()
