@@ -24,9 +24,10 @@
 // other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
 // to fp16, as the cache's V is; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
 // its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
-// query for an fp16 output is two such terms, the second from shared memory in the place of a third page of the
-// ring: with one, the scores' rounding would show (4.3e-4 relative instead of 2.9e-4).  A bf16 output's own
-// rounding (1.7e-3) hides it, and one term is faster (16 trees of 21 over 16K: 152 us against 177).
+// query is two such terms, whatever the output's type, the second from shared memory in the place of a third page of
+// the ring: an error of the scores is one of the weights, which no rounding of the output hides where values of both
+// signs all but cancel.  It costs a quarter of the time (16 trees of 21 over 16K: 180 us against 154 at burst clocks, 212
+// against 170 sustained), which a caller saves by asking rl_attn_qk_append for 16-bit queries.
 // Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
 // not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
 // rows past the last node are cleared for the same reason.  A drafted V row that is not finite would reach the
@@ -730,8 +731,9 @@ int attn_tree_rows() { return kRows; }
 int attn_tree_max_batch() { return kMaxBatch; }
 
 cudaError_t launch_attn_tree(const AttnTreeArgs& a, cudaStream_t st) {
-    // fp16 and bf16 queries are exact in one fp16 term
-    if (a.q_type == 0 && a.o_type == 1) attn_tree_kernel<true><<<a.grid, kThreads, kSmemBytes, st>>>(a);
+    // One term holds 16-bit queries: the row's largest element is scaled into [2^7, 2^8), so that fp16 elements down to 2^-21
+    // of it (bf16 to 2^-24) are exact and smaller ones off by 2^-32 of it at most.
+    if (a.q_type == 0) attn_tree_kernel<true><<<a.grid, kThreads, kSmemBytes, st>>>(a);
     else attn_tree_kernel<false><<<a.grid, kThreads, kSmemBytes, st>>>(a);
     cudaLaunchConfig_t cfg = {};
     const int row_tiles = (a.max_nodes * (a.n_q / a.n_kv) + kRows - 1) / kRows;

@@ -192,3 +192,26 @@ def test_drafts_of_no_nodes():
         assert taken.tolist() == [0] * B
     _lib.check_device()
     assert not stack.layers[0].S.any() and not stack.layers[1].k_pool.any()
+
+
+@pytest.mark.parametrize("o_type", [torch.float16, torch.bfloat16])
+def test_fp32_queries_keep_their_digits(o_type):
+    """Two tokens of all but equal scores, which meet different halves of the query: one half is 0.98 half steps of fp16
+    above a value of fp16, the other on it.  A query of one fp16 term would lose the difference of the scores, 64 x 0.98 x
+    2^-11, of which the output is a quarter each way (V is 1 and -1).  Two terms of 2^-22 and the sums of 256 products in
+    fp32 leave at most 2^-16 of the score, whatever the output's type."""
+    from rapidllm_b200 import _lib, ops
+    n_q, n_kv, n = 24, 4, 3
+    k, v = torch.zeros(2 + n, n_kv, HD), torch.zeros(2 + n, n_kv, HD)
+    k[0, :, :128], k[1, :, 128:], k[2:] = 1.0, 1.0, -1.0
+    v[0], v[1], v[2:] = 1.0, -1.0, 1.0
+    kp, vp, table = ops.new_pool(2, n_kv), ops.new_pool(2, n_kv), _i32([[1]])
+    ops.kv_append(kp, vp, table[0], k.half().cuda(), v.half().cuda(), pos0=0)
+    q = torch.full((1, n, n_q, HD), 8.0)
+    q[..., :128] *= 1 + 0.98 * 2.0 ** -11
+    got = ops.attn_tree(q.cuda(), kp, vp, table, _i32([2]), out_dtype=o_type)
+    _lib.check_device()
+    o, mag, _ = _attn_exact(q[0], None, (k.half(), v.half()), 2, [-1, 0, 1], n, n_q, n_kv)
+    assert (o > 0.015).all()
+    bound = (2 * math.expm1(64 * 2.0 ** -16) + 2.0 ** -11 + 2.0 ** -15) * mag + HALF_STEP[o_type] * o.abs()
+    assert ((got[0].cpu().double() - o).abs() <= bound).all()
