@@ -22,7 +22,8 @@
 // and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
 // 16 softmax warps in two groups take alternate pages, so that one page's exponentials run under the
 // other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
-// to fp16, as the cache's V is; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
+// to fp16, as the cache's V is and as prefill and decode hold it: an error of 2^-11 of a weight at most, which a sum over many tokens
+// averages; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
 // its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
 // query is two such terms, whatever the output's type, the second from shared memory in the place of a third page of
 // the ring: an error of the scores is one of the weights, which no rounding of the output hides where values of both
@@ -53,6 +54,11 @@ constexpr uint32_t kTmemCols = 512;
 // first 32 columns of its own S, so that the next page's S is computed while this one is exponentiated.
 constexpr uint32_t kColS = 0, kColO = 128, kColQ = 384;
 constexpr float kRescaleThreshold = 8.f;          // log2 units
+// P is held times 2^kWeightLift, the largest weight in [2^kWeightLift, 2^15]: fp16's last step, 2^-24, is then 2^-31 of that
+// weight or less (without the factor tokens of weight e^-17.5 counted as 0, however many).
+// Sums and O carry the same factor, which the division takes out.  A lower threshold leaves room for a larger factor, but
+// every raise waits for O (4 x 64 nodes over 32K sustained: 210 us with 8, 224 with 4, 230 with 2).
+constexpr float kWeightLift = 15.f - kRescaleThreshold;
 constexpr float kNoMax = -1e30f;                   // of a row that has seen nothing; scores are below 2^8 * 65504 * 256
 constexpr int kMaxBatch = 512;
 
@@ -538,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_kernel(AttnTreeArgs a) 
                     for (int i = 0; i < 32; ++i) raw[i] = __float_as_uint(__uint_as_float(raw[i]) - m_new);
                     m_log2 = 0.f;
                 }
+                m_log2 -= kWeightLift;
                 uint32_t ph[16];
                 float lsum0 = 0.f, lsum1 = 0.f;
 #pragma unroll

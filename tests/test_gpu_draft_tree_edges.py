@@ -215,3 +215,26 @@ def test_fp32_queries_keep_their_digits(o_type):
     assert (o > 0.015).all()
     bound = (2 * math.expm1(64 * 2.0 ** -16) + 2.0 ** -11 + 2.0 ** -15) * mag + HALF_STEP[o_type] * o.abs()
     assert ((got[0].cpu().double() - o).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("gap", [12.0, 17.5, 22.0])
+@pytest.mark.parametrize("base,batch,n_kv", [(700, 1, 1), (40000, 1, 1), (3000, 40, 4)])      # the last: a CTA has whole sequences
+def test_many_small_weights_count(gap, base, batch, n_kv):
+    """One token takes all but a little of the weight and has V = 0; the output is what is left for the many others, whose
+    weights e^-gap are below fp16's range for a largest weight of 1 (2^-17, 2^-25, 2^-32).  Weights are held as fp16 under a
+    scale of at least 2^7, an absolute error of 2^-32 of the largest each."""
+    from rapidllm_b200 import _lib, ops
+    n_q, n = 6 * n_kv, 2
+    k, v = torch.zeros(base + n, n_kv, HD), torch.ones(base + n, n_kv, HD)
+    k[base // 3] = gap / 16
+    v[base // 3] = 0.0
+    pages = (base + n + 63) // 64
+    kp, vp = ops.new_pool(pages, n_kv), ops.new_pool(pages, n_kv)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0).repeat(batch, 1)     # one cache, many drafts
+    ops.kv_append(kp, vp, table[0], k.half().cuda(), v.half().cuda(), pos0=0)
+    q = torch.ones(batch, n, n_q, HD, dtype=torch.float16)
+    got = ops.attn_tree(q.cuda(), kp, vp, table, _i32([base] * batch))
+    _lib.check_device()
+    o, mag, _ = _attn_exact(q[0], None, (k.half(), v.half()), base, [-1, 0], n, n_q, n_kv)
+    bound = (2.0 ** -11 + 2.0 ** -15) * mag + base * 2.0 ** -32 + HALF_STEP[torch.float16] * o + 2.0 ** -25
+    assert ((got.cpu().double() - o).abs() <= bound).all(), (got[0, 0, 0, 0].item(), o[0, 0, 0].item())
