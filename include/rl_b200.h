@@ -439,13 +439,15 @@ typedef struct rl_attn_qk_append_params {
     float theta, eps;            /* 1e7, 1e-6 */
     long long qg_stride, k_stride, v_stride;   /* floats between rows (0 = dense), multiples of 4: q | gate, k
                                                 * and v may be column ranges of one projection */
+    int angle_f32;               /* 0: the rotation's angle in 64 bits; else the fp32 product of rl_attn_qk_prepare */
 } rl_attn_qk_append_params;
 
 /* rl_attn_qk_prepare and rl_kv_append in one pass over the projections: q/gate split, head RMSNorm
  * (1 + gamma) of q and k, rotation of the first rotary_dim dims, K and V rows (fp16, round to nearest
  * even) into the paged F16 cache at positions pos[b] + t.  Row t of sequence b is rotated by pos[b] + t,
  * or, with parents (n_tok <= 64), by pos[b] + depth of node t.  The rotation's angle is formed in 64 bits
- * (rl_attn_qk_prepare follows the reference's fp32 angle, which is 4e-3 rad off at position 100 000).
+ * (rl_attn_qk_prepare follows the reference's fp32 angle, which is 4e-3 rad off at position 100 000); in a cache that
+ * rl_attn_qk_prepare's rows share, angle_f32 makes q, K and V those of rl_attn_qk_prepare and rl_kv_append bit for bit.
  *   qg fp32 [batch * n_tok] rows of [n_q][2 * 256] ([q | gate] per head); k, v fp32 rows of [n_kv][256]
  *   q_norm, k_norm fp32 [256] or NULL;  q_out [batch * n_tok][n_q][256] of q_type
  *   gate_out fp32 [batch * n_tok][n_q][256], or NULL: not copied (rl_attn_tree reads it in place)

@@ -76,7 +76,8 @@ class AttnQkPrepareParams(C.Structure):
 class AttnQkAppendParams(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_q", "n_kv", "head_dim", "rotary_dim", "batch", "n_tok", "page_tokens", "n_pages",
                                        "max_pages_per_seq", "q_type")] + [
-        ("theta", C.c_float), ("eps", C.c_float)] + [(n, C.c_longlong) for n in ("qg_stride", "k_stride", "v_stride")]
+        ("theta", C.c_float), ("eps", C.c_float)] + [(n, C.c_longlong) for n in ("qg_stride", "k_stride", "v_stride")] + [
+        ("angle_f32", C.c_int)]
 
 
 class AttnTreeParams(C.Structure):

@@ -1492,7 +1492,9 @@ int rl_attn_qk_append(void* k_pool, void* v_pool, const int32_t* page_table, con
     a.q_type = p->q_type;
     a.eps = p->eps;
     const int pairs = p->rotary_dim / 2;
-    for (int i = 0; i < pairs; ++i) a.inv_turn[i] = pow(double(p->theta), -double(i) / pairs) / 6.283185307179586476925;
+    for (int i = 0; i < pairs; ++i)
+        a.rate[i] = p->angle_f32 ? double(1.f / powf(p->theta, float(i) / float(pairs))) : pow(double(p->theta), -double(i) / pairs) / 6.283185307179586476925;
+    a.angle_f32 = p->angle_f32;
     rl::launch_attn_qk_append(a, p->batch, as_stream(stream));
     RL_CUDA(cudaGetLastError());
     return RL_OK;

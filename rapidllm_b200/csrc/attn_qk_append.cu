@@ -9,7 +9,8 @@
 // What attn_qk_prepare and kv_append do in two passes with k going out to memory and back; here k
 // leaves the registers as the fp16 row of its page.  The angle is formed in 64 bits, as a fraction of
 // a turn: at position 100 000 the fp32 product of position and frequency is 4e-3 rad off, more than
-// the rounding of K to fp16.
+// the rounding of K to fp16.  In a cache whose other rows attn_qk_prepare rotated, angle_f32 takes its fp32
+// product instead: q, K and V are then those of attn_qk_prepare and kv_append bit for bit.
 //
 // Bound by bandwidth (a row of 24 + 4 heads reads 57 KB and writes 16 to 52 KB).  A warp takes one
 // row of one head, 8 consecutive dims per lane, so that every load and store is 16 bytes wide and
@@ -25,7 +26,7 @@ namespace {
 
 constexpr int kWarps = 8;
 
-__device__ __forceinline__ float sum_warp(float v) {
+__device__ __forceinline__ double sum_warp(double v) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
@@ -91,18 +92,23 @@ __global__ void __launch_bounds__(kWarps * 32) attn_qk_append_kernel(AttnQkAppen
             depth = __popcll(tree::of_node(w.lo, w.hi, t)) - 1;
         }
         for (int i = lane; i < pairs; i += 32) {
-            const double turns = (double(base) + depth) * a.inv_turn[i];
-            float s, c;
-            sincospif(2.f * float(turns - rint(turns)), &s, &c);
-            turn[i] = make_float2(c, s);
+            if (a.angle_f32) {
+                const float angle = float((long long)base + depth) * float(a.rate[i]);
+                turn[i] = make_float2(cosf(angle), sinf(angle));
+            } else {
+                const double turns = (double(base) + depth) * a.rate[i];
+                float s, c;
+                sincospif(2.f * float(turns - rint(turns)), &s, &c);
+                turn[i] = make_float2(c, s);
+            }
         }
     }
     __syncthreads();
     if (is_q || is_k) {
-        float ss = 0.f;
+        double ss = 0.0;                                      // as attn_qk_prepare sums (in 32 bits a prompt of 4 096 rows takes 74.1 us, so 75.6)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x.v[e], x.v[e], ss);
-        const float inv = 1.f / sqrtf(sum_warp(ss) * (1.f / kHeadDim) + a.eps);
+        for (int e = 0; e < 8; ++e) ss = fma(double(x.v[e]), double(x.v[e]), ss);
+        const float inv = 1.f / sqrtf(float(sum_warp(ss) / kHeadDim) + a.eps);
         const float* gamma = is_q ? a.q_norm : a.k_norm;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x.v[e] *= inv;
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_qk_append_kernel(AttnQkAppen
             const float y = __shfl_sync(0xffffffffu, x.v[e], partner);
             if (low || high) {
                 const float2 cs = turn[(low ? d : d - pairs) + e];
-                x.v[e] = low ? x.v[e] * cs.x - y * cs.y : x.v[e] * cs.x + y * cs.y;
+                x.v[e] = fmaf(x.v[e], cs.x, low ? -(y * cs.y) : y * cs.y);     // the roundings of attn_qk_prepare
             }
         }
     }

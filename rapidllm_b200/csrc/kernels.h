@@ -293,8 +293,9 @@ struct AttnQkAppendArgs {
     int* err;
     size_t qg_stride, k_stride, v_stride;
     int n_q, n_kv, n_tok, n_pages, max_pages_per_seq, rotary_dim, q_type;    // q_type: 0 fp32, 1 fp16, 2 bf16
+    int angle_f32;
     float eps;
-    double inv_turn[256 / 2];   // turns of pair i per position: theta^(-i / pairs) / (2 pi)
+    double rate[256 / 2];       // of pair i per position: turns theta^(-i / pairs) / (2 pi), with angle_f32 radians in fp32
 };
 void launch_attn_qk_append(const AttnQkAppendArgs& a, int batch, cudaStream_t st);
 

@@ -475,13 +475,15 @@ def _pools(k_pool, v_pool, page_table, batch, dev):
 
 
 def attn_qk_append(qg, k, v, k_pool, v_pool, page_table, pos, q_norm=None, k_norm=None, parents=None, n_nodes=None,
-                   rotary_dim=64, theta=1e7, eps=1e-6, q_dtype=torch.float32, want_gate=True, q_out=None, gate_out=None):
+                   rotary_dim=64, theta=1e7, eps=1e-6, q_dtype=torch.float32, want_gate=True, q_out=None, gate_out=None,
+                   angle_f32=False):
     """From the projections to the operands of the attention in one pass: q/gate split, head RMSNorm
     (1 + gamma), rotation, K and V rows into the paged F16 cache at pos[b] + t.
 
     qg fp32 [batch][n_tok][n_q][512] ([q | gate] per head), k, v fp32 [batch][n_tok][n_kv][256], column
     ranges of one projection or dense; pos int32 [batch].  Row t is rotated by pos[b] + t, with parents
-    [batch][n_tok] (n_tok <= 64) by pos[b] + the node's depth.  Returns q of q_dtype (or of q_out) and the
+    [batch][n_tok] (n_tok <= 64) by pos[b] + the node's depth; the angle is formed in 64 bits, or with angle_f32 as
+    attn_qk_prepare forms it (for a cache that holds its rows too).  Returns q of q_dtype (or of q_out) and the
     gate, None without want_gate.  Rows behind n_nodes[b] are left as they are."""
     dev = torch.cuda.current_device()
     batch, n_tok, n_q, two_hd = qg.shape
@@ -501,7 +503,7 @@ def attn_qk_append(qg, k, v, k_pool, v_pool, page_table, pos, q_norm=None, k_nor
     elif gate_out is None:
         gate_out = torch.empty(shape, dtype=_F32, device=qg.device)
     p = _lib.AttnQkAppendParams(n_q, n_kv, HEAD_DIM, rotary_dim, batch, n_tok, PAGE_TOKENS, n_pages, pages,
-                                _TYPES[q_out.dtype], theta, eps, qg_row, k_row, v_row)
+                                _TYPES[q_out.dtype], theta, eps, qg_row, k_row, v_row, angle_f32)
     check(lib().rl_attn_qk_append(kp, vp, table, _needed(pos, _I32, (batch,), dev, "pos"),
                                   _arg(parents, _I32, (batch, n_tok), dev, "parents"), _arg(n_nodes, _I32, (batch,), dev, "n_nodes"),
                                   qg_p, k_p, v_p, _arg(q_norm, _F32, (HEAD_DIM,), dev, "q_norm"),

@@ -238,3 +238,60 @@ def test_many_small_weights_count(gap, base, batch, n_kv):
     o, mag, _ = _attn_exact(q[0], None, (k.half(), v.half()), base, [-1, 0], n, n_q, n_kv)
     bound = (2.0 ** -11 + 2.0 ** -15) * mag + base * 2.0 ** -32 + HALF_STEP[torch.float16] * o + 2.0 ** -25
     assert ((got.cpu().double() - o).abs() <= bound).all(), (got[0, 0, 0, 0].item(), o[0, 0, 0].item())
+
+
+@pytest.mark.parametrize("rot", [64, 256])
+def test_append_can_rotate_as_qk_prepare_does(rot):
+    """With angle_f32, q, K and V are those of attn_qk_prepare and kv_append at any position, bit for bit: the same sum of
+    the norm, the same angle, the same roundings."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(48)
+    pos, n, n_q, n_kv = [0, 63, 130001, 16777300], 6, 12, 2
+    B = len(pos)
+    table = torch.full((B, max(pos) // 64 + 2), -1, dtype=torch.int32)
+    for b, p in enumerate(pos):
+        table[b, p // 64], table[b, p // 64 + 1] = 2 * b, 2 * b + 1
+    table = table.cuda()
+    qg, k, v = (torch.randn(B, n, h, d, generator=gen).cuda() for h, d in ((n_q, 512), (n_kv, HD), (n_kv, HD)))
+    qn, kn = (0.2 * torch.randn(HD, generator=gen).cuda() for _ in range(2))
+    pools = [ops.new_pool(2 * B, n_kv) for _ in range(4)]
+    q, gate = ops.attn_qk_append(qg, k, v, *pools[:2], table, _i32(pos), qn, kn, rotary_dim=rot, angle_f32=True)
+    at = (_i32(pos).unsqueeze(1) + torch.arange(n, dtype=torch.int32, device="cuda")).reshape(-1).contiguous()
+    rotated = k.reshape(B * n, n_kv, HD).clone()
+    want, want_gate = ops.attn_qk_prepare(qg.reshape(B * n, n_q, 512), rotated, qn, kn, pos=at, rotary_dim=rot)
+    for b, p in enumerate(pos):
+        ops.kv_append(*pools[2:], table[b], rotated.view(B, n, n_kv, HD)[b].contiguous(), v[b].contiguous(), pos0=p)
+    _lib.check_device()
+    assert torch.equal(gate.view_as(want_gate), want_gate) and torch.equal(q.view_as(want), want)
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+
+
+def test_attention_mixer_far_into_a_context():
+    """A chain through verify_tree behind 100 003 tokens writes the cache rows of as many decode steps and gives their
+    outputs: queries of 16 times the usual norm, so that scores spread over +- 50 and their rounding counts (P and the
+    output in fp16, 2^-11 each, remain).  The rows differ by what the projections do, whose GEMMs have another number of
+    rows: sums of 128 products in another order, 2 x 128 x 2^-24 of magnitudes that are 5 times the sum, 1e-4 of a row's
+    root mean square, and the step of fp16 that this may move (an angle of another rule, 4e-3 rad, is far above)."""
+    from rapidllm_b200 import _lib
+    from rapidllm_b200.mixer import GatedAttentionMixer
+    torch.backends.cuda.matmul.allow_tf32 = False
+    gen = torch.Generator().manual_seed(49)
+    weights, _ = _weights(gen, 128)
+    weights["q_norm"] = torch.full((HD,), 15.0)
+    base, n = 100003, 5
+    pages = (base + n + 63) // 64
+    table = torch.randperm(pages, generator=gen).int().view(1, -1).cuda()
+    x = torch.randn(1, n, 128, generator=gen).cuda()
+    mixers = [GatedAttentionMixer(weights, n_pages=pages, n_q=6, n_kv=1) for _ in range(2)]
+    for m in mixers:
+        fill = torch.Generator(device="cuda").manual_seed(50)
+        for pool in (m.k_pool, m.v_pool):
+            pool.copy_(torch.randn(pool.shape, generator=fill, device="cuda"))
+    y = mixers[0].verify_tree(x, table, _i32([base]), None)
+    want = torch.stack([mixers[1].decode(x[:, i].contiguous(), table, _i32([base + i])) for i in range(n)], 1)
+    _lib.check_device()
+    for a, b in zip(*([m.k_pool, m.v_pool] for m in mixers)):
+        for i in range(n):
+            got, ref = (_pool_row(p, table, 0, base + i).float() for p in (a, b))
+            assert ((got - ref).abs() <= 2.0 ** -10 * ref.abs() + 1e-4 * ref.square().mean().sqrt()).all(), i
+    assert rel_l2((y - x).cpu(), (want - x).cpu()) <= 2.0 ** -8
