@@ -161,8 +161,8 @@ class GatedAttentionMixer:
     def verify_tree(self, x, page_table, base_len, parents, n_nodes=None):
         """Every node of a draft tree: x fp32 [batch][nodes][hidden] -> the nodes' new hidden states.  Node i's K and V
         go to cache position base_len[b] + i (int32 [batch], the committed tokens); commit_tree moves one path's
-        rows together.  From the same projection the cache rows are those of decode bit for bit; the
-        query meets the tensor cores as fp16, as K does."""
+        rows together.  From the same projection, queries and cache rows are those of decode bit
+        for bit."""
         B, n, hidden = x.shape
         qn, kn = self.n_q * self.hd, self.n_kv * self.hd
         rows = x.reshape(B * n, hidden)
@@ -172,7 +172,7 @@ class GatedAttentionMixer:
         v = proj[..., 2 * qn + kn:].view(B, n, self.n_kv, self.hd)
         q, _ = ops.attn_qk_append(qg, k, v, self.k_pool, self.v_pool, page_table, base_len, self.q_norm, self.k_norm,
                                   parents=parents, n_nodes=n_nodes, rotary_dim=self.rotary_dim, theta=self.theta,
-                                  eps=self.eps, q_dtype=torch.float16, want_gate=False, angle_f32=True)
+                                  eps=self.eps, want_gate=False, angle_f32=True)
         o = ops.attn_tree(q, self.k_pool, self.v_pool, page_table, base_len, parents, n_nodes=n_nodes, gate=qg[..., self.hd:])
         return (rows + _matmul(o.view(B * n, qn), self.W_out)).view(B, n, hidden)
 
