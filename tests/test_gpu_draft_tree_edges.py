@@ -13,6 +13,32 @@ from test_gpu_draft_tree import (DK, HALF_STEP, HD, _attn_exact, _gdn_exact, _gd
 pytestmark = pytest.mark.gpu
 
 
+def _gdn_tree_exact(S, win, qkv, w, beta, g, parents, n, n_qk, tiled):
+    """o of the first n nodes of one sequence in 64 bits on the device, each node from its parent's state and window."""
+    n_v, qd = S.shape[0], n_qk * DK
+    hs = torch.tensor([h % n_qk if tiled else h // (n_v // n_qk) for h in range(n_v)], device="cuda")
+    S, win, w, qkv, beta, g = (t.cuda().double() for t in (S, win, w, qkv, beta, g))
+    at, out = {-1: (S, win)}, []
+    for i in range(n):
+        state, window = at[parents[i]]
+        window = torch.cat([window[:, 1:], qkv[i].unsqueeze(1)], 1)
+        y = (window * w).sum(1)
+        y = y / (1 + torch.exp(-y))
+        q, k, v = y[:qd].view(-1, DK)[hs], y[qd:2 * qd].view(-1, DK)[hs], y[2 * qd:].view(-1, DK)
+        q = q / (q.square().sum(1, keepdim=True) + 1e-6).sqrt() / DK ** 0.5
+        k = k / (k.square().sum(1, keepdim=True) + 1e-6).sqrt()
+        state = state * g[i].exp().view(-1, 1, 1)
+        state = state + k.unsqueeze(2) * (beta[i].unsqueeze(1) * (v - (k.unsqueeze(2) * state).sum(1))).unsqueeze(1)
+        at[i] = state, window
+        out.append((q.unsqueeze(2) * state).sum(1))
+    return torch.stack(out).cpu() if out else None
+
+
+def _full_batch(n_v):
+    """Sequences at which the value heads of a key head share a CTA of gdn_tree: more than two heads per SM."""
+    return 2 * torch.cuda.get_device_properties(0).multi_processor_count // n_v + 1
+
+
 def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
 
@@ -295,3 +321,87 @@ def test_attention_mixer_far_into_a_context():
             got, ref = (_pool_row(p, table, 0, base + i).float() for p in (a, b))
             assert ((got - ref).abs() <= 2.0 ** -10 * ref.abs() + 1e-4 * ref.square().mean().sqrt()).all(), i
     assert rel_l2((y - x).cpu(), (want - x).cpu()) <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("n_v,n_qk,tiled,nodes,width", [
+    (48, 16, False, 13, 3), (48, 16, True, 16, 1), (48, 16, False, 21, 4), (32, 16, True, 32, 6), (48, 16, False, 40, 3),
+    (64, 16, True, 48, 8), (48, 16, False, 64, 1), (48, 16, True, 63, 5), (64, 64, False, 20, 2),
+])
+def test_gdn_tree_of_a_full_batch(n_v, n_qk, tiled, nodes, width):
+    """Value heads one after the other in a CTA (every size of the kernel, both orders of heads): ragged counts, an empty
+    draft and one of a single node among them."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(nodes * 10 + n_v + tiled)
+    batch = _full_batch(n_v)
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, batch, nodes, n_v, n_qk, batch)
+    parents = _tree(gen, batch, nodes, width)
+    counts = [max(1, nodes - 5 * b) for b in range(batch)]
+    counts[1], counts[2] = 0, 1
+    out = torch.full((batch, nodes, n_v, DK), 5.0, device="cuda")
+    ops.gdn_tree(*(t.cuda() for t in (S, win)), None, *(t.cuda() for t in (qkv, w, beta, g, parents)), n_qk, n_nodes=_i32(counts),
+                 head_map=_lib.RL_HEADS_TILED if tiled else _lib.RL_HEADS_GROUPED, out=out)
+    _lib.check_device()
+    for b in range(batch):
+        assert (out[b, counts[b]:] == 5.0).all()
+        if counts[b]:
+            want = _gdn_tree_exact(S[b], win[b], qkv[b], w, beta[b], g[b], parents[b].tolist(), counts[b], n_qk, tiled)
+            got = out[b, :counts[b]].cpu()
+            for h in range(n_v):
+                assert rel_l2(got[:, h], want[:, h]) <= STATE_REL_L2, (b, h)
+
+
+@pytest.mark.parametrize("n_v,n_qk,tiled,nodes", [(48, 16, False, 14), (48, 16, True, 30), (48, 16, False, 45), (32, 16, False, 64)])
+def test_gdn_tree_bad_nodes_and_closed_gates_of_a_full_batch(n_v, n_qk, tiled, nodes):
+    """In every head of a CTA, the first and the later ones: inputs that are not finite reach their node's descendants in
+    the heads concerned alone, and gates that forget everything cost no digits behind them."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(51)
+    batch, ratio = _full_batch(n_v), n_v // n_qk
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, batch, nodes, n_v, n_qk, batch)
+    parents = _tree(gen, batch, nodes, 6)
+    heads = [h for h in range(n_v) if (h % n_qk if tiled else h // ratio) == 2]       # those of key head 2, in a CTA's order
+    qkv[0, 5, 2 * DK + 3] = math.inf                          # q of key head 2
+    qkv[1, 7, n_qk * DK + 2 * DK + 9] = math.nan              # its k
+    for z, h in enumerate(heads):
+        qkv[2, 3 + z, 2 * n_qk * DK + h * DK + 17 * z] = math.nan                     # a column of each value head
+        beta[3, 4 + z, h] = math.nan
+        g[3, 8 + z, h] = math.inf
+        g[4, 1 + 2 * z::5, h] = (-60.0, -5000.0, -math.inf, -90.0)[z]
+    o = ops.gdn_tree(*(t.cuda() for t in (S, win)), None, *(t.cuda() for t in (qkv, w, beta, g, parents)), n_qk,
+                     head_map=_lib.RL_HEADS_TILED if tiled else _lib.RL_HEADS_GROUPED).cpu()
+    _lib.check_device()
+    for b in range(batch):
+        want = _gdn_tree_exact(S[b], win[b], qkv[b], w, beta[b], g[b], parents[b].tolist(), nodes, n_qk, tiled)
+        fine = torch.isfinite(want)
+        assert fine.all() == (b > 3) and torch.equal(torch.isfinite(o[b]), fine), b
+        for h in range(n_v):
+            assert rel_l2(o[b, :, h][fine[:, h]], want[:, h][fine[:, h]]) <= STATE_REL_L2, (b, h)
+
+
+@pytest.mark.parametrize("up", [10, 20])
+@pytest.mark.parametrize("full", [False, True])
+def test_gdn_tree_of_siblings_of_unequal_size(up, full):
+    """One sibling's v 2^up times the others'.  A value is held to 2^-22 of itself or 2^-39 of the largest of its column (two
+    fp16 terms under one scale), twice: in W and in U.  With 2^20 that is 2 x 2^-19 = 4e-6 of the others' v, within the
+    tolerance of a node's whole output; their outputs are of v's size, since the state is small here."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(52)
+    n_v, n_qk, nodes = (48, 16, 24) if full else (6, 2, 24)
+    batch = _full_batch(n_v) if full else 2
+    S, win, qkv, w, beta, g = _gdn_inputs(gen, batch, nodes, n_v, n_qk, batch)
+    S *= 0.1
+    parents = torch.full((batch, nodes), -1, dtype=torch.int32)
+    parents[:, 12:] = torch.arange(12).int()                  # twelve roots, a child each
+    v0 = 2 * n_qk * DK
+    qkv[:, 4, v0:] = qkv[:, 4, v0:].abs() * 2.0 ** up         # (SiLU takes large positive values as they are)
+    w[v0:] = w[v0:].abs()
+    qkv[:, 16, v0:] = qkv[:, 3, v0:]
+    o = ops.gdn_tree(*(t.cuda() for t in (S, win)), None, *(t.cuda() for t in (qkv, w, beta, g, parents)), n_qk).cpu()
+    _lib.check_device()
+    for b in range(batch):
+        want = _gdn_tree_exact(S[b], win[b], qkv[b], w, beta[b], g[b], parents[b].tolist(), nodes, n_qk, False)
+        small = [i for i in range(nodes) if i not in (4, 16)]
+        assert want[4].abs().mean() > 2.0 ** (up - 4) * want[small].abs().mean()
+        for h in range(n_v):
+            assert rel_l2(o[b, small, h], want[small, h]) <= STATE_REL_L2, (b, h)
+            assert rel_l2(o[b, [4, 16], h], want[[4, 16], h]) <= STATE_REL_L2, (b, h)
