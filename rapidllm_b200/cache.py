@@ -90,6 +90,11 @@ class HybridCache:
     def conv(self, i):
         return _view(lib().rl_cache_conv(self._h, i), (self.n_slots, self.conv_dim, self.conv_k), torch.float32)
 
+    def conv_phase(self, i):
+        """Ring positions of layer i's conv windows, int32 [n_slots]: what conv(i) is read with (ops.gdn_decode,
+        ops.gdn_tree, ops.gdn_tree_commit)."""
+        return _view(lib().rl_cache_conv_phase(self._h, i), (self.n_slots,), torch.int32)
+
     def conv_windows(self, i):
         """The conv windows of DeltaNet layer i in the reference's form [n_slots][conv_dim][4], oldest
         tap first (a copy: the cache keeps them as rings, see rl_gdn_decode)."""

@@ -405,3 +405,68 @@ def test_gdn_tree_of_siblings_of_unequal_size(up, full):
         for h in range(n_v):
             assert rel_l2(o[b, small, h], want[small, h]) <= STATE_REL_L2, (b, h)
             assert rel_l2(o[b, [4, 16], h], want[[4, 16], h]) <= STATE_REL_L2, (b, h)
+
+
+def test_a_tree_on_the_device_cache():
+    """Pools, states, conv rings and their phases of a HybridCache: a tree verified and one path committed through its views
+    equal the cache's own decode steps along that path, and the next decode step goes on from there."""
+    from rapidllm_b200 import _lib, ops
+    from rapidllm_b200.cache import HybridCache
+    gen = torch.Generator().manual_seed(53)
+    kinds = [_lib.RL_LAYER_LINEAR_ATTENTION, _lib.RL_LAYER_FULL_ATTENTION]
+    B, n, history, lens = 2, 9, 3, [60, 130]
+    cache = HybridCache(kinds, n_pages=6, n_slots=3, max_batch=2, max_pages_per_seq=3)
+    table, slots = _i32([[4, 0, -1], [2, 5, 1]]), _i32([2, 0])
+    sh = cache.io_shapes(B)
+    conv_w = torch.randn(sh["conv_w"], generator=gen).cuda() * 0.5
+    parents = _tree(gen, 1, n, 3).repeat(B, 1)
+    path = _path(parents[0].tolist(), n - 1)
+
+    def token():
+        t = {x: torch.randn(sh[x], generator=gen).cuda() for x in ("attn_q", "attn_gate", "attn_k", "attn_v", "delta_qkv")}
+        t["delta_beta"] = torch.sigmoid(torch.randn(sh["delta_beta"], generator=gen)).cuda()
+        t["delta_g"] = -0.3 * torch.rand(sh["delta_g"], generator=gen).cuda()
+        return t
+
+    def step(t, at):
+        io = dict(t, attn_o=torch.zeros(sh["attn_o"], device="cuda"), delta_o=torch.zeros(sh["delta_o"], device="cuda"),
+                  conv_w=conv_w, page_table=table, slot_ids=slots, pos=_i32(at))
+        cache.decode(io, B)
+        torch.cuda.synchronize()
+        return io["attn_o"][0].clone(), io["delta_o"][0].clone()
+
+    for pool in (cache.k_pool(0), cache.v_pool(0)):
+        pool.copy_(torch.randn(pool.shape, generator=gen))
+    for d in range(history):                                  # the rings' phases leave 0
+        step(token(), [x + d for x in lens])
+    base = [x + history for x in lens]
+    views = [cache.k_pool(0), cache.v_pool(0), cache.state(0), cache.conv(0), cache.conv_phase(0)]
+    kept = [v.clone() for v in views]
+    assert views[4][slots.long()].tolist() == [history % 4] * B
+    nodes, nxt = [token() for _ in range(n)], token()
+    want = [step(nodes[i], [x + d for x in base]) for d, i in enumerate(path)]
+    after = [cache.state(0).clone(), cache.conv_windows(0)]
+    want_next = step(nxt, [x + len(path) for x in base])
+    for v, was in zip(views, kept):
+        v.copy_(was)
+
+    rows = lambda x: torch.stack([t[x][0] for t in nodes], 1).contiguous()  # noqa: E731
+    k, v = rows("attn_k"), rows("attn_v")
+    for b in range(B):
+        ops.kv_append(*views[:2], table[b], k[b], v[b], pos0=base[b])
+    o = ops.attn_tree(rows("attn_q"), *views[:2], table, _i32(base), parents.cuda(), gate=rows("attn_gate"))
+    gdn = (*views[2:], rows("delta_qkv"), conv_w[0], rows("delta_beta"), rows("delta_g"), parents.cuda())
+    do = ops.gdn_tree(*gdn, n_qk=16, slot_ids=slots)
+    leaf = _i32([n - 1] * B)
+    taken = ops.kv_tree_commit(*views[:2], table, _i32(base), parents.cuda(), leaf)
+    ops.gdn_tree_commit(*gdn, leaf, n_qk=16, slot_ids=slots)
+    _lib.check_device()
+    assert taken.tolist() == [len(path)] * B
+    for d, i in enumerate(path):
+        assert rel_l2(o[:, i].float().cpu(), want[d][0].cpu()) <= 1e-3
+        assert rel_l2(do[:, i].cpu(), want[d][1].cpu()) <= STATE_REL_L2
+    assert rel_l2(cache.state(0).cpu(), after[0].cpu()) <= STATE_REL_L2
+    assert torch.equal(cache.conv_windows(0), after[1])
+    got = step(nxt, [x + len(path) for x in base])
+    assert rel_l2(got[0].cpu(), want_next[0].cpu()) <= 1e-3 and rel_l2(got[1].cpu(), want_next[1].cpu()) <= STATE_REL_L2
+    cache.close()
