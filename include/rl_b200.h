@@ -459,7 +459,7 @@ int rl_attn_qk_append(void* k_pool, void* v_pool, const int32_t* page_table, con
 
 typedef struct rl_attn_tree_params {
     int n_q, n_kv, head_dim;     /* 24, 4, 256; n_q / n_kv <= 8 */
-    int batch, max_nodes;        /* sequences, rows per sequence in q and o (<= 64) */
+    int batch, max_nodes;        /* sequences (<= 512), rows per sequence in q and o (<= 64) */
     int page_tokens, n_pages, max_pages_per_seq;
     int max_seq_len;             /* host-side upper bound of every base_len[b] + n_nodes[b] */
     int q_type;                  /* RL_TYPE_* of q */
@@ -476,7 +476,8 @@ size_t rl_attn_tree_workspace_bytes(const rl_attn_tree_params* p);
  *   q [batch][max_nodes][n_q][256];  gate fp32, element (row, head, d) at row * gate_row + head * gate_head + d;
  *     q, o and workspace 32-byte aligned
  *   o [batch][max_nodes][n_q][256] in 16 bits: a mean of fp16 values times a gate in (0, 1), it fits fp16,
- *     and the probabilities meet V as fp16, so 32 bits would carry no more
+ *     and the probabilities meet V as fp16, so 32 bits would carry no more.  fp32 queries keep 22 bits of a row's largest
+ *     element for either output type; 16-bit ones are faster (by a fifth over long caches)
  * What a row does not see has no part in it, whatever it holds; a drafted V row that is not finite makes the
  * whole output row of the nodes and heads that see it NaN.  A sequence longer than max_seq_len is recorded
  * (rl_device_error) and left out.  Calls that may overlap need workspaces of their own.  Reads only the F16
@@ -519,7 +520,8 @@ typedef struct rl_gdn_tree_params {
  *   o   fp32 [batch][max_nodes][n_v][128]
  * beta in [0, 2] and g_log <= 0 as the gates give them (the coefficients between nodes are held in a fixed range).
  * Inputs of a node that are not finite (g_log = -inf is a closed gate) reach its descendants alone.  The nodes'
- * values share a scale per column: one 2^k above its siblings' leaves those k fewer than 22 bits.
+ * values share a scale per column of the state: each is held to 2^-22 of itself or 2^-39 of the column's largest, so that
+ * one 2^17 times its siblings costs them nothing and one of 2^(17 + k) leaves them k fewer than 22 bits.
  * workspace: rl_gdn_tree_workspace_bytes() bytes, 16-byte aligned, for the rows after the conv; calls that may
  * overlap need workspaces of their own. */
 size_t rl_gdn_tree_workspace_bytes(const rl_gdn_tree_params* p);

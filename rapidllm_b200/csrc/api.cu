@@ -1523,9 +1523,8 @@ static int attn_tree_check(const rl_attn_tree_params* p) {
 // tokens take 15.3 us with 1 page, 14.8 with 2, 16.2 with 3, 16.5 with 4 (more CTAs leave more partials to merge).
 static const int kTreeMinShare = knob("RL_B200_TREE_MIN_SHARE", 2);
 // What a CTA pays to close one (sequence, head, row tile) and open the next (partial out, queries in, behind the pages
-// already requested), in pages.  16 trees of 21 over 16K: 159.8 us with 8, 157.0 with 12, 153.2 with 16, 151.7 with 20 in
-// short runs, 174.2 with 16 and 177.1 with 20 in long ones; 4 trees of 64 over 32K: 182.5, 189.4, 187.1, 178.8 (+- 5) and
-// 211.5, 214.2.
+// already requested), in pages.  Sustained, with 8, 12, 16 and 24: 16 trees of 21 over 16K (16-bit queries) 179, 173, 171 and
+// 177 us, over 2 000 tokens 50.7, 48.0, 49.3 and 53.2, 4 trees of 64 over 32K 217, 213, 214 and 218 (+- 2).
 static const int kTreeBoundary = knob("RL_B200_TREE_BOUNDARY", 16);
 struct AttnTreePlan {
     int grid;

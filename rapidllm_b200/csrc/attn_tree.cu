@@ -5,9 +5,12 @@
 //
 // All query rows of a KV head -- (node, query head of the group) pairs, up to 64 x 8 -- share its K and V,
 // so the 128 rows of an MMA tile are such pairs and a sequence's pages are read once per 128 rows (at 24 / 4
-// heads: once for up to 21 nodes).  Up to there the cache's bandwidth is the bound (16 trees of 21 over 16K: 779 MB
-// in 151 us, boundaries included), beyond it the pages' way into each SM (4 trees of 64 over 32K: 187 us, tensor pipe
-// 41 % busy).
+// heads: once for up to 21 nodes).  Up to there the cache's bandwidth is the bound (16 trees of 21 over 16K, 16-bit
+// queries: 779 MB in 151 us at burst clocks, boundaries included; 171 us a call sustained).  Beyond it no unit is (4 trees
+// of 64 over 32K: 189 us at burst clocks, 212 a call sustained; HBM 32 % busy, L2 26 %, tensor pipe 42 %, issue slots 33 %):
+// a page's time is the chain S -> tensor-memory loads -> exponentials -> P -> P V with two pages in it, S being
+// M 128 x N 64 products of about 45 clocks instead of 32; half of the warps' waits are for loads.  The 16 softmax warps
+// have 96 registers a thread and spill (288 bytes of stores a thread, 494 with fp32 queries), about as the prefill kernel.
 //
 // Work division: the (sequence, KV head, row tile, page) units of the whole batch form one list, computed on
 // the device from base_len and n_nodes (a captured step may advance them), and every CTA of a persistent
@@ -22,8 +25,9 @@
 // and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
 // 16 softmax warps in two groups take alternate pages, so that one page's exponentials run under the
 // other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
-// to fp16, as the cache's V is and as prefill and decode hold it: an error of 2^-11 of a weight at most, which a sum over many tokens
-// averages; sums, maxima and O are fp32.  Q is scaled per row by a power of two before
+// to fp16, as the cache's V is and as prefill and decode hold it: 2^-11 of a weight at most, which a sum over many tokens
+// averages (against 64 bits 2.6e-4 instead of 2.1e-4 with fp16 outputs, 1.67e-3 instead of 1.66e-3 with bf16; a second
+// term of P would take 204 us instead of 173 on the 16 trees, 258 instead of 212 on the 4).  Sums, maxima and O are fp32.  Q is scaled per row by a power of two before
 // its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
 // query is two such terms, whatever the output's type, the second from shared memory in the place of a third page of
 // the ring: an error of the scores is one of the weights, which no rounding of the output hides where values of both
