@@ -423,6 +423,7 @@ int rl_delta_gates(const float* a, const float* b, const float* A_log, const flo
  * all on the device.  A parent, count or leaf out of its range is recorded like bad pages and slots
  * (rl_device_error): the parent counts as -1, the count as 0, the leaf as -1.  The K and V rows of node i
  * lie at cache position base_len + i until the commit; its rotary position is base_len + its depth.
+ * Parameters are taken whole: a caller zeroes them first, and what it does not set is 0.
  * One verify round of a layer:
  *   rl_attn_qk_append -> rl_attn_tree -> (choose the leaf) -> rl_kv_tree_commit,   or
  *   rl_gdn_tree -> (choose the leaf) -> rl_gdn_tree_commit with the same inputs. */

@@ -470,3 +470,67 @@ def test_a_tree_on_the_device_cache():
     got = step(nxt, [x + len(path) for x in base])
     assert rel_l2(got[0].cpu(), want_next[0].cpu()) <= 1e-3 and rel_l2(got[1].cpu(), want_next[1].cpu()) <= STATE_REL_L2
     cache.close()
+
+
+def test_attn_tree_of_the_largest_batch():
+    """512 sequences, most of them short: every eighth against 64 bits; 513 are refused.  The same call again gives the same
+    bits; a tight bound of the lengths (another division of the work) the same values."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(54)
+    B, n, n_q, n_kv = 512, 5, 12, 2
+    base = [(b * 37) % 150 for b in range(B)]
+    base[100], base[511] = 3000, 1100
+    counts = [(b * 3) % (n + 1) for b in range(B)]
+    kp, vp, table, rows = _pages(gen, base, counts, n_kv, float("nan"))
+    parents, q = _tree(gen, B, n, 3), torch.randn(B, n, n_q, HD, generator=gen).half()
+    args = (q.cuda(), kp, vp, table, _i32(base), parents.cuda())
+    out = [torch.full((B, n, n_q, HD), 5.0, dtype=torch.float16, device="cuda") for _ in range(3)]
+    ops.attn_tree(*args, n_nodes=_i32(counts), out=out[0])
+    ops.attn_tree(*args, n_nodes=_i32(counts), out=out[1])
+    ops.attn_tree(*args, n_nodes=_i32(counts), out=out[2], max_seq_len=max(x + c for x, c in zip(base, counts)))
+    _lib.check_device()
+    assert torch.equal(out[0], out[1])
+    assert rel_l2(out[2].float().cpu(), out[0].float().cpu()) <= 2.0 ** -11
+    for b in [*range(0, B, 8), 100, 511]:
+        assert (out[0][b, counts[b]:] == 5.0).all()
+        if counts[b]:
+            o, _, _ = _attn_exact(q[b], None, rows[b], base[b], parents[b].tolist(), counts[b], n_q, n_kv)
+            assert rel_l2(out[0][b, :counts[b]].float().cpu(), o) <= 1e-3, b
+    with pytest.raises(_lib.RlError):
+        ops.attn_tree(torch.cat([args[0], args[0][:1]]), kp, vp, torch.cat([table, table[:1]]), _i32(base + [0]), None)
+
+
+def test_rounds_on_two_streams():
+    """Delta rule and commits of two groups of slots on streams of their own, round after round, give what one stream
+    gives."""
+    from rapidllm_b200 import _lib, ops
+    gen = torch.Generator().manual_seed(55)
+    n_v, n_qk, n, half = 6, 2, 11, 3
+    S, win, qkv, w, beta, g = (t.cuda() for t in _gdn_inputs(gen, 2 * half, n, n_v, n_qk, 2 * half))
+    parents, leaf, counts = _tree(gen, 2 * half, n, 3).cuda(), _i32([10, 4, -1, 0, 6, 3]), _i32([11, 5, 3, 1, 7, 4])
+    slots = _i32([4, 0, 2, 5, 1, 3])
+
+    def rounds(state, window, part):
+        cut = [t[part].contiguous() for t in (qkv, beta, g, parents, leaf, counts, slots)]
+        got = []
+        for _ in range(6):
+            got.append(ops.gdn_tree(state, window, None, cut[0], w, cut[1], cut[2], cut[3], n_qk, slot_ids=cut[6]))
+            ops.gdn_tree_commit(state, window, None, cut[0], w, cut[1], cut[2], cut[3], cut[4], n_qk, slot_ids=cut[6], n_nodes=cut[5])
+        return got
+
+    parts = [slice(0, half), slice(half, 2 * half)]
+    one = [S.clone(), win.clone()]
+    want = [rounds(*one, p) for p in parts]
+    two = [S.clone(), win.clone()]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in parts], []
+    for s, p in zip(streams, parts):
+        with torch.cuda.stream(s):
+            got.append(rounds(*two, p))
+    torch.cuda.synchronize()
+    _lib.check_device()
+    for a, b in zip(one, two):
+        assert torch.equal(a, b)
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
