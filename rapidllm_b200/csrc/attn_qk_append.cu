@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_qk_append_kernel(AttnQkAppen
     }
     __syncthreads();
     if (is_q || is_k) {
-        double ss = 0.0;                                      // as attn_qk_prepare sums (in 32 bits a prompt of 4 096 rows takes 74.1 us, so 75.6)
+        double ss = 0.0;                                      // as attn_qk_prepare sums (4 096 rows: 75.6 us, in 32 bits 74.1)
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fma(double(x.v[e]), double(x.v[e]), ss);
         const float inv = 1.f / sqrtf(float(sum_warp(ss) / kHeadDim) + a.eps);

@@ -21,18 +21,18 @@
 // the same way: here a lane has a row, whose gate it would read 16 bytes from a line at a time (all outputs written
 // by the merge: 1 x 8 nodes over 120 tokens 14.1 us against 20.2, 16 x 64 over 2000 123 against 146).
 //
-// Inside a segment: S = Q K^T (M 128, N 64) and O += P V (M 128, N 256) with Q, P, S and O in tensor memory
-// and the pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).
-// 16 softmax warps in two groups take alternate pages, so that one page's exponentials run under the
-// other's MMAs; the row maximum is handed from page to page and only raised by more than 2^8.  P is rounded
-// to fp16, as the cache's V is and as prefill and decode hold it: 2^-11 of a weight at most, which a sum over many tokens
-// averages (against 64 bits 2.6e-4 instead of 2.1e-4 with fp16 outputs, 1.67e-3 instead of 1.66e-3 with bf16; a second
-// term of P would take 204 us instead of 173 on the 16 trees, 258 instead of 212 on the 4).  Sums, maxima and O are fp32.  Q is scaled per row by a power of two before
-// its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An fp32
-// query is two such terms, whatever the output's type, the second from shared memory in the place of a third page of
-// the ring: an error of the scores is one of the weights, which no rounding of the output hides where values of both
-// signs all but cancel.  It costs a quarter of the time (16 trees of 21 over 16K: 180 us against 154 at burst clocks, 212
-// against 170 sustained), which a caller saves by asking rl_attn_qk_append for 16-bit queries.
+// Inside a segment: S = Q K^T (M 128, N 64) and O += P V (M 128, N 256) with Q, P, S and O in tensor memory and the
+// pages consumed as they lie in HBM (their slices are stored in the tensor cores' tile format).  16 softmax warps in
+// two groups take alternate pages, so that one page's exponentials run under the other's MMAs; the row maximum is
+// handed from page to page and only raised by more than 2^8.  P is rounded to fp16, as the cache's V is and as prefill
+// and decode hold it: 2^-11 of a weight at most, which a sum over many tokens averages (against 64 bits 2.6e-4 instead
+// of 2.1e-4 with fp16 outputs, 1.67e-3 instead of 1.66e-3 with bf16; a second term of P would take 204 us instead of
+// 173 on the 16 trees, 258 instead of 212 on the 4).  Sums, maxima and O are fp32.  Q is scaled per row by a power of
+// two before its rounding to fp16, so that no magnitude of a query overflows it; the score takes the scale back.  An
+// fp32 query is two such terms, whatever the output's type, the second from shared memory in the place of a third page
+// of the ring: an error of the scores is one of the weights, which no rounding of the output hides where values of
+// both signs all but cancel.  It costs a quarter of the time (16 trees of 21 over 16K: 180 us against 154 at burst
+// clocks, 212 against 170 sustained), which a caller saves by asking rl_attn_qk_append for 16-bit queries.
 // Positions past the committed rows are visible by a bit of the node's ancestor word; K columns that are
 // not are replaced, not added to, so that what an unused row of the last page holds cannot matter, and V
 // rows past the last node are cleared for the same reason.  A drafted V row that is not finite would reach the
